@@ -12,6 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libhelrm_b200.so")
 
 c_int, c_double, c_u64, c_size = ctypes.c_int, ctypes.c_double, ctypes.c_uint64, ctypes.c_size_t
+c_i64 = ctypes.c_int64
 P = ctypes.POINTER
 c_void = ctypes.c_void_p
 
@@ -127,6 +128,15 @@ SIGNATURES = {
     "helrm_kernel_rescale_noalloc": [c_void, c_void, c_int, c_int, c_void],
     "helrm_kernel_mac": [P(c_void), P(c_void), c_int, c_int, c_void, c_void],
     "helrm_kernel_rotate_hoisted": [c_void, c_int, c_int, P(c_int), c_int, c_void, c_void],
+    "helrm_GatedForward": [c_int] * 3 + [c_i64] * 3 + [c_void, c_i64] * 3 + [c_void, c_void, P(c_size), c_void],
+    "helrm_GatedBackward": [c_int] * 3 + [c_i64] * 3 + [c_void, c_i64] * 2 + [c_void] * 2 + [c_void, c_i64] * 2
+                           + [c_void] * 4 + [P(c_size), c_void],
+    "helrm_PackCheckpoint": [c_int] * 2 + [c_i64] * 2 + [c_void, c_i64] + [c_void] * 3,
+    "helrm_UnpackCheckpoint": [c_int] * 2 + [c_i64] * 2 + [c_void] * 4,
+    "helrm_VocabularyLossForward": [c_int] * 2 + [c_i64] * 3 + [c_void, c_i64] * 2 + [c_void, c_i64] + [c_void] * 3
+                                   + [P(c_size), c_void],
+    "helrm_VocabularyLossBackward": [c_int] * 2 + [c_i64] * 3 + [c_void] + [c_void, c_i64] * 2 + [c_void] * 2
+                                    + [c_i64] + [c_void] * 3 + [P(c_size), c_void],
     "helrm_Synchronize": [],
     "helrm_TimerStart": [],
     "helrm_TimerStop": [P(c_double)],

@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "../../include/helrm_b200.h"
+#include "hb_error.hpp"
 #include "hb_host.hpp"
 #include "hb_kernels.cuh"
 
@@ -43,19 +44,6 @@ static_assert(HB_LT_GIANT_GROUP >= 1 && HB_LT_GIANT_GROUP <= HB_MAX_GIANTS, "gia
 #endif
 
 namespace hb {
-
-struct HbError : std::runtime_error {
-    int code;
-    HbError(int c, const std::string &m) : std::runtime_error(m), code(c) {}
-};
-#define HB_THROW(code, msg) throw HbError(code, msg)
-
-static void cuda_check(cudaError_t e, const char *what) {
-    if (e != cudaSuccess) {
-        if (e == cudaErrorMemoryAllocation) HB_THROW(HB_ENOMEM, std::string(what) + ": out of device memory");
-        HB_THROW(HB_ECUDA, std::string(what) + ": " + cudaGetErrorString(e));
-    }
-}
 
 enum : u64 {
     DOM_SK_POS = 1, DOM_SK_SIGN = 2, DOM_ENC_A = 3, DOM_ENC_E = 4,
@@ -1929,7 +1917,15 @@ public:
 };
 
 static std::unique_ptr<Context> g_ctx;
-static std::string g_err;
+
+// The last failure's message: a plain buffer, since a training call on
+// another thread may fail while the caller reads it.
+static char g_err[1024];
+void set_last_error(const char *msg) {
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lk(mu);
+    std::strncpy(g_err, msg, sizeof(g_err) - 1);
+}
 
 static Context &C() {
     if (!g_ctx) HB_THROW(HB_ESTATE, "B200 backend not initialised. Call NewScheme first.");
@@ -1940,35 +1936,10 @@ static Context &C() {
 
 using namespace hb;
 
-#define HB_API extern "C" __attribute__((visibility("default")))
-
-template <class F>
-static int guard(F &&f) {
-    try {
-        f();
-        return HB_OK;
-    } catch (const HbError &e) {
-        g_err = e.what();
-        return e.code;
-    } catch (const std::invalid_argument &e) {
-        g_err = e.what();
-        return HB_EINVAL;
-    } catch (const std::out_of_range &e) {
-        g_err = e.what();
-        return HB_ENOENT;
-    } catch (const std::bad_alloc &e) {
-        g_err = "host allocation failed";
-        return HB_ENOMEM;
-    } catch (const std::exception &e) {
-        g_err = e.what();
-        return HB_ECUDA;
-    }
-}
-
 #define OUT(p) \
     if (!(p)) HB_THROW(HB_EINVAL, "null output pointer")
 
-HB_API const char *helrm_LastError(void) { return g_err.c_str(); }
+HB_API const char *helrm_LastError(void) { return g_err; }
 
 HB_API int helrm_NewScheme(int logn, const int *logq, int nlogq, const int *logp, int nlogp, int logscale,
                            int hamming_weight, int dnum, uint64_t seed, int device) {

@@ -7,6 +7,7 @@
 // descriptors) is staged in shared memory; everything else streams with
 // 16-byte vector accesses.
 #include <cooperative_groups.h>
+#include <atomic>
 #include <cstdio>
 #include <cstdlib>
 #include <stdexcept>
@@ -58,7 +59,7 @@ static bool primes_sized(int p0, int n, bool below) {
 // read or written once) and integer work (modular products, or NTT
 // butterflies).  prof_collect() resolves the events.
 // =====================================================================
-static unsigned long long g_launches = 0;
+static std::atomic<unsigned long long> g_launches{0};  // training calls count from their own threads
 static bool g_prof_on = false;
 struct ProfRec {
     cudaEvent_t a, b;
@@ -107,6 +108,7 @@ static const char *kClassNames[KC_COUNT] = {
 
 const char *kclass_name(int c) { return (c >= 0 && c < KC_COUNT) ? kClassNames[c] : ""; }
 unsigned long long launch_count() { return g_launches; }
+void count_launches(int n) { g_launches += (unsigned long long)n; }
 
 void prof_collect(ProfStats *out) {
     for (auto &r : g_pending) {

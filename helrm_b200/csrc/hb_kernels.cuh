@@ -70,6 +70,7 @@ void prof_enable(bool on);             // resets the statistics
 void prof_collect(ProfStats *out);     // waits for the recorded events
 const char *kclass_name(int c);
 unsigned long long launch_count();     // kernels launched since load
+void count_launches(int n);            // adds launches made outside hb_kernels.cu
 
 // ---- NTT -----------------------------------------------------------------
 void ntt_forward(u64 *data, int nrows, RowMap map, const NttTables &t, cudaStream_t s);

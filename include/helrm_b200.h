@@ -328,6 +328,73 @@ int helrm_kernel_rescale_noalloc(const uint64_t *d_in, uint64_t *d_out, int nq, 
 /* synchronise the library stream */
 int helrm_Synchronize(void);
 
+/* ---- training operators (no reference counterpart; the reference loads
+ * weights trained elsewhere) -------------------------------------------------
+ * The operators that train, in the clear, the weights the encrypted forward
+ * evaluates.  They need no scheme.  Conventions:
+ *   - device pointers on `device`; work is enqueued on `stream` (NULL: the
+ *     device's default stream), nothing synchronises, and no call allocates
+ *     device memory;
+ *   - 16-bit floats of one type per call (HELRM_FP16 / HELRM_BF16); sums,
+ *     softmax statistics and losses in 32 bits; a matrix is row-major with
+ *     unit column stride and a row pitch `ld*` in elements (>= its columns)
+ *     for inputs, outputs are dense; no output may overlap an input;
+ *   - calls with `ws`, `ws_bytes`: with ws NULL nothing runs and *ws_bytes
+ *     receives the bytes of workspace these arguments need (0 or more);
+ *     otherwise ws points to *ws_bytes of it, 256-byte aligned.  It holds
+ *     nothing between calls; calls whose GPU work overlaps need one each;
+ *   - tokens may be 0 (weight gradients are then zero), other sizes are >= 1;
+ *     a call whose kernel gave up waiting (a hardware failure) makes the next
+ *     training call on any stream return HB_ECUDA. */
+#define HELRM_FP16 0
+#define HELRM_BF16 1
+#define HELRM_ACT_IDENTITY 0
+#define HELRM_ACT_RELU 1
+#define HELRM_ACT_SILU 2
+#define HELRM_ACT_GELU 3   /* x Phi(x), Phi the normal distribution function */
+#define HELRM_CKPT_GROUP 32
+/* h[tokens][width] = act(x wg^T) * (x wu^T), x [tokens][inner], wg and wu
+ * [width][inner]. */
+int helrm_GatedForward(int device, int dtype, int act, int64_t tokens, int64_t inner, int64_t width, const void *x,
+                       int64_t ldx, const void *wg, int64_t ldg, const void *wu, int64_t ldu, void *h, void *ws,
+                       size_t *ws_bytes, void *stream);
+/* The gradients dx [tokens][inner], dwg and dwu [width][inner] of a loss
+ * whose gradient by h is dh [tokens][width].  The projections are formed
+ * again from x, or, with x NULL, from its 8-bit checkpoint (q, e).  An output
+ * that is NULL is not computed. */
+int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, int64_t inner, int64_t width, const void *dh,
+                        int64_t lddh, const void *x, int64_t ldx, const int8_t *q, const uint8_t *e, const void *wg,
+                        int64_t ldg, const void *wu, int64_t ldu, void *dx, void *dwg, void *dwu, void *ws,
+                        size_t *ws_bytes, void *stream);
+/* The 8-bit checkpoint of x [tokens][inner].  Groups of 32 consecutive
+ * features of a row (the last group of a row may be shorter) share the least
+ * power of two s = 2^(e-127) >= 2^-126 (fp16: >= 2^-24) with max |x| <= 127 s;
+ * q holds x / s rounded to the nearest integer, halves to even, and limited to
+ * what the type holds as q s.  A group with an infinity or a NaN has e = 255
+ * and reads back as NaN.  q s is exact in the 16-bit type.
+ * q [tokens][32 G], e [tokens][G], G = ceil(inner / 32); q is zero past inner
+ * and 16-byte aligned. */
+int helrm_PackCheckpoint(int device, int dtype, int64_t tokens, int64_t inner, const void *x, int64_t ldx, int8_t *q,
+                         uint8_t *e, void *stream);
+int helrm_UnpackCheckpoint(int device, int dtype, int64_t tokens, int64_t inner, const int8_t *q, const uint8_t *e,
+                           void *x, void *stream);
+/* loss[i] = lse_i - h_i . w_t(i), lse_i = log sum_j exp(h_i . w_j) over the
+ * vocab rows of w [vocab][inner]; h [tokens][inner], int64 targets.  A target
+ * equal to ignore_index has loss 0; any other one outside [0, vocab) has
+ * loss NaN.  lse [tokens][2] holds lse_i as a sum: the row's largest logit and
+ * the log of the sum of exponentials relative to it. */
+int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, int64_t inner, int64_t vocab, const void *h,
+                                int64_t ldh, const void *w, int64_t ldw, const int64_t *targets, int64_t ignore_index,
+                                float *loss, float *lse, void *ws, size_t *ws_bytes, void *stream);
+/* dh [tokens][inner] and dw [vocab][inner] from dloss [tokens] and the
+ * forward call's lse.  The vocabulary is taken in pieces, whose logits are
+ * formed again; ignored rows take no part, rows with a target out of range
+ * give NaN.  An output that is NULL is not computed. */
+int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, int64_t inner, int64_t vocab,
+                                 const float *dloss, const void *h, int64_t ldh, const void *w, int64_t ldw,
+                                 const int64_t *targets, const float *lse, int64_t ignore_index, void *dh, void *dw,
+                                 void *ws, size_t *ws_bytes, void *stream);
+
 /* ---- measurement (no reference counterpart; the reference times with
  * torch.cuda.synchronize + wall clock, examples/criteo/bench_sweep.py:192-222) -- */
 /* CUDA events on the library stream around a region of work. */
