@@ -45,6 +45,7 @@
 // own copies and MMAs (bounded) and release its TMEM.
 // Included by hb_kernels.cu (it reads the per-prime __constant__ table).
 #pragma once
+#include "hb_ptx.cuh"
 
 namespace hb {
 
@@ -72,8 +73,6 @@ static_assert(kTcABuf % 16 == 0 && kTcBBuf % 1024 == 0, "smem alignment");
 
 namespace tc {
 
-__device__ __forceinline__ unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-
 // byte offset of (row, k) in a K-major tile of 32-byte rows without swizzle:
 // core matrices of 8 rows x 16 bytes, the two K halves 128 B apart (LBO),
 // 8-row groups 256 B apart (SBO)
@@ -88,46 +87,6 @@ __device__ __forceinline__ uint64_t sdesc(unsigned saddr) {
 // instruction descriptor: s32 accumulator, u8 x u8, both K-major, N = 144, M = 64
 constexpr unsigned kIdesc = (2u << 4) | ((unsigned)(kTcN >> 3) << 17) | ((64u >> 4) << 24);
 
-__device__ __forceinline__ void mbar_init(unsigned a, unsigned count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(a), "r"(count));
-}
-__device__ __forceinline__ void mbar_arrive(unsigned a) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_tx(unsigned a, unsigned bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(a), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_try(unsigned a, unsigned parity) {
-    unsigned ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(ok)
-        : "r"(a), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ unsigned long long gtimer() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-// Bounded wait for the given phase parity.  Gives up after `limit_ns`, or
-// at once when another thread of the CTA has given up (*abort set, unless
-// abort is null); returns false then, after recording `code` in *err.
-__device__ __forceinline__ bool mbar_wait(unsigned a, unsigned parity, volatile int *abort, int *err, int code,
-                                          unsigned long long limit_ns) {
-    if (mbar_try(a, parity)) return true;
-    const unsigned long long t0 = gtimer();
-    for (unsigned it = 1;; it++) {
-        if (mbar_try(a, parity)) return true;
-        if (abort && *abort) return false;
-        if ((it & 63) == 0 && gtimer() - t0 > limit_ns) {
-            if (abort) *abort = 1;
-            atomicOr(err, code);
-            return false;
-        }
-    }
-}
 __device__ __forceinline__ void bulk_g2s(unsigned dst, const void *src, unsigned bytes, unsigned mbar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                  "l"(src), "r"(bytes), "r"(mbar)
@@ -153,9 +112,6 @@ __device__ __forceinline__ void tmem_ld4(unsigned taddr, unsigned (&v)[4]) {
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                  : "r"(taddr));
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void named_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

@@ -1,10 +1,14 @@
 // hb_train.cu -- the training operators' launches and their extern "C"
 // entry points (include/helrm_b200.h).
+#include <atomic>
+#include <mutex>
 #include <type_traits>
+#include <vector>
 
 #include "hb_error.hpp"
 #include "hb_kernels.cuh"
 #include "hb_train.cuh"
+#include "hb_train_mma.cuh"
 
 namespace hb {
 namespace train {
@@ -74,12 +78,175 @@ static void check_matrix(const void *p, int64_t ld, int64_t cols, int64_t rows) 
     require(ld >= cols, "a row pitch is below the number of columns");
 }
 
-template <class T, int EPI, int ACT, bool DUAL, bool SECOND>
-static void product(View a, View b, View a1, View b1, int64_t M, int64_t N, int64_t K, const EpiArgs &e,
-                    cudaStream_t s) {
-    const dim3 grid(blocks(M, kTile), blocks(N, kTile));
-    k_product<T, EPI, ACT, DUAL, SECOND><<<grid, 256, 0, s>>>(a, b, a1, b1, M, N, K, e);
+// ---- the process's state: a word of host memory that a kernel whose wait
+// ran out writes, and the driver's tensor-map encoder
+struct Runtime {
+    int *error = nullptr;
+    decltype(&cuTensorMapEncodeTiled) encode = nullptr;
+    int sms[64] = {};
+};
+static Runtime &runtime() {
+    static Runtime r;
+    static std::mutex mu;
+    static std::atomic<bool> ready{false};
+    if (!ready) {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!ready) {
+            // allowed while another thread or this one captures a graph
+            cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+            cuda_check(cudaThreadExchangeStreamCaptureMode(&mode), "capture mode");
+            void *fn = nullptr;
+            cudaDriverEntryPointQueryResult found;
+            cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+            if (e == cudaSuccess && !r.error) {
+                e = cudaHostAlloc(reinterpret_cast<void **>(&r.error), sizeof(int), cudaHostAllocPortable);
+                if (e == cudaSuccess) *r.error = 0;
+            }
+            cudaThreadExchangeStreamCaptureMode(&mode);
+            cuda_check(e, "training set-up");
+            if (!fn || found != cudaDriverEntryPointSuccess) HB_THROW(HB_ECUDA, "the driver has no tensor maps");
+            r.encode = reinterpret_cast<decltype(&cuTensorMapEncodeTiled)>(fn);
+            ready = true;
+        }
+    }
+    if (const int code = *static_cast<volatile int *>(r.error)) {
+        *static_cast<volatile int *>(r.error) = 0;
+        HB_THROW(HB_ECUDA, "an earlier training call gave up waiting in its kernel (code " + std::to_string(code) +
+                               "): its results are not valid");
+    }
+    return r;
+}
+static int sm_count() {
+    int dev = 0;
+    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    int &n = runtime().sms[dev & 63];
+    if (!n) cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+    return n;
+}
+
+// A row-major 16-bit matrix.
+struct Matrix {
+    const void *p = nullptr;
+    int64_t rows = 0, cols = 0, ld = 0;
+};
+static int64_t pitch(int64_t cols) { return pad(cols, 8); }
+static bool fits_vectors(const void *p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
+
+// Operands that the TMA unit can read: what lies on 16-byte boundaries as it
+// is, anything else copied into the workspace first.
+struct Operands {
+    Workspace &w;
+    struct Copy {
+        Matrix from;
+        unsigned short *to;
+    };
+    std::vector<Copy> copies;
+    explicit Operands(Workspace &ws) : w(ws) {}
+    Matrix fit(Matrix m) {
+        if (m.rows <= 1) m.ld = pitch(m.cols);
+        if (fits_vectors(m.p, m.ld)) return m;
+        const int64_t ld = pitch(m.cols);
+        unsigned short *to = w.take<unsigned short>(m.rows * ld);
+        copies.push_back({m, to});
+        return {to, m.rows, m.cols, ld};
+    }
+    void copy(cudaStream_t s) const {
+        for (const Copy &c : copies) {
+            const int64_t ld = pitch(c.from.cols);
+            k_repitch<<<blocks(c.from.rows * ld, 256), 256, 0, s>>>(static_cast<const unsigned short *>(c.from.p),
+                                                                    c.from.ld, c.from.rows, c.from.cols, c.to, ld);
+            launched("copy to aligned rows");
+        }
+    }
+};
+
+static CUtensorMap tensor_map(const Matrix &m, bool bf16, int major) {
+    CUtensorMap map;
+    const cuuint64_t dims[2] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)m.ld * 2};
+    const cuuint32_t box[2] = {64, major == K_MAJOR ? 128u : 64u}, steps[2] = {1, 1};
+    const CUresult r = runtime().encode(
+        &map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(m.p),
+        dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) HB_THROW(HB_EINVAL, "no tensor map for a matrix (" + std::to_string((int)r) + ")");
+    return map;
+}
+
+// One product launch.  a, b (and a1, b1 where used) lie K-major or MN-major:
+// a K-major operand has the product's depth in its columns, an MN-major one in
+// its rows.
+struct Product {
+    Matrix a, b, a1, b1;
+    int64_t M = 0, N = 0, K = 0, K1 = 0;
+    int outputs = 1, splits = 1;
+    EpiArgs e;
+};
+template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
+static void launch(const Product &d, cudaStream_t s) {
+    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    constexpr bool dual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+    ProductArgs p;
+    p.a = tensor_map(d.a, bf16, AMAJ);
+    p.b = tensor_map(d.b, bf16, BMAJ);
+    p.a1 = d.a1.p ? tensor_map(d.a1, bf16, AMAJ) : p.a;
+    p.b1 = d.b1.p ? tensor_map(d.b1, bf16, BMAJ) : p.b;
+    p.M = d.M;
+    p.N = d.N;
+    p.tiles_m = (int)blocks(d.M, kRows);
+    p.tiles_n = (int)blocks(d.N, dual ? 128 : kCols);
+    p.outputs = d.outputs;
+    p.splits = d.splits;
+    p.kb = (int)blocks(d.K, kDepth);
+    p.kb1 = (int)blocks(d.K1, kDepth);
+    p.e = d.e;
+    p.error = runtime().error;
+    static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised for this kernel
+    int dev = 0;
+    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    auto kernel = k_mma_product<T, AMAJ, BMAJ, EPI, ACT>;
+    if (!(set >> (dev & 63) & 1)) {
+        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "shared memory");
+        set |= (uint64_t)1 << (dev & 63);
+    }
+    const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
+    kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), kThreads, kSmem, s>>>(p);
     launched("training product");
+}
+
+// Parts of the depth for a product of few tiles: enough to give every SM pair
+// one, each at least 4 slices deep.
+static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
+    const int64_t tiles = (int64_t)blocks(M, kRows) * blocks(N, kCols) * outputs, slices = blocks(depth, kDepth);
+    const int64_t n = 74 / tiles < slices / 4 ? 74 / tiles : slices / 4;
+    return n > 1 ? (int)n : 1;
+}
+template <class T>
+static void join(const float *acc, int parts, int64_t M, int64_t N, int64_t ld, const int *shift, void *out,
+                 cudaStream_t s) {
+    k_join<T><<<blocks(M * (ld / 4), 256), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out), N);
+    launched("join parts");
+}
+// D = A B^T (+ A1 B1^T), or with outputs = 2 also A1 B^T, as dense 16-bit rows
+// at out[0], out[1]; the sums of a split depth are joined in acc.
+template <class T, int AMAJ, int BMAJ>
+static void product_out(Product d, void *const *out, float *acc, cudaStream_t s) {
+    if (d.splits == 1) {
+        d.e.o0 = out[0];
+        d.e.o1 = d.outputs > 1 ? out[1] : nullptr;
+        d.e.ldo = d.N;
+        d.e.vec = fits_vectors(out[0], d.N) && (d.outputs == 1 || fits_vectors(out[1], d.N));
+        launch<T, AMAJ, BMAJ, EPI_STORE, 0>(d, s);
+        return;
+    }
+    d.e.acc = acc;
+    d.e.ldo = pad(d.N, 4);
+    launch<T, AMAJ, BMAJ, EPI_SUM, 0>(d, s);
+    for (int i = 0; i < d.outputs; i++)
+        join<T>(acc + (int64_t)i * d.splits * d.M * d.e.ldo, d.splits, d.M, d.N, d.e.ldo, d.e.shift, out[i], s);
+}
+static int64_t sums(int64_t M, int64_t N, int splits, int outputs) {
+    return splits > 1 ? (int64_t)outputs * splits * M * pad(N, 4) : 0;
 }
 
 template <class F>
@@ -124,17 +291,21 @@ HB_API int helrm_GatedForward(int device, int dtype, int act, int64_t tokens, in
         require(tokens == 0 || h != nullptr, "the output pointer is NULL");
         require(act >= 0 && act <= HELRM_ACT_GELU, "unknown activation");
         Workspace w{static_cast<char *>(ws)};
+        Operands in(w);
+        Product d;
+        d.a = in.fit({x, tokens, inner, ldx});
+        d.b = in.fit({wg, width, inner, ldg});
+        d.b1 = in.fit({wu, width, inner, ldu});
         if (sized(w, ws_bytes) || tokens == 0) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
+        in.copy(s);
+        d.M = tokens, d.N = width, d.K = inner;
+        d.e.o0 = h;
+        d.e.ldo = width;
+        d.e.vec = fits_vectors(h, width);
         by_dtype(dtype, [&](auto t) {
-            by_act(act, [&](auto a) {
-                EpiArgs e;
-                e.o0 = h;
-                e.ldo = width;
-                product<decltype(t), EPI_GATED, decltype(a)::value, true, false>(
-                    {x, ldx, 1}, {wg, ldg, 1}, {}, {wu, ldu, 1}, tokens, width, inner, e, s);
-            });
+            by_act(act, [&](auto a) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_GATED, decltype(a)::value>(d, s); });
         });
     });
 }
@@ -155,9 +326,18 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
         require(dx || dwg || dwu, "no output is asked for");
         require(act >= 0 && act <= HELRM_ACT_GELU, "unknown activation");
         Workspace w{static_cast<char *>(ws)};
-        const int64_t ldd = pad(width, 8), ldk = pad(inner, 8);
+        Operands in(w);
+        const int64_t ldd = pitch(width);
         uint16_t *dg = w.take<uint16_t>(tokens * ldd), *du = w.take<uint16_t>(tokens * ldd);
-        uint16_t *xr = x ? nullptr : w.take<uint16_t>(tokens * ldk);
+        uint16_t *read = x ? nullptr : w.take<uint16_t>(tokens * pitch(inner));
+        const Matrix mx = x ? in.fit({x, tokens, inner, ldx}) : Matrix{read, tokens, inner, pitch(inner)};
+        const Matrix mg = in.fit({wg, width, inner, ldg}), mu = in.fit({wu, width, inner, ldu});
+        const Matrix mdg{dg, tokens, width, ldd}, mdu{du, tokens, width, ldd};
+        const int both = dwg && dwu ? 2 : 1;
+        const int parts_x = dx ? parts_for(tokens, inner, 2 * width, 1) : 1;
+        const int parts_w = dwg || dwu ? parts_for(width, inner, tokens, both) : 1;
+        const int64_t sums_x = sums(tokens, inner, parts_x, 1), sums_w = sums(width, inner, parts_w, both);
+        float *acc = w.take<float>(sums_x > sums_w ? sums_x : sums_w);
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
@@ -166,39 +346,40 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
                 if (p) cuda_check(cudaMemsetAsync(p, 0, (size_t)width * inner * 2, s), "zero gradient");
             return;
         }
+        in.copy(s);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
-            const void *xp = x;
-            int64_t lx = ldx;
             if (!x) {
-                k_unpack<T><<<blocks(tokens * inner, 256), 256, 0, s>>>(q, ex, tokens, inner, reinterpret_cast<T *>(xr),
-                                                                        ldk);
+                k_unpack<T><<<blocks(tokens * inner, 256), 256, 0, s>>>(q, ex, tokens, inner,
+                                                                        reinterpret_cast<T *>(read), pitch(inner));
                 launched("read checkpoint");
-                xp = xr;
-                lx = ldk;
             }
-            by_act(act, [&](auto a) {
-                EpiArgs e;
-                e.o0 = dg;
-                e.o1 = du;
-                e.ldo = ldd;
-                e.dh = dh;
-                e.lddh = lddh;
-                product<T, EPI_GATED_BWD, decltype(a)::value, true, false>({xp, lx, 1}, {wg, ldg, 1}, {}, {wu, ldu, 1},
-                                                                           tokens, width, inner, e, s);
-            });
-            EpiArgs e;
-            e.ldo = inner;
-            e.o0 = dx;
-            if (dx)
-                product<T, EPI_STORE, 0, false, true>({dg, ldd, 1}, {wg, 1, ldg}, {du, ldd, 1}, {wu, 1, ldu}, tokens,
-                                                      inner, width, e, s);
-            e.o0 = dwg;
-            if (dwg)
-                product<T, EPI_STORE, 0, false, false>({dg, 1, ldd}, {xp, 1, lx}, {}, {}, width, inner, tokens, e, s);
-            e.o0 = dwu;
-            if (dwu)
-                product<T, EPI_STORE, 0, false, false>({du, 1, ldd}, {xp, 1, lx}, {}, {}, width, inner, tokens, e, s);
+            Product d;
+            d.a = mx, d.b = mg, d.b1 = mu;
+            d.M = tokens, d.N = width, d.K = inner;
+            d.e.o0 = dg;
+            d.e.o1 = du;
+            d.e.ldo = ldd;
+            d.e.dh = dh;
+            d.e.lddh = lddh;
+            d.e.vec = 1 | (fits_vectors(dh, lddh) ? 2 : 0);
+            by_act(act, [&](auto a) { launch<T, K_MAJOR, K_MAJOR, EPI_GATED_BWD, decltype(a)::value>(d, s); });
+            if (dx) {
+                Product g;
+                g.a = mdg, g.b = mg, g.a1 = mdu, g.b1 = mu;
+                g.M = tokens, g.N = inner, g.K = g.K1 = width;
+                g.splits = parts_x;
+                product_out<T, K_MAJOR, MN_MAJOR>(g, &dx, acc, s);
+            }
+            if (dwg || dwu) {
+                Product g;
+                g.a = dwg ? mdg : mdu, g.a1 = mdu, g.b = mx;
+                g.M = width, g.N = inner, g.K = tokens;
+                g.outputs = both;
+                g.splits = parts_w;
+                void *out[2] = {dwg ? dwg : dwu, dwu};
+                product_out<T, MN_MAJOR, MN_MAJOR>(g, out, acc, s);
+            }
         });
     });
 }
@@ -248,22 +429,24 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         require(tokens == 0 || (targets && loss && lse), "targets, loss or lse is NULL");
         require(((uintptr_t)lse & 7) == 0, "lse is not 8-byte aligned");
         Workspace w{static_cast<char *>(ws)};
-        const int64_t tiles = blocks(vocab, kTile);
-        float2 *part = w.take<float2>(tiles * tokens);
+        Operands in(w);
+        Product d;
+        d.a = in.fit({h, tokens, inner, ldh});
+        d.b = in.fit({wt, vocab, inner, ldw});
+        const int64_t parts = 2 * (int64_t)blocks(vocab, kCols);
+        float2 *part = w.take<float2>(parts * tokens);
         float *at = w.take<float>(tokens);
         if (sized(w, ws_bytes) || tokens == 0) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
-        by_dtype(dtype, [&](auto t) {
-            EpiArgs e;
-            e.part = part;
-            e.at = at;
-            e.target = targets;
-            product<decltype(t), EPI_LSE, 0, false, false>({h, ldh, 1}, {wt, ldw, 1}, {}, {}, tokens, vocab, inner, e,
-                                                           s);
-        });
-        k_loss<<<blocks(tokens, 128), 128, 0, s>>>(part, tiles, at, targets, ignore_index, vocab, tokens, loss,
-                                                     reinterpret_cast<float2 *>(lse));
+        in.copy(s);
+        d.M = tokens, d.N = vocab, d.K = inner;
+        d.e.part = part;
+        d.e.at = at;
+        d.e.target = targets;
+        by_dtype(dtype, [&](auto t) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_LSE, 0>(d, s); });
+        k_loss<<<blocks(tokens, 32), 1024, 0, s>>>(part, parts, at, targets, ignore_index, vocab, tokens, loss,
+                                                   reinterpret_cast<float2 *>(lse));
         launched("loss");
     });
 }
@@ -280,9 +463,15 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         require(((uintptr_t)lse & 7) == 0, "lse is not 8-byte aligned");
         require(dh || dw, "no output is asked for");
         Workspace w{static_cast<char *>(ws)};
-        const int64_t cols = piece_columns(tokens, vocab), ldz = pad(cols, 8);
+        Operands in(w);
+        const Matrix mh = in.fit({h, tokens, inner, ldh}), mw = in.fit({wt, vocab, inner, ldw});
+        const int64_t cols = piece_columns(tokens, vocab), ldz = pitch(cols), lda = pad(inner, 4);
         uint16_t *z = w.take<uint16_t>(tokens * ldz);
-        float *acc = w.take<float>(cols < vocab ? tokens * inner : 0);
+        // dh over several pieces is a 32-bit sum; the parts of a piece's depth each keep their own
+        const int parts_h = dh ? parts_for(tokens, inner, cols, 1) : 1, parts_w = dw ? parts_for(cols, inner, tokens, 1) : 1;
+        const bool summed = dh && (cols < vocab || parts_h > 1);
+        float *acc = w.take<float>(summed ? parts_h * tokens * lda : 0);
+        float *acc_w = w.take<float>(sums(cols, inner, parts_w, 1));
         int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
@@ -291,6 +480,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
             return;
         }
+        in.copy(s);
         const bool scaled = dtype == HELRM_FP16;
         if (scaled) {
             k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
@@ -300,29 +490,48 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             typedef decltype(t) T;
             for (int64_t c0 = 0; c0 < vocab; c0 += cols) {
                 const int64_t n = vocab - c0 < cols ? vocab - c0 : cols;
-                const T *wc = static_cast<const T *>(wt) + c0 * ldw;
-                EpiArgs e;
-                e.shift = scaled ? shift : nullptr;
-                e.o0 = z;
-                e.ldo = ldz;
-                e.target = targets;
-                e.lse = reinterpret_cast<const float2 *>(lse);
-                e.dloss = dloss;
-                e.ignore = ignore_index;
-                e.col0 = c0;
-                e.vocab = vocab;
-                product<T, EPI_Z, 0, false, false>({h, ldh, 1}, {wc, ldw, 1}, {}, {}, tokens, n, inner, e, s);
-                e.ldo = inner;
-                e.o0 = static_cast<T *>(dw) + c0 * inner;
-                if (dw)
-                    product<T, EPI_STORE, 0, false, false>({z, 1, ldz}, {h, 1, ldh}, {}, {}, n, inner, tokens, e, s);
-                if (!dh) continue;
-                e.o0 = dh;
-                e.acc = acc;
-                e.first = c0 == 0;
-                e.last = c0 + n == vocab;
-                product<T, EPI_STORE, 0, false, false>({z, ldz, 1}, {wc, 1, ldw}, {}, {}, tokens, inner, n, e, s);
+                const Matrix mc{static_cast<const T *>(mw.p) + c0 * mw.ld, n, inner, mw.ld}, mz{z, tokens, n, ldz};
+                Product d;
+                d.a = mh, d.b = mc;
+                d.M = tokens, d.N = n, d.K = inner;
+                d.e.shift = scaled ? shift : nullptr;
+                d.e.o0 = z;
+                d.e.ldo = ldz;
+                d.e.vec = 1;
+                d.e.target = targets;
+                d.e.lse = reinterpret_cast<const float2 *>(lse);
+                d.e.dloss = dloss;
+                d.e.ignore = ignore_index;
+                d.e.col0 = c0;
+                d.e.vocab = vocab;
+                launch<T, K_MAJOR, K_MAJOR, EPI_Z, 0>(d, s);
+                if (dw) {
+                    Product g;
+                    g.a = mz, g.b = mh;
+                    g.M = n, g.N = inner, g.K = tokens;
+                    g.splits = parts_w;
+                    g.e.shift = scaled ? shift : nullptr;
+                    void *out = static_cast<T *>(dw) + c0 * inner;
+                    product_out<T, MN_MAJOR, MN_MAJOR>(g, &out, acc_w, s);
+                }
+                if (dh) {
+                    Product g;
+                    g.a = mz, g.b = mc;
+                    g.M = tokens, g.N = inner, g.K = n;
+                    g.e.shift = scaled ? shift : nullptr;
+                    if (summed) {
+                        // the last piece may be too short for every part: those keep their sums
+                        g.splits = parts_h < (int)blocks(n, kDepth) ? parts_h : (int)blocks(n, kDepth);
+                        g.e.acc = acc;
+                        g.e.ldo = lda;
+                        g.e.first = c0 == 0;
+                        launch<T, K_MAJOR, MN_MAJOR, EPI_SUM, 0>(g, s);
+                    } else {
+                        product_out<T, K_MAJOR, MN_MAJOR>(g, &dh, nullptr, s);
+                    }
+                }
             }
+            if (summed) join<T>(acc, parts_h, tokens, inner, lda, scaled ? shift : nullptr, dh, s);
         });
     });
 }

@@ -57,167 +57,52 @@ __device__ __forceinline__ void act_df(float g, float &a, float &d) {
 }
 
 // ---------------------------------------------------------------- products
-// A strided operand: element (r, k) at p[r * sr + k * sk].
-struct View {
-    const void *p;
-    int64_t sr, sk;
-};
-enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_STORE, EPI_LSE, EPI_Z };
+enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_STORE, EPI_SUM, EPI_LSE, EPI_Z };
 struct EpiArgs {
-    void *o0 = nullptr, *o1 = nullptr;  // outputs, dense rows of ldo
-    int64_t ldo = 0;
+    void *o0 = nullptr, *o1 = nullptr;  // 16-bit outputs
+    int64_t ldo = 0;                    // their row pitch, or that of acc
+    int vec = 0;                        // 1: outputs fit 16-byte stores, 2: dh fits 16-byte loads
     const void *dh = nullptr;
     int64_t lddh = 0;
-    float *acc = nullptr;               // EPI_STORE: 32-bit running sum over the pieces
-    int first = 1, last = 1;
-    float2 *part = nullptr;             // EPI_LSE: (max, sum) of each [tile][row]
+    float *acc = nullptr;               // EPI_SUM: 32-bit sums, [output][part][row][ldo]
+    int first = 1;                      // 0: added to what acc holds
+    float2 *part = nullptr;             // EPI_LSE: (max, sum) of each [half tile][row]
     float *at = nullptr;                // EPI_LSE: the target's logit
     const int64_t *target = nullptr;
     const float2 *lse = nullptr;        // EPI_Z: the row's (maximum, log of the sum relative to it)
     const float *dloss = nullptr;
     int64_t ignore = 0, col0 = 0;       // first column of the piece in the vocabulary of
     int64_t vocab = 0;                  // this many
-    const int *shift = nullptr;         // Z is scaled by 2^shift, undone in EPI_STORE
+    const int *shift = nullptr;         // Z is scaled by 2^shift, undone when the products with it are stored
 };
-
-constexpr int kTile = 64, kStep = 16;
-
-// D[m][n] = sum_k A(m, k) B(n, k) over one 64 x 64 tile, 4 x 4 a thread, the
-// operands staged as 32-bit floats.  DUAL: a second product with B1.  SECOND:
-// a second pair of operands added to the same sum.
-template <class T, int EPI, int ACT, bool DUAL, bool SECOND>
-__global__ void __launch_bounds__(256) k_product(View a, View b, View a1, View b1, int64_t M, int64_t N, int64_t K,
-                                                 EpiArgs e) {
-    __shared__ float sa[kStep][kTile + 4], sb[kStep][kTile + 4], sc[DUAL ? kStep : 1][kTile + 4];
-    __shared__ float red[EPI == EPI_LSE ? kTile : 1][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile;
-    float acc[4][4] = {}, acc1[4][4] = {};
-    for (int pass = 0; pass < (SECOND ? 2 : 1); pass++) {
-        const View va = pass ? a1 : a, vb = pass ? b1 : b;
-        for (int64_t k0 = 0; k0 < K; k0 += kStep) {
-            for (int i = threadIdx.x; i < kTile * kStep; i += 256) {
-                const bool ka = va.sk == 1, kb = vb.sk == 1;
-                const int ra = ka ? i / kStep : i % kTile, ca = ka ? i % kStep : i / kTile;
-                const int rb = kb ? i / kStep : i % kTile, cb = kb ? i % kStep : i / kTile;
-                sa[ca][ra] = m0 + ra < M && k0 + ca < K
-                                 ? to_f(static_cast<const T *>(va.p)[(m0 + ra) * va.sr + (k0 + ca) * va.sk])
-                                 : 0.0f;
-                sb[cb][rb] = n0 + rb < N && k0 + cb < K
-                                 ? to_f(static_cast<const T *>(vb.p)[(n0 + rb) * vb.sr + (k0 + cb) * vb.sk])
-                                 : 0.0f;
-                if (DUAL)
-                    sc[cb][rb] = n0 + rb < N && k0 + cb < K
-                                     ? to_f(static_cast<const T *>(b1.p)[(n0 + rb) * b1.sr + (k0 + cb) * b1.sk])
-                                     : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kStep; k++) {
-                float x[4], y[4], z[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    x[i] = sa[k][ty * 4 + i];
-                    y[i] = sb[k][tx * 4 + i];
-                    if (DUAL) z[i] = sc[k][tx * 4 + i];
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
-                        if (DUAL) acc1[i][j] = fmaf(x[i], z[j], acc1[i][j]);
-                    }
-            }
-            __syncthreads();
-        }
-    }
-    if (EPI == EPI_LSE) {
-        for (int i = 0; i < 4; i++) {
-            const int64_t m = m0 + ty * 4 + i;
-            float top = -INFINITY;
-            for (int j = 0; j < 4; j++)
-                if (n0 + tx * 4 + j < N) top = fmaxf(top, acc[i][j]);
-            red[ty * 4 + i][tx] = top;
-            if (m < M) {
-                const int64_t t = e.target[m] - n0 - tx * 4;
-                for (int j = 0; j < 4; j++)
-                    if (t == j && n0 + tx * 4 + j < N) e.at[m] = acc[i][j];
-            }
-        }
-        __syncthreads();
-        for (int i = 0; i < 4; i++) {
-            float top = -INFINITY;
-            for (int j = 0; j < 16; j++) top = fmaxf(top, red[ty * 4 + i][j]);
-            float s = 0.0f;
-            for (int j = 0; j < 4; j++)
-                if (n0 + tx * 4 + j < N) s += top == -INFINITY && acc[i][j] == top ? 0.0f : __expf(acc[i][j] - top);
-            for (int o = 8; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            const int64_t m = m0 + ty * 4 + i;
-            if (tx == 0 && m < M) e.part[blockIdx.y * M + m] = make_float2(top, s);
-        }
-        return;
-    }
-    for (int i = 0; i < 4; i++) {
-        const int64_t m = m0 + ty * 4 + i;
-        if (m >= M) continue;
-        int64_t t = -1;
-        float g = 0.0f;
-        float2 lse = make_float2(0.0f, 0.0f);
-        if (EPI == EPI_Z) {
-            t = e.target[m];
-            if (t != e.ignore) g = e.dloss[m], lse = e.lse[m];
-            if (e.shift) g = ldexpf(g, *e.shift);
-        }
-        for (int j = 0; j < 4; j++) {
-            const int64_t n = n0 + tx * 4 + j;
-            if (n >= N) continue;
-            if (EPI == EPI_GATED) static_cast<T *>(e.o0)[m * e.ldo + n] = from_f<T>(act_f<ACT>(acc[i][j]) * acc1[i][j]);
-            if (EPI == EPI_GATED_BWD) {
-                const float dh = to_f(static_cast<const T *>(e.dh)[m * e.lddh + n]);
-                float v, d;
-                act_df<ACT>(acc[i][j], v, d);
-                static_cast<T *>(e.o0)[m * e.ldo + n] = from_f<T>(dh * acc1[i][j] * d);
-                static_cast<T *>(e.o1)[m * e.ldo + n] = from_f<T>(dh * v);
-            }
-            if (EPI == EPI_Z) {
-                float z = 0.0f;
-                if (t != e.ignore) {
-                    const float x = acc[i][j] - lse.x - lse.y;
-                    z = e.col0 + n == t ? expm1f(x) : __expf(x);
-                    z = t < 0 || t >= e.vocab ? NAN : z * g;
-                }
-                static_cast<T *>(e.o0)[m * e.ldo + n] = from_f<T>(z);
-            }
-            if (EPI == EPI_STORE) {
-                float v = acc[i][j];
-                if (!e.first) v += e.acc[m * N + n];
-                if (e.last)
-                    static_cast<T *>(e.o0)[m * e.ldo + n] = from_f<T>(e.shift ? ldexpf(v, -*e.shift) : v);
-                else
-                    e.acc[m * N + n] = v;
-            }
-        }
-    }
-}
 
 // ---------------------------------------------------------------- the loss
 // The row's (maximum, log of the sum relative to it) and loss from the (max,
 // sum) of every tile of the vocabulary.  The pair is kept apart: rounded to one
 // 32-bit number, a log-sum-exp of some thousands would be off by 2^-13, and so
 // would every probability.
-__global__ void k_loss(const float2 *__restrict__ part, int64_t tiles, const float *__restrict__ at,
-                       const int64_t *__restrict__ target, int64_t ignore, int64_t vocab, int64_t M,
-                       float *__restrict__ loss, float2 *__restrict__ lse) {
-    const int64_t m = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (m >= M) return;
-    float top = -INFINITY;
-    for (int64_t i = 0; i < tiles; i++) top = fmaxf(top, part[i * M + m].x);
-    float s = 0.0f;
-    for (int64_t i = 0; i < tiles; i++) {
-        const float2 p = part[i * M + m];
-        s += p.x == -INFINITY ? p.y : p.y * __expf(p.x - top);
+// A block takes 32 rows, its 32 warps every 32nd of the parts.
+__global__ void __launch_bounds__(1024) k_loss(const float2 *__restrict__ part, int64_t parts,
+                                               const float *__restrict__ at, const int64_t *__restrict__ target,
+                                               int64_t ignore, int64_t vocab, int64_t M, float *__restrict__ loss,
+                                               float2 *__restrict__ lse) {
+    __shared__ float2 red[32][33];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t m = (int64_t)blockIdx.x * 32 + lane;
+    float top = -INFINITY, s = 0.0f;
+    auto join = [&](float2 p) {
+        const float mx = fmaxf(top, p.x), ref = mx == -INFINITY ? 0.0f : mx;
+        s = (top == mx ? s : s * __expf(top - ref)) + (p.x == mx ? p.y : p.y * __expf(p.x - ref));
+        top = mx;
+    };
+    if (m < M) {
+#pragma unroll 4
+        for (int64_t i = warp; i < parts; i += 32) join(part[i * M + m]);
     }
+    red[warp][lane] = make_float2(top, s);
+    __syncthreads();
+    if (warp || m >= M) return;
+    for (int i = 1; i < 32; i++) join(red[i][lane]);
     const float l = logf(s);
     const int64_t t = target[m];
     lse[m] = make_float2(top, l);
@@ -237,7 +122,7 @@ __global__ void k_loss_shift(const float *__restrict__ dloss, const int64_t *__r
     __syncthreads();
     if (threadIdx.x == 0) {
         for (unsigned i = 1; i < blockDim.x / 32; i++) top = fmaxf(top, red[i]);
-        *shift = top > 0.0f && top < INFINITY ? 14 - ilogbf(top) : 0;
+        *shift = top > 0.0f && top < INFINITY ? max(-100, min(120, 14 - ilogbf(top))) : 0;
     }
 }
 

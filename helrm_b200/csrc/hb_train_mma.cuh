@@ -1,0 +1,609 @@
+// hb_train_mma.cuh -- the training operators' matrix product on the
+// 5th-generation tensor cores.  Included by hb_train.cu after hb_train.cuh.
+//
+// D[m][n] = sum_k A(m, k) B(n, k) over tiles of 256 x 256, one tile at a time
+// on a pair of SMs (a cluster of two, tcgen05 cta_group::2).  Each SM holds
+// half of A's rows and half of B's rows of a 64-deep slice in shared memory:
+// 32 KB a slice and SM, which halves the shared-memory traffic a 128 x 256
+// tile on one SM would have (96 B a clock written and 96 read, where an SM
+// moves 128).  Six slices are in flight, and two accumulators of 256 columns
+// fill the tensor memory, so that a tile's epilogue runs under the next
+// tile's products.  The grid is persistent: a cluster for every SM pair.
+//
+// Operands come by TMA with the 128-byte swizzle and may lie either way: rows
+// along k ("K-major") or rows along m / n ("MN-major"), so that the gradients
+// read dG, dU, Z, X, H and the weights as they are stored.  Rows, columns and
+// depth past the end are filled with zeros by the TMA unit.
+//
+// Warps (384 threads): 0 TMA, 1 MMA issue (first SM of the pair), 2 tensor
+// memory, 4-11 epilogue: quadrant warp & 3 of the accumulator's rows, and the
+// first or second half of its columns.
+//
+// Every wait is bounded: when one runs out, the block stops taking work,
+// waits for what it has in flight, frees its tensor memory and leaves a word
+// in host memory that the next training call reports.
+#pragma once
+#include <cuda.h>
+
+#include "hb_ptx.cuh"
+
+namespace hb {
+namespace train {
+
+constexpr int kRows = 256;     // rows of a tile, 128 on each SM
+constexpr int kCols = 256;     // accumulator columns of a tile
+constexpr int kDepth = 64;     // slice of k: 128 bytes
+constexpr int kStages = 6;
+constexpr int kOperand = 128 * kDepth * 2;  // bytes of an operand's slice on one SM
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = 128 + 32 * kEpiWarps;
+constexpr int kStageOut = 4096;  // staging bytes of an epilogue warp
+constexpr int kBarriers = 2 * kStages + 5;
+constexpr int kSmem = 2 * kStages * kOperand + kEpiWarps * kStageOut + 8 * kBarriers + 16;
+constexpr unsigned long long kWaitNs = 4000000000ull;
+
+enum { K_MAJOR = 0, MN_MAJOR = 1 };
+
+struct ProductArgs {
+    CUtensorMap a, a1, b, b1;
+    int64_t M, N;
+    int tiles_m, tiles_n;  // of one output
+    int outputs;           // 2: a second product A1 B^T into o1
+    int splits;            // the depth in this many parts, each with a partial sum of its own
+    int kb, kb1;           // slices of (A, B), and after them of (A1, B1)
+    EpiArgs e;
+    int *error;            // host memory
+};
+
+namespace ptx {
+__device__ __forceinline__ unsigned rank() {
+    unsigned r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// the address of the pair's first SM for a shared-memory address of this one
+__device__ __forceinline__ unsigned of_first(unsigned a) {
+    unsigned r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ void arrive_cluster(unsigned a) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+}
+__device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// Shared-memory matrix descriptor with the 128-byte swizzle.  K-major: rows of
+// 128 bytes, groups of 8 rows 1024 bytes apart.  MN-major: columns of 64
+// elements (128 bytes) 8192 bytes apart, groups of 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t descriptor(unsigned addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ void mma(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate));
+}
+// arrives on both SMs' barrier once the MMAs issued so far are done
+__device__ __forceinline__ void commit_both(unsigned bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((unsigned short)3)
+        : "memory");
+}
+__device__ __forceinline__ void commit_own(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// 32 columns of this warp's 32 accumulator rows
+__device__ __forceinline__ void load32(unsigned addr, float (&v)[32]) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,"
+        "%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+}  // namespace ptx
+
+template <class T> __device__ __forceinline__ unsigned pack2(float lo, float hi);
+template <> __device__ __forceinline__ unsigned pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const unsigned *>(&v);
+}
+template <class T> __device__ __forceinline__ float2 unpack2(unsigned v);
+template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned v) {
+    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned v) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
+}
+
+// A warp's 32 x 32 block of 16-bit values between registers (a row a lane) and
+// global memory, turned in shared memory so that a row's 64 bytes move
+// together.  Rows from M and columns from N on are left out.
+template <class T>
+__device__ __forceinline__ void store_block(unsigned char *st, const unsigned (&v)[16], T *out, int64_t ld, int64_t m0,
+                                            int64_t M, int64_t n0, int64_t N, bool vec, int lane) {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+        *reinterpret_cast<uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+            make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    __syncwarp();
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + (lane >> 2), c = lane & 3;
+            const uint4 w = *reinterpret_cast<const uint4 *>(st + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+            const int64_t m = m0 + r, n = n0 + c * 8;
+            if (m < M) {
+                if (n + 8 <= N) {
+                    *reinterpret_cast<uint4 *>(out + m * ld + n) = w;
+                } else {
+                    const unsigned p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (n + k < N)
+                            reinterpret_cast<unsigned short *>(out)[m * ld + n + k] =
+                                (unsigned short)(p[k >> 1] >> (16 * (k & 1)));
+                }
+            }
+        }
+    } else {
+        for (int r = 0; r < 32; r++)
+            if (m0 + r < M && n0 + lane < N)
+                reinterpret_cast<unsigned short *>(out)[(m0 + r) * ld + n0 + lane] =
+                    *reinterpret_cast<const unsigned short *>(st + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) +
+                                                              (lane & 7) * 2);
+    }
+    __syncwarp();
+}
+template <class T>
+__device__ __forceinline__ void load_block(unsigned char *st, unsigned (&v)[16], const T *in, int64_t ld, int64_t m0,
+                                           int64_t M, int64_t n0, int64_t N, bool vec, int lane) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int r = i * 8 + (lane >> 2), c = lane & 3;
+            const int64_t m = m0 + r, n = n0 + c * 8;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (m < M) {
+                if (n + 8 <= N) {
+                    w = *reinterpret_cast<const uint4 *>(in + m * ld + n);
+                } else {
+                    unsigned p[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (n + k < N)
+                            p[k >> 1] |= (unsigned)reinterpret_cast<const unsigned short *>(in)[m * ld + n + k]
+                                         << (16 * (k & 1));
+                    w = make_uint4(p[0], p[1], p[2], p[3]);
+                }
+            }
+            *reinterpret_cast<uint4 *>(st + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = w;
+        }
+    } else {
+        for (int r = 0; r < 32; r++)
+            *reinterpret_cast<unsigned short *>(st + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) =
+                m0 + r < M && n0 + lane < N ? reinterpret_cast<const unsigned short *>(in)[(m0 + r) * ld + n0 + lane]
+                                            : (unsigned short)0;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+        v[4 * j] = w.x, v[4 * j + 1] = w.y, v[4 * j + 2] = w.z, v[4 * j + 3] = w.w;
+    }
+    __syncwarp();
+}
+// The same for 32-bit sums, whose rows are padded to whole vectors.
+__device__ __forceinline__ void store_sums(unsigned char *st, const float (&v)[32], float *out, int64_t ld, int64_t m0,
+                                           int64_t M, int64_t n0, bool add, int lane) {
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+        *reinterpret_cast<float4 *>(st + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const int r = i * 4 + (lane >> 3), c = lane & 7;
+        float4 w = *reinterpret_cast<const float4 *>(st + r * 128 + ((c ^ (r & 7)) << 4));
+        const int64_t m = m0 + r, n = n0 + c * 4;
+        if (m < M && n < ld) {
+            float4 *p = reinterpret_cast<float4 *>(out + m * ld + n);
+            if (add) {
+                const float4 o = *p;
+                w.x += o.x, w.y += o.y, w.z += o.z, w.w += o.w;
+            }
+            *p = w;
+        }
+    }
+    __syncwarp();
+}
+
+template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    k_mma_product(const __grid_constant__ ProductArgs p) {
+    constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+    extern __shared__ __align__(1024) unsigned char smem[];
+    unsigned char *stage = smem + 2 * kStages * kOperand;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kEpiWarps * kStageOut);
+    const unsigned sA = tc::smem_u32(smem), sB = sA + kStages * kOperand;
+    const unsigned full = tc::smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages,
+                   tempty = tfull + 16, drain = tempty + 16;
+    unsigned *s_tmem = reinterpret_cast<unsigned *>(bars + kBarriers);
+    int *s_error = reinterpret_cast<int *>(s_tmem + 1);
+    volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 2);
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const unsigned rank = ptx::rank();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; i++) {
+            tc::mbar_init(full + 8 * i, 1);
+            tc::mbar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < 2; i++) {
+            tc::mbar_init(tfull + 8 * i, 1);
+            tc::mbar_init(tempty + 8 * i, 2 * kEpiWarps);
+        }
+        tc::mbar_init(drain, 1);
+        *s_error = 0;
+        *s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(s_tmem)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    tc::fence_before();
+    __syncthreads();
+    ptx::cluster_sync();
+    tc::fence_after();
+    const unsigned tmem = *s_tmem;
+
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int64_t items = (int64_t)tiles * p.splits * p.outputs;
+    const int depth = p.kb + p.kb1;
+    const int64_t first_item = blockIdx.x >> 1, step = gridDim.x >> 1;
+    struct Item {
+        int out, split, mt, nt, k0, k1;
+    };
+    // Tiles go down groups of 8 tile rows, column after column, so that the
+    // clusters at work share a few panels of A and of B in L2.
+    auto item = [&](int64_t i) {
+        Item t;
+        int r = (int)(i % tiles);
+        const int64_t q = i / tiles;
+        t.split = (int)(q % p.splits);
+        t.out = (int)(q / p.splits);
+        const int per = 8 * p.tiles_n, g = r / per;
+        r -= g * per;
+        const int h = p.tiles_m - g * 8 < 8 ? p.tiles_m - g * 8 : 8;
+        t.mt = g * 8 + r % h;
+        t.nt = r / h;
+        t.k0 = (int)((int64_t)depth * t.split / p.splits);
+        t.k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        return t;
+    };
+
+    if (warp == 0) {
+        // ------------------------------------------------------------ TMA
+        if (lane == 0) {
+            int s = 0;
+            unsigned ph = 0;
+            int64_t loads = 0;
+            bool ok = true;
+            for (int64_t i = first_item; ok && i < items; i += step) {
+                const Item t = item(i);
+                const int m = t.mt * kRows + 128 * (int)rank;
+                const int n = kDual ? t.nt * 128 : t.nt * kCols + 128 * (int)rank;
+                for (int k = t.k0; k < t.k1; k++) {
+                    if (!tc::mbar_wait(empty + 8 * s, ph ^ 1, s_abort, s_error, 1, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    if (rank == 0) tc::mbar_arrive_tx(full + 8 * s, 4 * kOperand);
+                    const unsigned bar = ptx::of_first(full + 8 * s);
+                    const bool second = k >= p.kb;
+                    const int x = (second ? k - p.kb : k) * kDepth;
+                    const CUtensorMap *ma = second || t.out ? &p.a1 : &p.a;
+                    const CUtensorMap *mb = second || (kDual && rank) ? &p.b1 : &p.b;
+                    const unsigned da = sA + s * kOperand, db = sB + s * kOperand;
+                    if (AMAJ == K_MAJOR) {
+                        ptx::tma_load(da, ma, x, m, bar);
+                    } else {
+                        ptx::tma_load(da, ma, m, x, bar);
+                        ptx::tma_load(da + kOperand / 2, ma, m + 64, x, bar);
+                    }
+                    if (BMAJ == K_MAJOR) {
+                        ptx::tma_load(db, mb, x, n, bar);
+                    } else {
+                        ptx::tma_load(db, mb, n, x, bar);
+                        ptx::tma_load(db + kOperand / 2, mb, n + 64, x, bar);
+                    }
+                    loads++;
+                    if (++s == kStages) s = 0, ph ^= 1;
+                }
+            }
+            // this SM stays until the last slices are consumed: their release
+            // arrives in its shared memory
+            for (int i = 0; ok && i < kStages && i < loads; i++) {
+                if (s == 0) ph ^= 1;
+                s = s == 0 ? kStages - 1 : s - 1;
+                ok = tc::mbar_wait(empty + 8 * s, ph, s_abort, s_error, 1, kWaitNs);
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ------------------------------------------------------------ MMA
+        if (rank == 0 && lane == 0) {
+            // 32-bit sums of bf16 or fp16, 256 x 256 over the pair
+            const unsigned idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) |
+                                   ((unsigned)AMAJ << 15) | ((unsigned)BMAJ << 16) | ((kCols >> 3) << 17) |
+                                   ((kRows >> 4) << 24);
+            // 16 of k: 32 bytes along a row, or 16 rows of 128 bytes
+            constexpr unsigned ka = AMAJ == K_MAJOR ? 32 : 2048, kb = BMAJ == K_MAJOR ? 32 : 2048;
+            int s = 0;
+            unsigned ph = 0;
+            int64_t n = 0;
+            bool ok = true;
+            for (int64_t i = first_item; ok && i < items; i += step, n++) {
+                const Item t = item(i);
+                const int buf = (int)(n & 1);
+                if (!tc::mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2, kWaitNs)) break;
+                tc::fence_after();
+                const unsigned d = tmem + buf * kCols;
+                for (int k = t.k0; k < t.k1; k++) {
+                    if (!tc::mbar_wait(full + 8 * s, ph, s_abort, s_error, 2, kWaitNs)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after();
+                    const uint64_t da = ptx::descriptor(sA + s * kOperand), db = ptx::descriptor(sB + s * kOperand);
+#pragma unroll
+                    for (int j = 0; j < kDepth / 16; j++)
+                        ptx::mma(d, da + ((j * ka) >> 4), db + ((j * kb) >> 4), idesc, k > t.k0 || j > 0);
+                    ptx::commit_both(empty + 8 * s);
+                    if (++s == kStages) s = 0, ph ^= 1;
+                }
+                if (ok) ptx::commit_both(tfull + 8 * buf);
+            }
+            // after a failure too, no MMA is left in flight
+            ptx::commit_own(drain);
+            tc::mbar_wait(drain, 0, nullptr, s_error, 8, kWaitNs);
+        }
+        __syncwarp();
+    } else if (warp >= 4) {
+        // ------------------------------------------------------------ epilogue
+        const int quad = warp & 3, half = (warp - 4) >> 2;
+        unsigned char *st = stage + (warp - 4) * kStageOut;
+        const unsigned bar_empty = ptx::of_first(tempty);
+        const EpiArgs &e = p.e;
+        constexpr float kLog2e = 1.4426950408889634f;
+        int64_t cnt = 0;
+        for (int64_t i = first_item; i < items; i += step, cnt++) {
+            const Item t = item(i);
+            const int buf = (int)(cnt & 1);
+            const int64_t m0 = (int64_t)t.mt * kRows + 128 * rank + 32 * quad, m = m0 + lane;
+            const unsigned acc = tmem + ((unsigned)(32 * quad) << 16) + buf * kCols;
+            auto release = [&] {
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) ptx::arrive_cluster(bar_empty + 8 * buf);
+            };
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(tfull + 8 * buf, (unsigned)((cnt >> 1) & 1), s_abort, s_error,
+                                                       4, kWaitNs)))
+                break;
+            tc::fence_after();
+            if constexpr (kDual) {
+                const int64_t n0 = (int64_t)t.nt * 128;
+                T *o0 = static_cast<T *>(e.o0), *o1 = static_cast<T *>(e.o1);
+                const bool vec = e.vec & 1, vdh = e.vec & 2;
+#pragma unroll 1
+                for (int c = 0; c < 2; c++) {
+                    const int col = half * 64 + c * 32;
+                    float g[32], u[32];
+                    unsigned w[16];
+                    ptx::load32(acc + col, g);
+                    ptx::load32(acc + 128 + col, u);
+                    if constexpr (EPI == EPI_GATED_BWD)
+                        load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, p.M, n0 + col, p.N, vdh, lane);
+                    tc::tmem_wait_ld();
+                    if (c == 1) release();
+                    if constexpr (EPI == EPI_GATED) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            w[j] = pack2<T>(act_f<ACT>(g[2 * j]) * u[2 * j], act_f<ACT>(g[2 * j + 1]) * u[2 * j + 1]);
+                        store_block<T>(st, w, o0, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
+                    } else {
+                        unsigned wu[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const float2 dh = unpack2<T>(w[j]);
+                            float a0, d0, a1, d1;
+                            act_df<ACT>(g[2 * j], a0, d0);
+                            act_df<ACT>(g[2 * j + 1], a1, d1);
+                            w[j] = pack2<T>(dh.x * u[2 * j] * d0, dh.y * u[2 * j + 1] * d1);
+                            wu[j] = pack2<T>(dh.x * a0, dh.y * a1);
+                        }
+                        store_block<T>(st, w, o0, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, wu, o1, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
+                    }
+                }
+            } else if constexpr (EPI == EPI_STORE || EPI == EPI_SUM) {
+                const int64_t n0 = (int64_t)t.nt * kCols;
+                const float scale = EPI == EPI_STORE && e.shift ? ldexpf(1.0f, -*e.shift) : 1.0f;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    const int col = half * 128 + c * 32;
+                    float v[32];
+                    ptx::load32(acc + col, v);
+                    tc::tmem_wait_ld();
+                    if (c == 3) release();
+                    if (n0 + col >= p.N) continue;
+                    if constexpr (EPI == EPI_STORE) {
+                        unsigned w[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) w[j] = pack2<T>(v[2 * j] * scale, v[2 * j + 1] * scale);
+                        store_block<T>(st, w, static_cast<T *>(t.out ? e.o1 : e.o0), e.ldo, m0, p.M, n0 + col, p.N,
+                                       e.vec & 1, lane);
+                    } else {
+                        float *o = e.acc + ((int64_t)t.out * p.splits + t.split) * p.M * e.ldo;
+                        store_sums(st, v, o, e.ldo, m0, p.M, n0 + col, !e.first, lane);
+                    }
+                }
+            } else if constexpr (EPI == EPI_LSE) {
+                const int64_t n0 = (int64_t)t.nt * kCols + half * 128;
+                const int64_t tg = m < p.M ? e.target[m] - n0 : -1;
+                float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float v[32];
+                    ptx::load32(acc + half * 128 + c * 32, v);
+                    tc::tmem_wait_ld();
+                    if (c == 3) release();
+                    const int64_t left = p.N - n0 - c * 32;  // columns of the vocabulary from here
+                    if (left < 32) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++)
+                            if (j >= left) v[j] = -INFINITY;
+                    }
+                    const int64_t at = tg - c * 32;
+                    if (at >= 0 && at < 32 && at < left) {
+                        float x = v[0];
+#pragma unroll
+                        for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
+                        e.at[m] = x;
+                    }
+                    float mx = v[0];
+#pragma unroll
+                    for (int j = 1; j < 32; j++) mx = fmaxf(mx, v[j]);
+                    mx = fmaxf(mx, top);
+                    // a row of minus infinities so far: relative to 0, nothing to add
+                    const float ref = mx == -INFINITY ? 0.0f : mx;
+                    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 32; j += 2) {
+                        s0 += ptx::ex2((v[j] - ref) * kLog2e);
+                        s1 += ptx::ex2((v[j + 1] - ref) * kLog2e);
+                    }
+                    sum = (top == mx ? sum : sum * ptx::ex2((top - ref) * kLog2e)) + (s0 + s1);
+                    top = mx;
+                }
+                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top, sum);
+            } else if constexpr (EPI == EPI_Z) {
+                const int64_t n0 = (int64_t)t.nt * kCols + half * 128;
+                int64_t tg = -1;
+                float g = 0.0f, x0 = 0.0f, x1 = 0.0f;
+                bool on = false;
+                if (m < p.M) {
+                    tg = e.target[m];
+                    on = tg != e.ignore;
+                    if (on) {
+                        g = tg < 0 || tg >= e.vocab ? NAN : e.dloss[m];
+                        if (e.shift) g = ldexpf(g, *e.shift);
+                        const float2 l = e.lse[m];
+                        x0 = l.x, x1 = l.y;
+                    }
+                    tg -= e.col0 + n0;
+                }
+#pragma unroll 1
+                for (int c = 0; c < 4; c++) {
+                    float v[32];
+                    unsigned w[16];
+                    ptx::load32(acc + half * 128 + c * 32, v);
+                    tc::tmem_wait_ld();
+                    if (c == 3) release();
+                    if (n0 + c * 32 >= p.N) continue;
+                    const int at = tg >= c * 32 && tg < c * 32 + 32 ? (int)tg - c * 32 : -1;
+                    float hot = 0.0f;
+                    if (on && at >= 0) {
+                        float x = v[0];
+#pragma unroll
+                        for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
+                        hot = expm1f(x - x0 - x1);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; j++) {
+                        float z = ptx::ex2((v[j] - x0 - x1) * kLog2e);
+                        if (at == j) z = hot;
+                        v[j] = on ? z * g : 0.0f;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 16; j++) w[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+                    store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, p.M, n0 + c * 32, p.N, e.vec & 1, lane);
+                }
+            }
+        }
+    }
+
+    // ---------------------------------------------------------------- the end
+    __syncwarp();
+    if (*s_abort) {
+        // a wait ran out: give the copies in flight a millisecond to land
+        const unsigned long long t0 = tc::gtimer();
+        while (tc::gtimer() - t0 < 1000000ull) {
+        }
+    }
+    tc::fence_before();
+    __syncthreads();
+    ptx::cluster_sync();
+    tc::fence_after();
+    if (warp == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    if (threadIdx.x == 0 && *s_error) {
+        *static_cast<volatile int *>(p.error) = *s_error;
+        __threadfence_system();
+    }
+}
+
+// out[m][n] = 16-bit (2^-shift * sum over the parts of acc[part][m][n])
+template <class T>
+__global__ void k_join(const float *__restrict__ acc, int parts, int64_t M, int64_t N, int64_t ld, const int *shift,
+                       T *__restrict__ out, int64_t ldo) {
+    const int64_t per = ld / 4, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= M * per) return;
+    const int64_t m = i / per, n = (i % per) * 4;
+    float4 s = make_float4(0, 0, 0, 0);
+    for (int k = 0; k < parts; k++) {
+        const float4 v = *reinterpret_cast<const float4 *>(acc + (k * M + m) * ld + n);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    float v[4] = {s.x, s.y, s.z, s.w};
+    for (int j = 0; j < 4; j++)
+        if (n + j < N) out[m * ldo + n + j] = from_f<T>(shift ? ldexpf(v[j], -*shift) : v[j]);
+}
+
+// A matrix with rows on 16-byte boundaries, for the TMA unit.
+__global__ void k_repitch(const unsigned short *__restrict__ in, int64_t ld, int64_t rows, int64_t cols,
+                          unsigned short *__restrict__ out, int64_t ldo) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= rows * ldo) return;
+    const int64_t r = i / ldo, c = i % ldo;
+    out[i] = c < cols ? in[r * ld + c] : (unsigned short)0;
+}
+
+}  // namespace train
+}  // namespace hb
