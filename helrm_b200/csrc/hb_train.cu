@@ -17,14 +17,18 @@ namespace train {
 struct DeviceGuard {
     int old = -1;
     explicit DeviceGuard(int device) {
+        cuda_check(cudaGetDevice(&old), "training call");
+        if (old == device) {
+            old = -1;
+            return;
+        }
         int n = 0;
         cuda_check(cudaGetDeviceCount(&n), "training call");
-        if (device < 0 || device >= n) HB_THROW(HB_EINVAL, "no CUDA device " + std::to_string(device));
-        cuda_check(cudaGetDevice(&old), "cudaGetDevice");
-        if (old != device)
-            cuda_check(cudaSetDevice(device), "cudaSetDevice");
-        else
+        if (device < 0 || device >= n) {
             old = -1;
+            HB_THROW(HB_EINVAL, "no CUDA device " + std::to_string(device));
+        }
+        cuda_check(cudaSetDevice(device), "cudaSetDevice");
     }
     ~DeviceGuard() {
         if (old >= 0) cudaSetDevice(old);
@@ -151,14 +155,42 @@ struct Operands {
         return {to, m.rows, m.cols, ld};
     }
     void copy(cudaStream_t s) const {
-        for (const Copy &c : copies) {
-            const int64_t ld = pitch(c.from.cols);
-            k_repitch<<<blocks(c.from.rows * ld, 256), 256, 0, s>>>(static_cast<const unsigned short *>(c.from.p),
-                                                                    c.from.ld, c.from.rows, c.from.cols, c.to, ld);
-            launched("copy to aligned rows");
+        if (copies.empty()) return;
+        Repitch p = {};
+        int64_t most = 0;
+        for (size_t i = 0; i < copies.size(); i++) {
+            const Matrix &m = copies[i].from;
+            p.from[i] = static_cast<const unsigned short *>(m.p);
+            p.to[i] = copies[i].to;
+            p.ld[i] = m.ld, p.rows[i] = m.rows, p.cols[i] = m.cols;
+            const int64_t n = m.rows * ((m.cols + 7) / 8);
+            if (n > most) most = n;
         }
+        const unsigned grid = blocks(most, 256) < 8u * 148 ? blocks(most, 256) : 8u * 148;
+        k_repitch<<<dim3(grid ? grid : 1, (unsigned)copies.size()), 256, 0, s>>>(p);
+        launched("copy to aligned rows");
     }
 };
+
+static CkptPlan ckpt_plan(int64_t rows, int64_t cols, bool vec, dim3 &grid) {
+    CkptPlan p;
+    p.rows = rows;
+    p.cols = cols;
+    p.chunks = 4 * (int)blocks(cols, HELRM_CKPT_GROUP);
+    p.per_block = p.chunks < kCkptThreads ? p.chunks : kCkptThreads;
+    p.rows_block = kCkptThreads / p.per_block;
+    p.vec = vec;
+    grid = dim3(blocks(rows, (int64_t)p.rows_block * kCkptRows), blocks(p.chunks, p.per_block));
+    return p;
+}
+template <class T>
+static void read_checkpoint(const int8_t *q, const uint8_t *ex, int64_t rows, int64_t cols, T *x, int64_t ldx,
+                            cudaStream_t s) {
+    dim3 grid;
+    const CkptPlan p = ckpt_plan(rows, cols, fits_vectors(x, ldx), grid);
+    k_unpack<T><<<grid, kCkptThreads, 0, s>>>(q, ex, p, x, ldx);
+    launched("read checkpoint");
+}
 
 static CUtensorMap tensor_map(const Matrix &m, bool bf16, int major) {
     CUtensorMap map;
@@ -320,7 +352,8 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
         if (x)
             check_matrix(x, ldx, inner, tokens);
         else
-            require(tokens == 0 || (q && ex && ((uintptr_t)q & 15) == 0), "neither x nor an aligned checkpoint is given");
+            require(inner <= 1 << 26 && (tokens == 0 || (q && ex && ((uintptr_t)q & 15) == 0)),
+                    "neither x nor an aligned checkpoint is given");
         check_matrix(wg, ldg, inner, width);
         check_matrix(wu, ldu, inner, width);
         require(dx || dwg || dwu, "no output is asked for");
@@ -349,11 +382,7 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
         in.copy(s);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
-            if (!x) {
-                k_unpack<T><<<blocks(tokens * inner, 256), 256, 0, s>>>(q, ex, tokens, inner,
-                                                                        reinterpret_cast<T *>(read), pitch(inner));
-                launched("read checkpoint");
-            }
+            if (!x) read_checkpoint<T>(q, ex, tokens, inner, reinterpret_cast<T *>(read), pitch(inner), s);
             Product d;
             d.a = mx, d.b = mg, d.b1 = mu;
             d.M = tokens, d.N = width, d.K = inner;
@@ -388,15 +417,16 @@ HB_API int helrm_PackCheckpoint(int device, int dtype, int64_t tokens, int64_t i
                                 int8_t *q, uint8_t *ex, void *stream) {
     return guard([&] {
         check_sizes(dtype, tokens, inner, 1);
+        require(inner <= 1 << 26, "rows of a checkpoint have at most 2^26 features");
         check_matrix(x, ldx, inner, tokens);
         if (tokens == 0) return;
         require(q && ex && ((uintptr_t)q & 15) == 0, "q or e is NULL, or q is not 16-byte aligned");
         DeviceGuard dev(device);
-        const int64_t groups = blocks(inner, HELRM_CKPT_GROUP);
+        dim3 grid;
+        const CkptPlan p = ckpt_plan(tokens, inner, fits_vectors(x, tokens > 1 ? ldx : pitch(inner)), grid);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
-            k_pack<T><<<blocks(tokens * groups * 32, 256), 256, 0, (cudaStream_t)stream>>>(
-                static_cast<const T *>(x), ldx, tokens, inner, q, ex);
+            k_pack<T><<<grid, kCkptThreads, 0, (cudaStream_t)stream>>>(static_cast<const T *>(x), ldx, p, q, ex);
         });
         launched("pack checkpoint");
     });
@@ -406,15 +436,14 @@ HB_API int helrm_UnpackCheckpoint(int device, int dtype, int64_t tokens, int64_t
                                   const uint8_t *ex, void *x, void *stream) {
     return guard([&] {
         check_sizes(dtype, tokens, inner, 1);
+        require(inner <= 1 << 26, "rows of a checkpoint have at most 2^26 features");
         if (tokens == 0) return;
         require(q && ex && x && ((uintptr_t)q & 15) == 0, "q, e or x is NULL, or q is not 16-byte aligned");
         DeviceGuard dev(device);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
-            k_unpack<T><<<blocks(tokens * inner, 256), 256, 0, (cudaStream_t)stream>>>(q, ex, tokens, inner,
-                                                                                      static_cast<T *>(x), inner);
+            read_checkpoint<T>(q, ex, tokens, inner, static_cast<T *>(x), inner, (cudaStream_t)stream);
         });
-        launched("unpack checkpoint");
     });
 }
 

@@ -116,29 +116,7 @@ __device__ __forceinline__ void load32(unsigned addr, float (&v)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 }  // namespace ptx
-
-template <class T> __device__ __forceinline__ unsigned pack2(float lo, float hi);
-template <> __device__ __forceinline__ unsigned pack2<__half>(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const unsigned *>(&v);
-}
-template <> __device__ __forceinline__ unsigned pack2<__nv_bfloat16>(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const unsigned *>(&v);
-}
-template <class T> __device__ __forceinline__ float2 unpack2(unsigned v);
-template <> __device__ __forceinline__ float2 unpack2<__half>(unsigned v) {
-    return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned v) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
-}
 
 // A warp's 32 x 32 block of 16-bit values between registers (a row a lane) and
 // global memory, turned in shared memory so that a row's 64 bytes move
@@ -402,7 +380,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         unsigned char *st = stage + (warp - 4) * kStageOut;
         const unsigned bar_empty = ptx::of_first(tempty);
         const EpiArgs &e = p.e;
-        constexpr float kLog2e = 1.4426950408889634f;
         int64_t cnt = 0;
         for (int64_t i = first_item; i < items; i += step, cnt++) {
             const Item t = item(i);
@@ -507,10 +484,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 32; j += 2) {
-                        s0 += ptx::ex2((v[j] - ref) * kLog2e);
-                        s1 += ptx::ex2((v[j + 1] - ref) * kLog2e);
+                        s0 += ex2((v[j] - ref) * kLog2e);
+                        s1 += ex2((v[j + 1] - ref) * kLog2e);
                     }
-                    sum = (top == mx ? sum : sum * ptx::ex2((top - ref) * kLog2e)) + (s0 + s1);
+                    sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + (s0 + s1);
                     top = mx;
                 }
                 if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top, sum);
@@ -548,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
 #pragma unroll
                     for (int j = 0; j < 32; j++) {
-                        float z = ptx::ex2((v[j] - x0 - x1) * kLog2e);
+                        float z = ex2((v[j] - x0 - x1) * kLog2e);
                         if (at == j) z = hot;
                         v[j] = on ? z * g : 0.0f;
                     }
@@ -596,13 +573,20 @@ __global__ void k_join(const float *__restrict__ acc, int parts, int64_t M, int6
         if (n + j < N) out[m * ldo + n + j] = from_f<T>(shift ? ldexpf(v[j], -*shift) : v[j]);
 }
 
-// A matrix with rows on 16-byte boundaries, for the TMA unit.
-__global__ void k_repitch(const unsigned short *__restrict__ in, int64_t ld, int64_t rows, int64_t cols,
-                          unsigned short *__restrict__ out, int64_t ldo) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= rows * ldo) return;
-    const int64_t r = i / ldo, c = i % ldo;
-    out[i] = c < cols ? in[r * ld + c] : (unsigned short)0;
+// Matrices with rows on 16-byte boundaries, for the TMA unit: up to four in a
+// launch, one for each blockIdx.y, eight elements a thread.
+struct Repitch {
+    const unsigned short *from[4];
+    unsigned short *to[4];
+    int64_t ld[4], rows[4], cols[4];
+};
+__global__ void k_repitch(const __grid_constant__ Repitch p) {
+    const int k = blockIdx.y;
+    const int64_t per = (p.cols[k] + 7) / 8, n = p.rows[k] * per;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / per, c = i % per * 8;
+        reinterpret_cast<uint4 *>(p.to[k])[i] = load8(p.from[k] + r * p.ld[k], c, p.cols[k], false);
+    }
 }
 
 }  // namespace train

@@ -52,12 +52,16 @@ def _matrix(t, name: str, cols: int | None = None):
         raise ValueError(f"{name} is {t.dtype}: the training operators take torch.float16 or torch.bfloat16")
     if not t.is_cuda:
         raise ValueError(f"{name} is on {t.device}: the training operators run on a CUDA device only")
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{name} has no features (shape {tuple(t.shape)})")
-    if cols is not None and t.shape[-1] != cols:
-        raise ValueError(f"{name} has {t.shape[-1]} features where {cols} are expected")
-    m = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    if m.stride(1) != 1 and m.shape[1] > 1 or m.shape[0] > 1 and m.stride(0) < m.shape[1]:
+    shape = t.shape
+    if len(shape) < 1 or shape[-1] < 1:
+        raise ValueError(f"{name} has no features (shape {tuple(shape)})")
+    if cols is not None and shape[-1] != cols:
+        raise ValueError(f"{name} has {shape[-1]} features where {cols} are expected")
+    m = t if len(shape) == 2 else t.reshape(-1, shape[-1])
+    if m.is_contiguous():
+        return m
+    rows, cols = m.shape
+    if m.stride(1) != 1 and cols > 1 or rows > 1 and m.stride(0) < cols:
         m = m.contiguous()
     return m
 
@@ -68,8 +72,9 @@ def _weight(t, name: str, cols: int):
     return _matrix(t, name, cols)
 
 
-def _pitch(m) -> int:
-    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
+def _place(m):
+    """(address, row pitch)"""
+    return m.data_ptr(), m.stride(0) if m.shape[0] > 1 else m.shape[1]
 
 
 def _same(first, **others):
@@ -86,14 +91,39 @@ def _activation(name: str) -> int:
     return ACTIVATIONS[name]
 
 
-def _run(name: str, dev, *args):
-    """One entry point that takes a workspace, on dev's current stream."""
-    fn = getattr(_capi.load(), name)
-    need = ctypes.c_size_t(0)
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    _capi.check(fn(*args, None, ctypes.byref(need), stream))
-    ws = torch.empty(max(1, need.value), dtype=torch.uint8, device=dev)
-    _capi.check(fn(*args, ws.data_ptr(), ctypes.byref(need), stream))
+_entries: dict = {}
+_workspaces: dict = {}  # bytes an entry needs, by its sizes, pitches and alignments
+
+
+def _entry(name: str):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(_capi.load(), name)
+    return fn
+
+
+def _stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+def _run(name: str, dev, sizes, *args):
+    """One entry point that takes a workspace, on dev's current stream.
+    sizes: what the workspace depends on."""
+    fn = _entry(name)
+    need = _workspaces.get(key := (name, sizes))
+    if need is None:
+        if len(_workspaces) > 4096:
+            _workspaces.clear()
+        n = ctypes.c_size_t(0)
+        _capi.check(fn(*args, None, ctypes.byref(n), 0))
+        need = _workspaces[key] = n.value
+    if need:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        rc = fn(*args, ws.data_ptr(), ctypes.byref(ctypes.c_size_t(need)), _stream(dev.index))
+    else:  # any aligned address will do
+        rc = fn(*args, 256, ctypes.byref(ctypes.c_size_t(0)), _stream(dev.index))
+    if rc:
+        _capi.check(rc)
 
 
 # ------------------------------------------------------------------ the gated block
@@ -111,8 +141,10 @@ def gated_forward(x, w_gate, w_up, activation: str = "silu"):
     if width < 1:
         raise ValueError("the weights have no rows")
     h = torch.empty(x.shape[:-1] + (width,), dtype=x.dtype, device=x.device)
-    _run("helrm_GatedForward", x.device, x.device.index, _DTYPES[x.dtype], act, tokens, inner, width, xm.data_ptr(),
-         _pitch(xm), wg.data_ptr(), _pitch(wg), wu.data_ptr(), _pitch(wu), h.data_ptr())
+    dev = x.device
+    px, lx, pg, lg, pu, lu = *_place(xm), *_place(wg), *_place(wu)
+    _run("helrm_GatedForward", dev, (tokens, inner, width, px % 16, lx, pg % 16, lg, pu % 16, lu), dev.index,
+         _DTYPES[x.dtype], act, tokens, inner, width, px, lx, pg, lg, pu, lu, h.data_ptr())
     return h
 
 
@@ -145,10 +177,14 @@ def gated_backward(dh, x, w_gate, w_up, activation: str = "silu", needs=(True, T
     dwg = torch.empty((width, inner), **like) if needs[1] else None
     dwu = torch.empty((width, inner), **like) if needs[2] else None
     if any(needs):
-        _run("helrm_GatedBackward", dh.device, dh.device.index, _DTYPES[dh.dtype], act, tokens, inner, width,
-             dhm.data_ptr(), _pitch(dhm), None if kept else xm.data_ptr(), inner if kept else _pitch(xm),
-             x.q.data_ptr() if kept else None, x.e.data_ptr() if kept else None, wg.data_ptr(), _pitch(wg),
-             wu.data_ptr(), _pitch(wu), *(None if t is None else t.data_ptr() for t in (dx, dwg, dwu)))
+        dev = dh.device
+        px, lx = (0, inner) if kept else _place(xm)
+        pd, ld, pg, lg, pu, lu = *_place(dhm), *_place(wg), *_place(wu)
+        _run("helrm_GatedBackward", dev,
+             (tokens, inner, width, kept, px % 16, lx, pg % 16, lg, pu % 16, lu, *(bool(n) for n in needs)),
+             dev.index, _DTYPES[dh.dtype], act, tokens, inner, width, pd, ld, px or None, lx,
+             x.q.data_ptr() if kept else None, x.e.data_ptr() if kept else None, pg, lg, pu, lu,
+             *(None if t is None else t.data_ptr() for t in (dx, dwg, dwu)))
     return dx, dwg, dwu
 
 
@@ -203,9 +239,11 @@ def pack_checkpoint(x) -> Checkpoint:
     groups = -(-cols // GROUP)
     q = torch.empty((rows, GROUP * groups), dtype=torch.int8, device=x.device)
     e = torch.empty((rows, groups), dtype=torch.uint8, device=x.device)
-    _capi.check(_capi.load().helrm_PackCheckpoint(
-        x.device.index, _DTYPES[x.dtype], rows, cols, m.data_ptr(), _pitch(m), q.data_ptr(), e.data_ptr(),
-        torch.cuda.current_stream(x.device).cuda_stream))
+    dev = x.device.index
+    rc = _entry("helrm_PackCheckpoint")(dev, _DTYPES[x.dtype], rows, cols, *_place(m), q.data_ptr(), e.data_ptr(),
+                                        _stream(dev))
+    if rc:
+        _capi.check(rc)
     return Checkpoint(q, e, tuple(x.shape), x.dtype)
 
 
@@ -215,9 +253,11 @@ def unpack_checkpoint(c: Checkpoint):
         raise ValueError("not a checkpoint that pack_checkpoint returned")
     rows = _check_checkpoint(c)
     x = torch.empty(c.shape, dtype=c.dtype, device=c.q.device)
-    _capi.check(_capi.load().helrm_UnpackCheckpoint(
-        x.device.index, _DTYPES[c.dtype], rows, c.shape[-1], c.q.data_ptr(), c.e.data_ptr(), x.data_ptr(),
-        torch.cuda.current_stream(x.device).cuda_stream))
+    dev = x.device.index
+    rc = _entry("helrm_UnpackCheckpoint")(dev, _DTYPES[c.dtype], rows, c.shape[-1], c.q.data_ptr(), c.e.data_ptr(),
+                                          x.data_ptr(), _stream(dev))
+    if rc:
+        _capi.check(rc)
     return x
 
 
@@ -252,9 +292,11 @@ def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
     t = _targets(targets, h.shape[:-1], h.device)
     loss = torch.empty(h.shape[:-1], dtype=torch.float32, device=h.device)
     lse = torch.empty(h.shape[:-1] + (2,), dtype=torch.float32, device=h.device)
-    _run("helrm_VocabularyLossForward", h.device, h.device.index, _DTYPES[h.dtype], hm.shape[0], hm.shape[1],
-         wm.shape[0], hm.data_ptr(), _pitch(hm), wm.data_ptr(), _pitch(wm), t.data_ptr(), int(ignore_index),
-         loss.data_ptr(), lse.data_ptr())
+    dev, tokens, inner, vocab = h.device, hm.shape[0], hm.shape[1], wm.shape[0]
+    ph, lh, pw, lw = *_place(hm), *_place(wm)
+    _run("helrm_VocabularyLossForward", dev, (tokens, inner, vocab, ph % 16, lh, pw % 16, lw), dev.index,
+         _DTYPES[h.dtype], tokens, inner, vocab, ph, lh, pw, lw, t.data_ptr(), int(ignore_index), loss.data_ptr(),
+         lse.data_ptr())
     return loss, lse
 
 
@@ -272,8 +314,11 @@ def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100
     dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if needs[0] else None
     dw = torch.empty(wm.shape, dtype=h.dtype, device=dev) if needs[1] else None
     if any(needs):
-        _run("helrm_VocabularyLossBackward", dev, dev.index, _DTYPES[h.dtype], hm.shape[0], hm.shape[1], wm.shape[0],
-             g.data_ptr(), hm.data_ptr(), _pitch(hm), wm.data_ptr(), _pitch(wm), t.data_ptr(), l.data_ptr(),
+        tokens, inner, vocab = hm.shape[0], hm.shape[1], wm.shape[0]
+        ph, lh, pw, lw = *_place(hm), *_place(wm)
+        _run("helrm_VocabularyLossBackward", dev,
+             (h.dtype, tokens, inner, vocab, ph % 16, lh, pw % 16, lw, bool(needs[0]), bool(needs[1])), dev.index,
+             _DTYPES[h.dtype], tokens, inner, vocab, g.data_ptr(), ph, lh, pw, lw, t.data_ptr(), l.data_ptr(),
              int(ignore_index), *(None if o is None else o.data_ptr() for o in (dh, dw)))
     return dh, dw
 
