@@ -238,11 +238,12 @@ static void launch(const Product &d, cudaStream_t s) {
     cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
     auto kernel = k_mma_product<T, AMAJ, BMAJ, EPI, ACT>;
     if (!(set >> (dev & 63) & 1)) {
-        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem), "shared memory");
+        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kProductSmem), "shared memory");
         set |= (uint64_t)1 << (dev & 63);
     }
     const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
-    kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), kThreads, kSmem, s>>>(p);
+    kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
+             kProductSmem, s>>>(p);
     launched("training product");
 }
 
@@ -462,8 +463,9 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         Product d;
         d.a = in.fit({h, tokens, inner, ldh});
         d.b = in.fit({wt, vocab, inner, ldw});
-        const int64_t parts = 2 * (int64_t)blocks(vocab, kCols);
-        float2 *part = w.take<float2>(parts * tokens);
+        const int64_t parts = epi_warps(EPI_LSE) / 4 * (int64_t)blocks(vocab, kCols);
+        const int64_t joined = parts > kLossParts ? blocks(parts, kLossParts) : 0;
+        float2 *part = w.take<float2>(parts * tokens), *few = w.take<float2>(joined * tokens);
         float *at = w.take<float>(tokens);
         if (sized(w, ws_bytes) || tokens == 0) return;
         DeviceGuard dev(device);
@@ -474,8 +476,14 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         d.e.at = at;
         d.e.target = targets;
         by_dtype(dtype, [&](auto t) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_LSE, 0>(d, s); });
-        k_loss<<<blocks(tokens, 32), 1024, 0, s>>>(part, parts, at, targets, ignore_index, vocab, tokens, loss,
-                                                   reinterpret_cast<float2 *>(lse));
+        if (joined) {
+            k_loss<false><<<dim3(blocks(tokens, 32), (unsigned)joined), 1024, 0, s>>>(
+                part, parts, nullptr, nullptr, 0, 0, tokens, nullptr, few);
+            launched("loss");
+        }
+        k_loss<true><<<blocks(tokens, 32), 1024, 0, s>>>(joined ? few : part, joined ? joined : parts, at, targets,
+                                                         ignore_index, vocab, tokens, loss,
+                                                         reinterpret_cast<float2 *>(lse));
         launched("loss");
     });
 }

@@ -15,9 +15,9 @@
 // read dG, dU, Z, X, H and the weights as they are stored.  Rows, columns and
 // depth past the end are filled with zeros by the TMA unit.
 //
-// Warps (384 threads): 0 TMA, 1 MMA issue (first SM of the pair), 2 tensor
-// memory, 4-11 epilogue: quadrant warp & 3 of the accumulator's rows, and the
-// first or second half of its columns.
+// Warps: 0 TMA, 1 MMA issue (first SM of the pair), 2 tensor memory, 4 on
+// epilogue: quadrant warp & 3 of the accumulator's rows, and the columns shared
+// out among the warps of a quadrant.
 //
 // Every wait is bounded: when one runs out, the block stops taking work,
 // waits for what it has in flight, frees its tensor memory and leaves a word
@@ -35,11 +35,14 @@ constexpr int kCols = 256;     // accumulator columns of a tile
 constexpr int kDepth = 64;     // slice of k: 128 bytes
 constexpr int kStages = 6;
 constexpr int kOperand = 128 * kDepth * 2;  // bytes of an operand's slice on one SM
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = 128 + 32 * kEpiWarps;
-constexpr int kStageOut = 4096;  // staging bytes of an epilogue warp
+constexpr int kStageOut = 32768;  // staging bytes of the epilogue warps together
 constexpr int kBarriers = 2 * kStages + 5;
-constexpr int kSmem = 2 * kStages * kOperand + kEpiWarps * kStageOut + 8 * kBarriers + 16;
+constexpr int kProductSmem = 2 * kStages * kOperand + kStageOut + 8 * kBarriers + 16;
+// Epilogue warps.  The loss's exponentials keep 16 busy (8 warps left the
+// special-function pipe at 52% of its rate, the warps waiting for their own
+// results); the others need the registers of 8.
+__host__ __device__ constexpr int epi_warps(int epi) { return epi == EPI_LSE || epi == EPI_Z ? 16 : 8; }
+__host__ __device__ constexpr int product_threads(int epi) { return 128 + 32 * epi_warps(epi); }
 constexpr unsigned long long kWaitNs = 4000000000ull;
 
 enum { K_MAJOR = 0, MN_MAJOR = 1 };
@@ -70,8 +73,10 @@ __device__ __forceinline__ unsigned of_first(unsigned a) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(a));
     return r;
 }
+// The accumulator's reads are ordered by the tcgen05 fences; a release at
+// cluster scope would wait for this thread's stores to global memory too.
 __device__ __forceinline__ void arrive_cluster(unsigned a) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
 }
 __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, int x, int y, unsigned bar) {
     asm volatile(
@@ -116,81 +121,65 @@ __device__ __forceinline__ void load32(unsigned addr, float (&v)[32]) {
           "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
 }
+// Waits for this warp's loads.  The registers pass through, so that nothing
+// that reads them can be moved before the wait.
+__device__ __forceinline__ void wait32(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                   "+f"(v[15]), "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]),
+                   "+f"(v[22]), "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]),
+                   "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+                 :
+                 : "memory");
+}
 }  // namespace ptx
 
 // A warp's 32 x 32 block of 16-bit values between registers (a row a lane) and
 // global memory, turned in shared memory so that a row's 64 bytes move
 // together.  Rows from M and columns from N on are left out.
+__device__ __forceinline__ unsigned block_at(int r, int c) { return r * 64 + ((c ^ ((r >> 1) & 3)) << 4); }
 template <class T>
 __device__ __forceinline__ void store_block(unsigned char *st, const unsigned (&v)[16], T *out, int64_t ld, int64_t m0,
                                             int64_t M, int64_t n0, int64_t N, bool vec, int lane) {
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        *reinterpret_cast<uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) =
+        *reinterpret_cast<uint4 *>(st + block_at(lane, j)) =
             make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
     __syncwarp();
-    if (vec) {
+    unsigned short *o = reinterpret_cast<unsigned short *>(out) + m0 * ld + n0;
+    if (vec && m0 + 32 <= M && n0 + 32 <= N) {
+        o += (lane >> 2) * ld + (lane & 3) * 8;
+        const unsigned char *from = st + block_at(lane >> 2, lane & 3);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + (lane >> 2), c = lane & 3;
-            const uint4 w = *reinterpret_cast<const uint4 *>(st + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-            const int64_t m = m0 + r, n = n0 + c * 8;
-            if (m < M) {
-                if (n + 8 <= N) {
-                    *reinterpret_cast<uint4 *>(out + m * ld + n) = w;
-                } else {
-                    const unsigned p[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        if (n + k < N)
-                            reinterpret_cast<unsigned short *>(out)[m * ld + n + k] =
-                                (unsigned short)(p[k >> 1] >> (16 * (k & 1)));
-                }
-            }
-        }
-    } else {
-        for (int r = 0; r < 32; r++)
-            if (m0 + r < M && n0 + lane < N)
-                reinterpret_cast<unsigned short *>(out)[(m0 + r) * ld + n0 + lane] =
-                    *reinterpret_cast<const unsigned short *>(st + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) +
-                                                              (lane & 7) * 2);
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(o + i * 8 * ld) = *reinterpret_cast<const uint4 *>(from + i * 512);
+    } else if (n0 + lane < N) {
+        const int rows = M - m0 < 32 ? (int)(M - m0) : 32;
+#pragma unroll 4
+        for (int r = 0; r < rows; r++)
+            o[r * ld + lane] = *reinterpret_cast<const unsigned short *>(st + block_at(r, lane >> 3) + (lane & 7) * 2);
     }
     __syncwarp();
 }
 template <class T>
 __device__ __forceinline__ void load_block(unsigned char *st, unsigned (&v)[16], const T *in, int64_t ld, int64_t m0,
                                            int64_t M, int64_t n0, int64_t N, bool vec, int lane) {
-    if (vec) {
+    const unsigned short *p = reinterpret_cast<const unsigned short *>(in) + m0 * ld + n0;
+    if (vec && m0 + 32 <= M && n0 + 32 <= N) {
+        p += (lane >> 2) * ld + (lane & 3) * 8;
+        unsigned char *to = st + block_at(lane >> 2, lane & 3);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int r = i * 8 + (lane >> 2), c = lane & 3;
-            const int64_t m = m0 + r, n = n0 + c * 8;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (m < M) {
-                if (n + 8 <= N) {
-                    w = *reinterpret_cast<const uint4 *>(in + m * ld + n);
-                } else {
-                    unsigned p[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int k = 0; k < 8; k++)
-                        if (n + k < N)
-                            p[k >> 1] |= (unsigned)reinterpret_cast<const unsigned short *>(in)[m * ld + n + k]
-                                         << (16 * (k & 1));
-                    w = make_uint4(p[0], p[1], p[2], p[3]);
-                }
-            }
-            *reinterpret_cast<uint4 *>(st + r * 64 + ((c ^ ((r >> 1) & 3)) << 4)) = w;
-        }
+        for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(to + i * 512) = *reinterpret_cast<const uint4 *>(p + i * 8 * ld);
     } else {
+#pragma unroll 4
         for (int r = 0; r < 32; r++)
-            *reinterpret_cast<unsigned short *>(st + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) =
-                m0 + r < M && n0 + lane < N ? reinterpret_cast<const unsigned short *>(in)[(m0 + r) * ld + n0 + lane]
-                                            : (unsigned short)0;
+            *reinterpret_cast<unsigned short *>(st + block_at(r, lane >> 3) + (lane & 7) * 2) =
+                m0 + r < M && n0 + lane < N ? p[r * ld + lane] : (unsigned short)0;
     }
     __syncwarp();
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        const uint4 w = *reinterpret_cast<const uint4 *>(st + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+        const uint4 w = *reinterpret_cast<const uint4 *>(st + block_at(lane, j));
         v[4 * j] = w.x, v[4 * j + 1] = w.y, v[4 * j + 2] = w.z, v[4 * j + 3] = w.w;
     }
     __syncwarp();
@@ -221,12 +210,13 @@ __device__ __forceinline__ void store_sums(unsigned char *st, const float (&v)[3
 }
 
 template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI), 1)
     k_mma_product(const __grid_constant__ ProductArgs p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
+    constexpr int kWarps = epi_warps(EPI);
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *stage = smem + 2 * kStages * kOperand;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kEpiWarps * kStageOut);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kStageOut);
     const unsigned sA = tc::smem_u32(smem), sB = sA + kStages * kOperand;
     const unsigned full = tc::smem_u32(bars), empty = full + 8 * kStages, tfull = empty + 8 * kStages,
                    tempty = tfull + 16, drain = tempty + 16;
@@ -243,7 +233,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         for (int i = 0; i < 2; i++) {
             tc::mbar_init(tfull + 8 * i, 1);
-            tc::mbar_init(tempty + 8 * i, 2 * kEpiWarps);
+            tc::mbar_init(tempty + 8 * i, 2 * kWarps);
         }
         tc::mbar_init(drain, 1);
         *s_error = 0;
@@ -376,8 +366,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------ epilogue
-        const int quad = warp & 3, half = (warp - 4) >> 2;
-        unsigned char *st = stage + (warp - 4) * kStageOut;
+        const int quad = warp & 3, half = (warp - 4) >> 2;  // half: or quarter, with 16 warps
+        unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
         const EpiArgs &e = p.e;
         int64_t cnt = 0;
@@ -408,7 +398,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     ptx::load32(acc + 128 + col, u);
                     if constexpr (EPI == EPI_GATED_BWD)
                         load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, p.M, n0 + col, p.N, vdh, lane);
-                    tc::tmem_wait_ld();
+                    ptx::wait32(g);
+                    ptx::wait32(u);
                     if (c == 1) release();
                     if constexpr (EPI == EPI_GATED) {
 #pragma unroll
@@ -438,7 +429,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     const int col = half * 128 + c * 32;
                     float v[32];
                     ptx::load32(acc + col, v);
-                    tc::tmem_wait_ld();
+                    ptx::wait32(v);
                     if (c == 3) release();
                     if (n0 + col >= p.N) continue;
                     if constexpr (EPI == EPI_STORE) {
@@ -453,46 +444,52 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                 }
             } else if constexpr (EPI == EPI_LSE) {
-                const int64_t n0 = (int64_t)t.nt * kCols + half * 128;
+                constexpr int kWide = kCols / (kWarps / 4);  // columns a warp
+                const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 const int64_t tg = m < p.M ? e.target[m] - n0 : -1;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < kWide / 32; c++) {
                     float v[32];
-                    ptx::load32(acc + half * 128 + c * 32, v);
-                    tc::tmem_wait_ld();
-                    if (c == 3) release();
-                    const int64_t left = p.N - n0 - c * 32;  // columns of the vocabulary from here
+                    ptx::load32(acc + half * kWide + c * 32, v);
+                    ptx::wait32(v);
+                    if (c == kWide / 32 - 1) release();
+                    const int left = (int)(p.N - n0 < kWide ? p.N - n0 : kWide) - c * 32;  // columns that exist
                     if (left < 32) {
 #pragma unroll
                         for (int j = 0; j < 32; j++)
                             if (j >= left) v[j] = -INFINITY;
                     }
-                    const int64_t at = tg - c * 32;
-                    if (at >= 0 && at < 32 && at < left) {
+                    const int at = tg >= c * 32 && tg < c * 32 + 32 && tg < c * 32 + left ? (int)tg - c * 32 : -1;
+                    if (__any_sync(0xffffffffu, at >= 0)) {
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        e.at[m] = x;
+                        if (at >= 0) e.at[m] = x;
                     }
-                    float mx = v[0];
+                    float m0 = v[0], m1 = v[1];
 #pragma unroll
-                    for (int j = 1; j < 32; j++) mx = fmaxf(mx, v[j]);
-                    mx = fmaxf(mx, top);
+                    for (int j = 2; j < 32; j += 2) m0 = fmaxf(m0, v[j]), m1 = fmaxf(m1, v[j + 1]);
+                    const float mx = fmaxf(fmaxf(m0, m1), top);
                     // a row of minus infinities so far: relative to 0, nothing to add
                     const float ref = mx == -INFINITY ? 0.0f : mx;
-                    float s0 = 0.0f, s1 = 0.0f;
+                    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 32; j += 2) {
+                    for (int j = 0; j < 32; j += 4) {
                         s0 += ex2((v[j] - ref) * kLog2e);
                         s1 += ex2((v[j + 1] - ref) * kLog2e);
+                        s2 += ex2((v[j + 2] - ref) * kLog2e);
+                        s3 += ex2((v[j + 3] - ref) * kLog2e);
                     }
-                    sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + (s0 + s1);
+                    sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + ((s0 + s1) + (s2 + s3));
                     top = mx;
                 }
-                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top, sum);
+                if (m < p.M) e.part[((int64_t)t.nt * (kWarps / 4) + half) * p.M + m] = make_float2(top, sum);
             } else if constexpr (EPI == EPI_Z) {
-                const int64_t n0 = (int64_t)t.nt * kCols + half * 128;
+                constexpr int kWide = kCols / (kWarps / 4);
+                const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
+                // z = g exp(v - x0 - x1) = sign 2^((v - x0) log2(e) + c): the difference to the row's maximum is exact
+                // where it matters, and |g| costs nothing.  Sign and rows without a target go over the packed words.
                 int64_t tg = -1;
                 float g = 0.0f, x0 = 0.0f, x1 = 0.0f;
                 bool on = false;
@@ -507,30 +504,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     tg -= e.col0 + n0;
                 }
+                const float add = log2f(fabsf(g)) - x1 * kLog2e;
+                const unsigned mask = on ? 0xffffffffu : 0u, sign = on && g < 0.0f ? 0x80008000u : 0u;
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
+                for (int c = 0; c < kWide / 32; c++) {
                     float v[32];
-                    unsigned w[16];
-                    ptx::load32(acc + half * 128 + c * 32, v);
-                    tc::tmem_wait_ld();
-                    if (c == 3) release();
+                    ptx::load32(acc + half * kWide + c * 32, v);
+                    ptx::wait32(v);
+                    if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    const int at = tg >= c * 32 && tg < c * 32 + 32 ? (int)tg - c * 32 : -1;
+                    const int at = on && tg >= c * 32 && tg < c * 32 + 32 ? (int)tg - c * 32 : -1;
+                    const bool any = __any_sync(0xffffffffu, at >= 0);
                     float hot = 0.0f;
-                    if (on && at >= 0) {
+                    if (any) {
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        hot = expm1f(x - x0 - x1);
+                        hot = expm1f(x - x0 - x1) * fabsf(g);
                     }
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        float z = ex2((v[j] - x0 - x1) * kLog2e);
-                        if (at == j) z = hot;
-                        v[j] = on ? z * g : 0.0f;
-                    }
+                    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - x0, kLog2e, add));
+                    if (any) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) w[j] = pack2<T>(v[2 * j], v[2 * j + 1]);
+                        for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
+                    }
+                    unsigned w[16];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) w[j] = (pack2<T>(v[2 * j], v[2 * j + 1]) & mask) ^ sign;
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, p.M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }
