@@ -72,9 +72,8 @@ def _weight(t, name: str, cols: int):
     return _matrix(t, name, cols)
 
 
-def _place(m):
-    """(address, row pitch)"""
-    return m.data_ptr(), m.stride(0) if m.shape[0] > 1 else m.shape[1]
+def _pitch(m) -> int:
+    return m.stride(0) if m.shape[0] > 1 else m.shape[1]
 
 
 def _same(first, **others):
@@ -92,7 +91,8 @@ def _activation(name: str) -> int:
 
 
 _entries: dict = {}
-_workspaces: dict = {}  # bytes an entry needs, by its sizes, pitches and alignments
+_plans: dict = {}  # what a call with these types, shapes and strides comes to
+_NOTHING = ctypes.byref(ctypes.c_size_t(0))
 
 
 def _entry(name: str):
@@ -106,22 +106,37 @@ def _stream(index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _run(name: str, dev, sizes, *args):
-    """One entry point that takes a workspace, on dev's current stream.
-    sizes: what the workspace depends on."""
+class _Plan:
+    """The checked form of a call: the entry's leading arguments, the row
+    pitches of its matrices, the result's shape, and the workspace it needs
+    by which addresses are on 16-byte boundaries."""
+    __slots__ = ("head", "pitches", "shape", "needs")
+
+    def __init__(self, head, pitches, shape):
+        self.head, self.pitches, self.shape, self.needs = head, pitches, shape, {}
+
+
+def _remember(key, plan):
+    if len(_plans) > 4096:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _run(name: str, like, needs, odd, *args):
+    """One entry point that takes a workspace, on the current stream of
+    like's device.  needs: the bytes it takes, by odd."""
     fn = _entry(name)
-    need = _workspaces.get(key := (name, sizes))
+    need = needs.get(odd)
     if need is None:
-        if len(_workspaces) > 4096:
-            _workspaces.clear()
         n = ctypes.c_size_t(0)
         _capi.check(fn(*args, None, ctypes.byref(n), 0))
-        need = _workspaces[key] = n.value
+        need = needs[odd] = n.value
     if need:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        rc = fn(*args, ws.data_ptr(), ctypes.byref(ctypes.c_size_t(need)), _stream(dev.index))
+        ws = like.new_empty(need, dtype=torch.uint8)
+        rc = fn(*args, ws.data_ptr(), ctypes.byref(ctypes.c_size_t(need)), _stream(args[0]))
     else:  # any aligned address will do
-        rc = fn(*args, 256, ctypes.byref(ctypes.c_size_t(0)), _stream(dev.index))
+        rc = fn(*args, 256, _NOTHING, _stream(args[0]))
     if rc:
         _capi.check(rc)
 
@@ -130,21 +145,33 @@ def _run(name: str, dev, sizes, *args):
 def gated_forward(x, w_gate, w_up, activation: str = "silu"):
     """act(x w_gate^T) * (x w_up^T), in one kernel; x [..., inner], weights
     [width, inner], the result [..., width]."""
-    act = _activation(activation)
-    xm = _matrix(x, "x")
-    inner = xm.shape[1]
-    wg, wu = _weight(w_gate, "w_gate", inner), _weight(w_up, "w_up", inner)
-    _same(xm, w_gate=wg, w_up=wu)
-    if wg.shape != wu.shape:
-        raise ValueError(f"w_gate {tuple(wg.shape)} and w_up {tuple(wu.shape)} differ in shape")
-    tokens, width = xm.shape[0], wg.shape[0]
-    if width < 1:
-        raise ValueError("the weights have no rows")
-    h = torch.empty(x.shape[:-1] + (width,), dtype=x.dtype, device=x.device)
-    dev = x.device
-    px, lx, pg, lg, pu, lu = *_place(xm), *_place(wg), *_place(wu)
-    _run("helrm_GatedForward", dev, (tokens, inner, width, px % 16, lx, pg % 16, lg, pu % 16, lu), dev.index,
-         _DTYPES[x.dtype], act, tokens, inner, width, px, lx, pg, lg, pu, lu, h.data_ptr())
+    try:
+        key = (activation, x.dtype, x.device, x.shape, x.stride(), w_gate.dtype, w_gate.device, w_gate.shape,
+               w_gate.stride(), w_up.dtype, w_up.device, w_up.shape, w_up.stride())
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        act = _activation(activation)
+        xm = _matrix(x, "x")
+        inner = xm.shape[1]
+        wg, wu = _weight(w_gate, "w_gate", inner), _weight(w_up, "w_up", inner)
+        _same(xm, w_gate=wg, w_up=wu)
+        if wg.shape != wu.shape:
+            raise ValueError(f"w_gate {tuple(wg.shape)} and w_up {tuple(wu.shape)} differ in shape")
+        width = wg.shape[0]
+        if width < 1:
+            raise ValueError("the weights have no rows")
+        plan = _Plan((x.device.index, _DTYPES[x.dtype], act, xm.shape[0], inner, width),
+                     (_pitch(xm), _pitch(wg), _pitch(wu)), x.shape[:-1] + (width,))
+        if xm.data_ptr() == x.data_ptr() and wg is w_gate and wu is w_up:
+            _remember(key, plan)
+        x, w_gate, w_up = xm, wg, wu  # the copies, where the strides asked for some
+    h = x.new_empty(plan.shape)
+    px, pg, pu = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
+    lx, lg, lu = plan.pitches
+    _run("helrm_GatedForward", x, plan.needs, (px & 15, pg & 15, pu & 15), *plan.head, px, lx, pg, lg, pu, lu,
+         h.data_ptr())
     return h
 
 
@@ -152,39 +179,50 @@ def gated_backward(dh, x, w_gate, w_up, activation: str = "silu", needs=(True, T
     """(dx, dw_gate, dw_up) from dh, the gradient by gated_forward's result.
     x is the block's input or its Checkpoint; the projections are formed
     again.  needs: which of the three are wanted (None in their place)."""
-    act = _activation(activation)
-    dhm = _matrix(dh, "dh")
     kept = isinstance(x, Checkpoint)
-    if kept:
-        shape, inner = tuple(x.shape), x.shape[-1]
-        _check_checkpoint(x)
-        if x.dtype != dhm.dtype or x.q.device != dhm.device:
-            raise ValueError(f"the checkpoint is {x.dtype} on {x.q.device}, dh {dhm.dtype} on {dhm.device}")
-        xm = None
-    else:
-        xm = _matrix(x, "x")
-        shape, inner = tuple(x.shape), xm.shape[1]
-        _same(dhm, x=xm)
-    wg, wu = _weight(w_gate, "w_gate", inner), _weight(w_up, "w_up", inner)
-    _same(dhm, w_gate=wg, w_up=wu)
-    if wg.shape != wu.shape:
-        raise ValueError(f"w_gate {tuple(wg.shape)} and w_up {tuple(wu.shape)} differ in shape")
-    tokens, width = dhm.shape
-    if tuple(dh.shape) != shape[:-1] + (wg.shape[0],):
-        raise ValueError(f"dh has shape {tuple(dh.shape)}, the block's result {shape[:-1] + (wg.shape[0],)}")
-    like = dict(dtype=dh.dtype, device=dh.device)
-    dx = torch.empty(shape, **like) if needs[0] else None
-    dwg = torch.empty((width, inner), **like) if needs[1] else None
-    dwu = torch.empty((width, inner), **like) if needs[2] else None
+    try:
+        xk = (x.q.dtype, x.q.device, x.q.shape, x.q.stride(), x.e.dtype, x.e.device, x.e.shape, x.e.stride(), x.shape,
+              x.dtype, x.q.data_ptr() & 15) if kept else (x.dtype, x.device, x.shape, x.stride())
+        key = (activation, tuple(needs), xk, dh.dtype, dh.device, dh.shape, dh.stride(), w_gate.dtype, w_gate.device,
+               w_gate.shape, w_gate.stride(), w_up.dtype, w_up.device, w_up.shape, w_up.stride())
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        act = _activation(activation)
+        dhm = _matrix(dh, "dh")
+        if kept:
+            _check_checkpoint(x)
+            xm, shape, inner, pitch = x, tuple(x.shape), x.shape[-1], x.shape[-1]
+            if x.dtype != dhm.dtype or x.q.device != dhm.device:
+                raise ValueError(f"the checkpoint is {x.dtype} on {x.q.device}, dh {dhm.dtype} on {dhm.device}")
+        else:
+            xm = _matrix(x, "x")
+            shape, inner, pitch = tuple(x.shape), xm.shape[1], _pitch(xm)
+            _same(dhm, x=xm)
+        wg, wu = _weight(w_gate, "w_gate", inner), _weight(w_up, "w_up", inner)
+        _same(dhm, w_gate=wg, w_up=wu)
+        if wg.shape != wu.shape:
+            raise ValueError(f"w_gate {tuple(wg.shape)} and w_up {tuple(wu.shape)} differ in shape")
+        tokens, width = dhm.shape
+        if tuple(dh.shape) != shape[:-1] + (wg.shape[0],):
+            raise ValueError(f"dh has shape {tuple(dh.shape)}, the block's result {shape[:-1] + (wg.shape[0],)}")
+        plan = _Plan((dh.device.index, _DTYPES[dh.dtype], act, tokens, inner, width),
+                     (_pitch(dhm), pitch, _pitch(wg), _pitch(wu)), (shape, (width, inner)))
+        if (dhm.data_ptr() == dh.data_ptr() and (kept or xm.data_ptr() == x.data_ptr()) and wg is w_gate
+                and wu is w_up):
+            _remember(key, plan)
+        dh, x, w_gate, w_up = dhm, xm, wg, wu  # the copies, where the strides asked for some
+    dx = dh.new_empty(plan.shape[0]) if needs[0] else None
+    dwg = dh.new_empty(plan.shape[1]) if needs[1] else None
+    dwu = dh.new_empty(plan.shape[1]) if needs[2] else None
     if any(needs):
-        dev = dh.device
-        px, lx = (0, inner) if kept else _place(xm)
-        pd, ld, pg, lg, pu, lu = *_place(dhm), *_place(wg), *_place(wu)
-        _run("helrm_GatedBackward", dev,
-             (tokens, inner, width, kept, px % 16, lx, pg % 16, lg, pu % 16, lu, *(bool(n) for n in needs)),
-             dev.index, _DTYPES[dh.dtype], act, tokens, inner, width, pd, ld, px or None, lx,
-             x.q.data_ptr() if kept else None, x.e.data_ptr() if kept else None, pg, lg, pu, lu,
-             *(None if t is None else t.data_ptr() for t in (dx, dwg, dwu)))
+        ld, lx, lg, lu = plan.pitches
+        pd, pg, pu = dh.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
+        px, pq, pe = (None, x.q.data_ptr(), x.e.data_ptr()) if kept else (x.data_ptr(), None, None)
+        _run("helrm_GatedBackward", dh, plan.needs, ((px or 0) & 15, pg & 15, pu & 15), *plan.head, pd, ld, px, lx, pq,
+             pe, pg, lg, pu, lu, None if dx is None else dx.data_ptr(), None if dwg is None else dwg.data_ptr(),
+             None if dwu is None else dwu.data_ptr())
     return dx, dwg, dwu
 
 
@@ -217,6 +255,9 @@ def gated_feed_forward(x, w_gate, w_up, activation: str = "silu", checkpoint: bo
 
 # ------------------------------------------------------------------ 8-bit checkpoints
 def _check_checkpoint(c):
+    q, e = c.q, c.e
+    if not isinstance(q, torch.Tensor) or not isinstance(e, torch.Tensor) or len(c.shape) < 1:
+        raise ValueError("not a checkpoint that pack_checkpoint returned")
     rows = 1
     for n in c.shape[:-1]:
         rows *= n
@@ -234,28 +275,46 @@ def pack_checkpoint(x) -> Checkpoint:
     power of two s with max |x| <= 127 s, the values are whole numbers of s
     (rounded, halves to even).  A group that holds an infinity or a NaN reads
     back as NaN."""
-    m = _matrix(x, "x")
-    rows, cols = m.shape
-    groups = -(-cols // GROUP)
-    q = torch.empty((rows, GROUP * groups), dtype=torch.int8, device=x.device)
-    e = torch.empty((rows, groups), dtype=torch.uint8, device=x.device)
-    dev = x.device.index
-    rc = _entry("helrm_PackCheckpoint")(dev, _DTYPES[x.dtype], rows, cols, *_place(m), q.data_ptr(), e.data_ptr(),
-                                        _stream(dev))
+    try:
+        key = ("pack", x.dtype, x.device, x.shape, x.stride())
+        plan = _plans.get(key)
+    except AttributeError:
+        key = plan = None
+    if plan is None:
+        m = _matrix(x, "x")
+        rows, cols = m.shape
+        groups = -(-cols // GROUP)
+        plan = _Plan((x.device.index, _DTYPES[x.dtype], rows, cols), _pitch(m),
+                     ((rows, GROUP * groups), (rows, groups), tuple(x.shape), x.dtype))
+        if m.data_ptr() == x.data_ptr():
+            _remember(key, plan)
+        x = m
+    shape_q, shape_e, shape, dtype = plan.shape
+    q, e = x.new_empty(shape_q, dtype=torch.int8), x.new_empty(shape_e, dtype=torch.uint8)
+    rc = _entry("helrm_PackCheckpoint")(*plan.head, x.data_ptr(), plan.pitches, q.data_ptr(), e.data_ptr(),
+                                        _stream(plan.head[0]))
     if rc:
         _capi.check(rc)
-    return Checkpoint(q, e, tuple(x.shape), x.dtype)
+    return Checkpoint(q, e, shape, dtype)
 
 
 def unpack_checkpoint(c: Checkpoint):
     """The tensor a checkpoint stands for, exact in its 16-bit type."""
     if not isinstance(c, Checkpoint):
         raise ValueError("not a checkpoint that pack_checkpoint returned")
-    rows = _check_checkpoint(c)
-    x = torch.empty(c.shape, dtype=c.dtype, device=c.q.device)
-    dev = x.device.index
-    rc = _entry("helrm_UnpackCheckpoint")(dev, _DTYPES[c.dtype], rows, c.shape[-1], c.q.data_ptr(), c.e.data_ptr(),
-                                          x.data_ptr(), _stream(dev))
+    q, e, shape, dtype = c
+    try:
+        key = ("unpack", q.dtype, q.device, q.shape, q.stride(), e.dtype, e.device, e.shape, e.stride(), shape, dtype,
+               q.data_ptr() & 15)
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        plan = _Plan((q.device.index, _DTYPES.get(dtype), _check_checkpoint(c), shape[-1]), None, shape)
+        _remember(key, plan)
+    x = q.new_empty(shape, dtype=dtype)
+    rc = _entry("helrm_UnpackCheckpoint")(*plan.head, q.data_ptr(), e.data_ptr(), x.data_ptr(),
+                                          _stream(plan.head[0]))
     if rc:
         _capi.check(rc)
     return x
@@ -273,9 +332,35 @@ def _targets(targets, lead, dev):
 
 
 def _floats(t, name: str, lead, dev):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev or tuple(t.shape) != tuple(lead):
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev or t.shape != lead:
         raise ValueError(f"{name} is not a float32 tensor of shape {tuple(lead)} on {dev}")
     return t.contiguous()
+
+
+def _loss_call(h, w, targets):
+    """(h, w, targets as the entries take them, the plan)"""
+    try:
+        key = ("loss", h.dtype, h.device, h.shape, h.stride(), w.dtype, w.device, w.shape, w.stride(), targets.dtype,
+               targets.device, targets.shape)
+        plan = _plans.get(key)
+    except (AttributeError, TypeError):
+        key = plan = None
+    if plan is None:
+        hm = _matrix(h, "h")
+        wm = _weight(w, "w", hm.shape[1])
+        _same(hm, w=wm)
+        if wm.shape[0] < 1:
+            raise ValueError("w has no rows")
+        lead = h.shape[:-1]
+        t = _targets(targets, lead, h.device)
+        plan = _Plan((h.device.index, _DTYPES[h.dtype], hm.shape[0], hm.shape[1], wm.shape[0]),
+                     (_pitch(hm), _pitch(wm)), (lead, h.shape, wm.shape, h.device))
+        if hm.data_ptr() == h.data_ptr() and wm is w:
+            _remember(key, plan)
+        return hm, wm, t, plan
+    if targets.dtype != torch.int64 or not targets.is_contiguous():
+        targets = targets.to(torch.int64).contiguous()
+    return h, w, targets, plan
 
 
 def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
@@ -284,42 +369,28 @@ def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
     the largest logit and the log of the sum relative to it.  h [..., inner],
     w [vocab, inner], targets [...].  Rows whose target is ignore_index have
     loss 0, other targets outside the vocabulary NaN."""
-    hm = _matrix(h, "h")
-    wm = _weight(w, "w", hm.shape[1])
-    _same(hm, w=wm)
-    if wm.shape[0] < 1:
-        raise ValueError("w has no rows")
-    t = _targets(targets, h.shape[:-1], h.device)
-    loss = torch.empty(h.shape[:-1], dtype=torch.float32, device=h.device)
-    lse = torch.empty(h.shape[:-1] + (2,), dtype=torch.float32, device=h.device)
-    dev, tokens, inner, vocab = h.device, hm.shape[0], hm.shape[1], wm.shape[0]
-    ph, lh, pw, lw = *_place(hm), *_place(wm)
-    _run("helrm_VocabularyLossForward", dev, (tokens, inner, vocab, ph % 16, lh, pw % 16, lw), dev.index,
-         _DTYPES[h.dtype], tokens, inner, vocab, ph, lh, pw, lw, t.data_ptr(), int(ignore_index), loss.data_ptr(),
-         lse.data_ptr())
+    h, w, t, plan = _loss_call(h, w, targets)
+    lead = plan.shape[0]
+    loss, lse = h.new_empty(lead, dtype=torch.float32), h.new_empty(lead + (2,), dtype=torch.float32)
+    ph, pw = h.data_ptr(), w.data_ptr()
+    _run("helrm_VocabularyLossForward", h, plan.needs, (ph & 15, pw & 15), *plan.head, ph, plan.pitches[0], pw,
+         plan.pitches[1], t.data_ptr(), int(ignore_index), loss.data_ptr(), lse.data_ptr())
     return loss, lse
 
 
 def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100, needs=(True, True)):
     """(dh, dw) from dloss [...] (float32) and vocabulary_loss_forward's lse.
     needs: which of the two are wanted (None in their place)."""
-    hm = _matrix(h, "h")
-    wm = _weight(w, "w", hm.shape[1])
-    _same(hm, w=wm)
-    if wm.shape[0] < 1:
-        raise ValueError("w has no rows")
-    lead, dev = h.shape[:-1], h.device
-    t = _targets(targets, lead, dev)
+    h, w, t, plan = _loss_call(h, w, targets)
+    lead, shape, shape_w, dev = plan.shape
     g, l = _floats(dloss, "dloss", lead, dev), _floats(lse, "lse", lead + (2,), dev)
-    dh = torch.empty(h.shape, dtype=h.dtype, device=dev) if needs[0] else None
-    dw = torch.empty(wm.shape, dtype=h.dtype, device=dev) if needs[1] else None
+    dh = h.new_empty(shape) if needs[0] else None
+    dw = h.new_empty(shape_w) if needs[1] else None
     if any(needs):
-        tokens, inner, vocab = hm.shape[0], hm.shape[1], wm.shape[0]
-        ph, lh, pw, lw = *_place(hm), *_place(wm)
-        _run("helrm_VocabularyLossBackward", dev,
-             (h.dtype, tokens, inner, vocab, ph % 16, lh, pw % 16, lw, bool(needs[0]), bool(needs[1])), dev.index,
-             _DTYPES[h.dtype], tokens, inner, vocab, g.data_ptr(), ph, lh, pw, lw, t.data_ptr(), l.data_ptr(),
-             int(ignore_index), *(None if o is None else o.data_ptr() for o in (dh, dw)))
+        ph, pw = h.data_ptr(), w.data_ptr()
+        _run("helrm_VocabularyLossBackward", h, plan.needs, (ph & 15, pw & 15, bool(needs[0]), bool(needs[1])),
+             *plan.head, g.data_ptr(), ph, plan.pitches[0], pw, plan.pitches[1], t.data_ptr(), l.data_ptr(),
+             int(ignore_index), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr())
     return dh, dw
 
 
