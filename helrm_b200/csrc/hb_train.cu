@@ -242,6 +242,7 @@ static void launch(const Product &d, cudaStream_t s) {
         set |= (uint64_t)1 << (dev & 63);
     }
     const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
+    require(items < (int64_t)1 << 31, "more than 2^31 tiles in one product");
     kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
              kProductSmem, s>>>(p);
     launched("training product");

@@ -61,12 +61,32 @@ constexpr float kLog2e = 1.4426950408889634f;
 // for small numerators (gated 64 x 432 x 512: 17.8 us with it, 8.1 without)
 __device__ __forceinline__ float sigmoid(float g) { return rcp(1.0f + ex2(-kLog2e * g)); }
 
+// The normal distribution function and density: Abramowitz and Stegun 7.1.26,
+// erfc(x) = (a1 t + .. + a5 t^5) exp(-x^2), t = 1 / (1 + 0.3275911 x), within
+// 1.5e-7, whose exponential the density needs anyway (with erff and a second
+// exponential the gated backward pass of 4096 x 1024 x 4096 took 92 us).
+__device__ __forceinline__ void normal(float g, float &cdf, float &pdf) {
+    const float x = fabsf(g) * 0.70710678118654752f, t = rcp(fmaf(0.3275911f, x, 1.0f));
+    const float e = ex2(g * g * (-0.5f * kLog2e));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    const float q = 0.5f * p * t * e;  // the smaller tail
+    cdf = g > 0.0f ? 1.0f - q : q;
+    pdf = 0.39894228040143268f * e;
+}
+
 // act(g), and with its derivative
 template <int ACT>
 __device__ __forceinline__ float act_f(float g) {
     if (ACT == HELRM_ACT_RELU) return fmaxf(g, 0.0f) + (g != g ? g : 0.0f);  // NaN stays NaN
     if (ACT == HELRM_ACT_SILU) return g * sigmoid(g);
-    if (ACT == HELRM_ACT_GELU) return 0.5f * g * (1.0f + erff(g * 0.70710678118654752f));
+    if (ACT == HELRM_ACT_GELU) {
+        float cdf, pdf;
+        normal(g, cdf, pdf);
+        return g * cdf;
+    }
     return g;
 }
 template <int ACT>
@@ -79,9 +99,10 @@ __device__ __forceinline__ void act_df(float g, float &a, float &d) {
         a = g * s;
         d = s * (1.0f + g * (1.0f - s));
     } else if (ACT == HELRM_ACT_GELU) {
-        const float p = 0.5f * (1.0f + erff(g * 0.70710678118654752f));
-        a = g * p;
-        d = p + g * 0.39894228040143268f * __expf(-0.5f * g * g);
+        float cdf, pdf;
+        normal(g, cdf, pdf);
+        a = g * cdf;
+        d = fmaf(g, pdf, cdf);
     } else {
         a = g;
         d = 1.0f;

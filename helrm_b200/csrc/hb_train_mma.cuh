@@ -153,6 +153,13 @@ __device__ __forceinline__ void store_block(unsigned char *st, const unsigned (&
         const unsigned char *from = st + block_at(lane >> 2, lane & 3);
 #pragma unroll
         for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(o + i * 8 * ld) = *reinterpret_cast<const uint4 *>(from + i * 512);
+    } else if (ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0 && n0 + 32 <= N) {
+        // rows on 8-byte boundaries: four of them at a time
+        const int rows = M - m0 < 32 ? (int)(M - m0) : 32;
+#pragma unroll 4
+        for (int r = lane >> 3; r < rows; r += 4)
+            *reinterpret_cast<uint2 *>(o + r * ld + (lane & 7) * 4) =
+                *reinterpret_cast<const uint2 *>(st + block_at(r, (lane & 7) >> 1) + (lane & 1) * 8);
     } else if (n0 + lane < N) {
         const int rows = M - m0 < 32 ? (int)(M - m0) : 32;
 #pragma unroll 4
@@ -170,8 +177,16 @@ __device__ __forceinline__ void load_block(unsigned char *st, unsigned (&v)[16],
         unsigned char *to = st + block_at(lane >> 2, lane & 3);
 #pragma unroll
         for (int i = 0; i < 4; i++) *reinterpret_cast<uint4 *>(to + i * 512) = *reinterpret_cast<const uint4 *>(p + i * 8 * ld);
+    } else if (ld % 4 == 0 && (reinterpret_cast<uintptr_t>(in) & 7) == 0 && n0 + 32 <= N) {
+        const int rows = M - m0 < 32 ? (int)(M - m0) : 32;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = i * 4 + (lane >> 3);
+            *reinterpret_cast<uint2 *>(st + block_at(r, (lane & 7) >> 1) + (lane & 1) * 8) =
+                r < rows ? *reinterpret_cast<const uint2 *>(p + r * ld + (lane & 7) * 4) : make_uint2(0, 0);
+        }
     } else {
-#pragma unroll 4
+#pragma unroll 16
         for (int r = 0; r < 32; r++)
             *reinterpret_cast<unsigned short *>(st + block_at(r, lane >> 3) + (lane & 7) * 2) =
                 m0 + r < M && n0 + lane < N ? p[r * ld + lane] : (unsigned short)0;
@@ -252,28 +267,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     tc::fence_after();
     const unsigned tmem = *s_tmem;
 
-    const int tiles = p.tiles_m * p.tiles_n;
-    const int64_t items = (int64_t)tiles * p.splits * p.outputs;
+    // The launch has fewer than 2^31 items, so that all of this is 32-bit
+    // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
+    const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+    const unsigned items = tiles * p.splits * p.outputs;
     const int depth = p.kb + p.kb1;
-    const int64_t first_item = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const unsigned first_item = blockIdx.x >> 1, step = gridDim.x >> 1;
     struct Item {
         int out, split, mt, nt, k0, k1;
     };
     // Tiles go down groups of 8 tile rows, column after column, so that the
     // clusters at work share a few panels of A and of B in L2.
-    auto item = [&](int64_t i) {
+    auto item = [&](unsigned i) {
         Item t;
-        int r = (int)(i % tiles);
-        const int64_t q = i / tiles;
-        t.split = (int)(q % p.splits);
-        t.out = (int)(q / p.splits);
-        const int per = 8 * p.tiles_n, g = r / per;
-        r -= g * per;
-        const int h = p.tiles_m - g * 8 < 8 ? p.tiles_m - g * 8 : 8;
-        t.mt = g * 8 + r % h;
-        t.nt = r / h;
-        t.k0 = (int)((int64_t)depth * t.split / p.splits);
-        t.k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        t.out = t.split = t.k0 = 0;
+        t.k1 = depth;
+        if (items > tiles) {
+            unsigned q = i / tiles;
+            i -= q * tiles;
+            t.out = q / p.splits;
+            t.split = q - t.out * p.splits;
+            t.k0 = (int)((int64_t)depth * t.split / p.splits);
+            t.k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        }
+        const unsigned per = 8u * p.tiles_n, g = p.tiles_m > 8 ? i / per : 0;
+        const unsigned r = i - g * per, h = p.tiles_m - g * 8;
+        if (h >= 8) {
+            t.mt = g * 8 + (r & 7);
+            t.nt = r >> 3;
+        } else {
+            t.nt = r / h;
+            t.mt = g * 8 + (r - t.nt * h);
+        }
         return t;
     };
 
@@ -284,7 +309,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             unsigned ph = 0;
             int64_t loads = 0;
             bool ok = true;
-            for (int64_t i = first_item; ok && i < items; i += step) {
+            for (unsigned i = first_item; ok && i < items; i += step) {
                 const Item t = item(i);
                 const int m = t.mt * kRows + 128 * (int)rank;
                 const int n = kDual ? t.nt * 128 : t.nt * kCols + 128 * (int)rank;
@@ -336,9 +361,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             constexpr unsigned ka = AMAJ == K_MAJOR ? 32 : 2048, kb = BMAJ == K_MAJOR ? 32 : 2048;
             int s = 0;
             unsigned ph = 0;
-            int64_t n = 0;
+            unsigned n = 0;
             bool ok = true;
-            for (int64_t i = first_item; ok && i < items; i += step, n++) {
+            for (unsigned i = first_item; ok && i < items; i += step, n++) {
                 const Item t = item(i);
                 const int buf = (int)(n & 1);
                 if (!tc::mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2, kWaitNs)) break;
@@ -370,9 +395,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
         const EpiArgs &e = p.e;
-        int64_t cnt = 0;
-        for (int64_t i = first_item; i < items; i += step, cnt++) {
+        unsigned cnt = 0;
+        // What the loss needs to know of this lane's row, fetched a tile ahead.
+        struct Row {
+            int64_t target = -1;
+            float dloss = 0.0f;
+            float2 lse = {0.0f, 0.0f};
+        };
+        auto fetch = [&](unsigned i) {
+            Row r;
+            if ((EPI == EPI_LSE || EPI == EPI_Z) && i < items) {
+                const int64_t m = (int64_t)item(i).mt * kRows + 128 * rank + 32 * quad + lane;
+                if (m < p.M) {
+                    r.target = e.target[m];
+                    if (EPI == EPI_Z) r.dloss = e.dloss[m], r.lse = e.lse[m];
+                }
+            }
+            return r;
+        };
+        Row next = fetch(first_item);
+        for (unsigned i = first_item; i < items; i += step, cnt++) {
             const Item t = item(i);
+            const Row row = next;
+            next = fetch(i + step);
             const int buf = (int)(cnt & 1);
             const int64_t m0 = (int64_t)t.mt * kRows + 128 * rank + 32 * quad, m = m0 + lane;
             const unsigned acc = tmem + ((unsigned)(32 * quad) << 16) + buf * kCols;
@@ -446,7 +491,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             } else if constexpr (EPI == EPI_LSE) {
                 constexpr int kWide = kCols / (kWarps / 4);  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
-                const int64_t tg = m < p.M ? e.target[m] - n0 : -1;
+                const int64_t tg = row.target - n0;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
@@ -456,12 +501,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     if (c == kWide / 32 - 1) release();
                     const int left = (int)(p.N - n0 < kWide ? p.N - n0 : kWide) - c * 32;  // columns that exist
                     if (left < 32) {
+                        asm volatile("");  // a branch, not 32 selections in every tile
 #pragma unroll
                         for (int j = 0; j < 32; j++)
                             if (j >= left) v[j] = -INFINITY;
                     }
                     const int at = tg >= c * 32 && tg < c * 32 + 32 && tg < c * 32 + left ? (int)tg - c * 32 : -1;
                     if (__any_sync(0xffffffffu, at >= 0)) {
+                        asm volatile("");
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
@@ -490,20 +537,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 // z = g exp(v - x0 - x1) = sign 2^((v - x0) log2(e) + c): the difference to the row's maximum is exact
                 // where it matters, and |g| costs nothing.  Sign and rows without a target go over the packed words.
-                int64_t tg = -1;
-                float g = 0.0f, x0 = 0.0f, x1 = 0.0f;
-                bool on = false;
-                if (m < p.M) {
-                    tg = e.target[m];
-                    on = tg != e.ignore;
-                    if (on) {
-                        g = tg < 0 || tg >= e.vocab ? NAN : e.dloss[m];
-                        if (e.shift) g = ldexpf(g, *e.shift);
-                        const float2 l = e.lse[m];
-                        x0 = l.x, x1 = l.y;
-                    }
-                    tg -= e.col0 + n0;
+                const bool on = m < p.M && row.target != e.ignore;
+                float g = 0.0f;
+                if (on) {
+                    g = row.target < 0 || row.target >= e.vocab ? NAN : row.dloss;
+                    if (e.shift) g = ldexpf(g, *e.shift);
                 }
+                const float x0 = on ? row.lse.x : 0.0f, x1 = on ? row.lse.y : 0.0f;
+                const int64_t tg = row.target - e.col0 - n0;
                 const float add = log2f(fabsf(g)) - x1 * kLog2e;
                 const unsigned mask = on ? 0xffffffffu : 0u, sign = on && g < 0.0f ? 0x80008000u : 0u;
 #pragma unroll 1
@@ -517,6 +558,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     const bool any = __any_sync(0xffffffffu, at >= 0);
                     float hot = 0.0f;
                     if (any) {
+                        asm volatile("");
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
@@ -525,6 +567,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 #pragma unroll
                     for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - x0, kLog2e, add));
                     if (any) {
+                        asm volatile("");
 #pragma unroll
                         for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
                     }
