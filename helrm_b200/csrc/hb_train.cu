@@ -9,6 +9,7 @@
 #include "hb_kernels.cuh"
 #include "hb_train.cuh"
 #include "hb_train_mma.cuh"
+#include "hb_train_loss.cuh"
 
 namespace hb {
 namespace train {
@@ -128,6 +129,17 @@ static int sm_count() {
     return n;
 }
 
+// Raises a kernel's shared-memory limit, once for each kernel and device.
+template <auto KERNEL>
+static void raise_shared_memory(int bytes) {
+    static std::atomic<uint64_t> set{0};
+    int dev = 0;
+    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    if (set >> (dev & 63) & 1) return;
+    cuda_check(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory");
+    set |= (uint64_t)1 << (dev & 63);
+}
+
 // A row-major 16-bit matrix.
 struct Matrix {
     const void *p = nullptr;
@@ -233,14 +245,8 @@ static void launch(const Product &d, cudaStream_t s) {
     p.kb1 = (int)blocks(d.K1, kDepth);
     p.e = d.e;
     p.error = runtime().error;
-    static std::atomic<uint64_t> set{0};  // devices whose shared-memory limit is raised for this kernel
-    int dev = 0;
-    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
     auto kernel = k_mma_product<T, AMAJ, BMAJ, EPI, ACT>;
-    if (!(set >> (dev & 63) & 1)) {
-        cuda_check(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kProductSmem), "shared memory");
-        set |= (uint64_t)1 << (dev & 63);
-    }
+    raise_shared_memory<k_mma_product<T, AMAJ, BMAJ, EPI, ACT>>(kProductSmem);
     const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
     require(items < (int64_t)1 << 31, "more than 2^31 tiles in one product");
     kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
@@ -299,6 +305,21 @@ static void by_act(int act, F &&f) {
         case HELRM_ACT_GELU: f(std::integral_constant<int, HELRM_ACT_GELU>()); break;
         default: HB_THROW(HB_EINVAL, "unknown activation");
     }
+}
+
+// Whether the loss's gradients come from the kernel that keeps Z in shared
+// memory, and its shape.
+struct Narrow {
+    bool on = false;
+    int depth = 0, group = 0, grid = 0;
+};
+static Narrow narrow(int64_t tokens, int64_t inner, int64_t vocab) {
+    Narrow n;
+    n.depth = (int)pad(inner, 16);
+    n.group = 128 / n.depth;
+    n.grid = 148;
+    n.on = inner <= kNarrow && vocab >= 128 * 148 && tokens * n.depth <= (1 << 19);
+    return n;
 }
 
 // Columns of a vocabulary piece: Z of a piece takes at most 256 MiB.
@@ -503,6 +524,48 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
         const Matrix mh = in.fit({h, tokens, inner, ldh}), mw = in.fit({wt, vocab, inner, ldw});
+        const Narrow nr = narrow(tokens, inner, vocab);
+        if (nr.on) {
+            const int groups = (int)blocks(blocks(tokens, 128), nr.group);
+            float *part = w.take<float>((int64_t)nr.grid * tokens * nr.depth);
+            float *acc = w.take<float>(groups > 1 ? vocab * nr.depth : 0);
+            int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
+            void *dws = dw ? dw : w.take<uint16_t>(vocab * inner);
+            if (sized(w, ws_bytes)) return;
+            DeviceGuard dev(device);
+            cudaStream_t s = (cudaStream_t)stream;
+            if (tokens == 0) {
+                if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
+                return;
+            }
+            in.copy(s);
+            if (dtype == HELRM_FP16) {
+                k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
+                launched("loss shift");
+            }
+            by_dtype(dtype, [&](auto t) {
+                typedef decltype(t) T;
+                NarrowArgs a;
+                a.h = tensor_map(mh, std::is_same<T, __nv_bfloat16>::value, K_MAJOR);
+                a.w = tensor_map(mw, std::is_same<T, __nv_bfloat16>::value, K_MAJOR);
+                a.tokens = tokens, a.vocab = vocab;
+                a.inner = (int)inner, a.depth = nr.depth, a.group = nr.group;
+                a.target = targets;
+                a.lse = reinterpret_cast<const float2 *>(lse);
+                a.dloss = dloss;
+                a.shift = dtype == HELRM_FP16 ? shift : nullptr;
+                a.ignore = ignore_index;
+                a.dw = dws;
+                a.acc_w = acc;
+                a.part_h = part;
+                a.error = runtime().error;
+                raise_shared_memory<k_loss_grads_narrow<T>>(kNarrowSmem);
+                k_loss_grads_narrow<T><<<nr.grid, kNarrowThreads, kNarrowSmem, s>>>(a);
+                launched("loss gradients");
+                if (dh) join<T>(part, nr.grid, tokens, inner, nr.depth, a.shift, dh, s);
+            });
+            return;
+        }
         const int64_t cols = piece_columns(tokens, vocab), ldz = pitch(cols), lda = pad(inner, 4);
         uint16_t *z = w.take<uint16_t>(tokens * ldz);
         // dh over several pieces is a 32-bit sum; the parts of a piece's depth each keep their own

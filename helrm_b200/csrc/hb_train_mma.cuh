@@ -86,10 +86,10 @@ __device__ __forceinline__ void tma_load(unsigned dst, const CUtensorMap *map, i
         : "memory");
 }
 // Shared-memory matrix descriptor with the 128-byte swizzle.  K-major: rows of
-// 128 bytes, groups of 8 rows 1024 bytes apart.  MN-major: columns of 64
-// elements (128 bytes) 8192 bytes apart, groups of 8 k 1024 bytes apart.
-__device__ __forceinline__ uint64_t descriptor(unsigned addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(8192 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+// 128 bytes, groups of 8 rows 1024 bytes apart.  MN-major: panels of 64
+// elements (128 bytes) `panel` bytes apart, groups of 8 k 1024 bytes apart.
+__device__ __forceinline__ uint64_t descriptor(unsigned addr, unsigned panel = 8192) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
            ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 __device__ __forceinline__ void mma(unsigned d, uint64_t a, uint64_t b, unsigned idesc, unsigned accumulate) {

@@ -353,8 +353,12 @@ LOSSES = [(1, 1, 1), (1, 16, 3), (2, 13, 1000), (64, 64, 1000), (127, 8, 129), (
           (300, 432, 5003), (777, 24, 2049), (256, 16, 40001), (33, 1025, 130)]
 
 
+# narrow rows over a vocabulary of every block's share: one token tile and several groups of them, every depth
+NARROW = [(64, 3, 30000), (1, 16, 19000), (1025, 16, 20001), (1000, 24, 18944), (130, 64, 19457), (2000, 50, 19001)]
+
+
 @pytest.mark.parametrize("dt", ["bf16", "fp16"])
-@pytest.mark.parametrize("shape", LOSSES)
+@pytest.mark.parametrize("shape", LOSSES + NARROW)
 def test_loss(tr, shape, dt):
     n, k, v = shape
     dt = DTYPES[dt]
