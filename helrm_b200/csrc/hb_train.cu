@@ -524,12 +524,23 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
         const Matrix mh = in.fit({h, tokens, inner, ldh}), mw = in.fit({wt, vocab, inner, ldw});
+        LossRow *rows = w.take<LossRow>(tokens);
+        int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
+        if (dtype != HELRM_FP16) shift = nullptr;
+        auto prepare = [&](cudaStream_t s) {
+            if (shift) {
+                k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
+                launched("loss shift");
+            }
+            k_loss_rows<<<blocks(tokens, 256), 256, 0, s>>>(dloss, targets, reinterpret_cast<const float2 *>(lse),
+                                                            ignore_index, vocab, tokens, shift, rows);
+            launched("loss rows");
+        };
         const Narrow nr = narrow(tokens, inner, vocab);
         if (nr.on) {
             const int groups = (int)blocks(blocks(tokens, 128), nr.group);
             float *part = w.take<float>((int64_t)nr.grid * tokens * nr.depth);
             float *acc = w.take<float>(groups > 1 ? vocab * nr.depth : 0);
-            int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
             void *dws = dw ? dw : w.take<uint16_t>(vocab * inner);
             if (sized(w, ws_bytes)) return;
             DeviceGuard dev(device);
@@ -539,10 +550,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 return;
             }
             in.copy(s);
-            if (dtype == HELRM_FP16) {
-                k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
-                launched("loss shift");
-            }
+            prepare(s);
             by_dtype(dtype, [&](auto t) {
                 typedef decltype(t) T;
                 NarrowArgs a;
@@ -550,11 +558,9 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 a.w = tensor_map(mw, std::is_same<T, __nv_bfloat16>::value, K_MAJOR);
                 a.tokens = tokens, a.vocab = vocab;
                 a.inner = (int)inner, a.depth = nr.depth, a.group = nr.group;
-                a.target = targets;
+                a.rows = rows;
                 a.lse = reinterpret_cast<const float2 *>(lse);
-                a.dloss = dloss;
-                a.shift = dtype == HELRM_FP16 ? shift : nullptr;
-                a.ignore = ignore_index;
+                a.shift = shift;
                 a.dw = dws;
                 a.acc_w = acc;
                 a.part_h = part;
@@ -573,7 +579,6 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         const bool summed = dh && (cols < vocab || parts_h > 1);
         float *acc = w.take<float>(summed ? parts_h * tokens * lda : 0);
         float *acc_w = w.take<float>(sums(cols, inner, parts_w, 1));
-        int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
@@ -582,11 +587,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             return;
         }
         in.copy(s);
-        const bool scaled = dtype == HELRM_FP16;
-        if (scaled) {
-            k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
-            launched("loss shift");
-        }
+        prepare(s);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             for (int64_t c0 = 0; c0 < vocab; c0 += cols) {
@@ -595,23 +596,20 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 Product d;
                 d.a = mh, d.b = mc;
                 d.M = tokens, d.N = n, d.K = inner;
-                d.e.shift = scaled ? shift : nullptr;
+                d.e.shift = shift;
                 d.e.o0 = z;
                 d.e.ldo = ldz;
                 d.e.vec = 1;
-                d.e.target = targets;
+                d.e.rows = rows;
                 d.e.lse = reinterpret_cast<const float2 *>(lse);
-                d.e.dloss = dloss;
-                d.e.ignore = ignore_index;
                 d.e.col0 = c0;
-                d.e.vocab = vocab;
                 launch<T, K_MAJOR, K_MAJOR, EPI_Z, 0>(d, s);
                 if (dw) {
                     Product g;
                     g.a = mz, g.b = mh;
                     g.M = n, g.N = inner, g.K = tokens;
                     g.splits = parts_w;
-                    g.e.shift = scaled ? shift : nullptr;
+                    g.e.shift = shift;
                     void *out = static_cast<T *>(dw) + c0 * inner;
                     product_out<T, MN_MAJOR, MN_MAJOR>(g, &out, acc_w, s);
                 }
@@ -619,7 +617,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                     Product g;
                     g.a = mz, g.b = mc;
                     g.M = tokens, g.N = inner, g.K = n;
-                    g.e.shift = scaled ? shift : nullptr;
+                    g.e.shift = shift;
                     if (summed) {
                         // the last piece may be too short for every part: those keep their sums
                         g.splits = parts_h < (int)blocks(n, kDepth) ? parts_h : (int)blocks(n, kDepth);
@@ -632,7 +630,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                     }
                 }
             }
-            if (summed) join<T>(acc, parts_h, tokens, inner, lda, scaled ? shift : nullptr, dh, s);
+            if (summed) join<T>(acc, parts_h, tokens, inner, lda, shift, dh, s);
         });
     });
 }

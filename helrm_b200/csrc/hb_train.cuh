@@ -123,9 +123,8 @@ struct EpiArgs {
     float *at = nullptr;                // EPI_LSE: the target's logit
     const int64_t *target = nullptr;
     const float2 *lse = nullptr;        // EPI_Z: the row's (maximum, log of the sum relative to it)
-    const float *dloss = nullptr;
-    int64_t ignore = 0, col0 = 0;       // first column of the piece in the vocabulary of
-    int64_t vocab = 0;                  // this many
+    const struct LossRow *rows = nullptr;
+    int64_t col0 = 0;                   // EPI_Z: first column of the piece in the vocabulary
     const int *shift = nullptr;         // Z is scaled by 2^shift, undone when the products with it are stored
 };
 
@@ -176,6 +175,32 @@ __global__ void __launch_bounds__(1024) k_loss(const float2 *__restrict__ part, 
     loss[m] = t == ignore ? 0.0f : t < 0 || t >= vocab ? NAN : top - at[m] + l;
 }
 
+// What the gradients' epilogues need to know of a row, in one 16-byte load:
+// z = g exp(l - max - x1) = sign(g) 2^((l - max) log2(e) + add).  A row without
+// a target has target kNoTarget, one whose target is out of range g = NaN.
+struct LossRow {
+    float max, add, g;
+    int target;
+};
+constexpr int kNoTarget = -2147483647 - 1;
+__global__ void k_loss_rows(const float *__restrict__ dloss, const int64_t *__restrict__ target,
+                            const float2 *__restrict__ lse, int64_t ignore, int64_t vocab, int64_t M,
+                            const int *__restrict__ shift, LossRow *__restrict__ rows) {
+    const int64_t m = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (m >= M) return;
+    LossRow r = {0.0f, 0.0f, 0.0f, kNoTarget};
+    const int64_t t = target[m];
+    if (t != ignore) {
+        const float2 l = lse[m];
+        r.g = t < 0 || t >= vocab ? NAN : dloss[m];
+        if (shift) r.g = ldexpf(r.g, *shift);
+        r.max = l.x;
+        r.add = log2f(fabsf(r.g)) - l.y * kLog2e;
+        r.target = t < 0 || t >= vocab ? -1 : (int)t;
+    }
+    rows[m] = r;
+}
+
 // fp16 only: the power of two that brings the largest |dloss| of a row that
 // takes part to [2^14, 2^15), so that Z keeps the probabilities down to 2^-38.
 __global__ void k_loss_shift(const float *__restrict__ dloss, const int64_t *__restrict__ target, int64_t ignore,
@@ -191,6 +216,33 @@ __global__ void k_loss_shift(const float *__restrict__ dloss, const int64_t *__r
         for (unsigned i = 1; i < blockDim.x / 32; i++) top = fmaxf(top, red[i]);
         *shift = top > 0.0f && top < INFINITY ? max(-100, min(120, 14 - ilogbf(top))) : 0;
     }
+}
+
+// 32 logits of a row, the first of them column `col` of the vocabulary, to Z,
+// packed in 16 words.  The target's exp(..) - 1 is formed without cancellation.
+template <class T>
+__device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col,
+                                       const float2 *__restrict__ lse, int64_t m) {
+    const int at = r.target >= col && r.target < col + 32 ? r.target - col : -1;
+    const bool any = __any_sync(0xffffffffu, at >= 0);
+    float hot = 0.0f;
+    if (any) {
+        asm volatile("");  // a branch: not 32 selections for every 32 logits
+        float x = v[0];
+#pragma unroll
+        for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
+        if (at >= 0) hot = expm1f(x - r.max - lse[m].y) * fabsf(r.g);
+    }
+#pragma unroll
+    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - r.max, kLog2e, r.add));
+    if (any) {
+        asm volatile("");
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
+    }
+    const unsigned mask = r.target == kNoTarget ? 0u : 0xffffffffu, sign = r.g < 0.0f ? 0x80008000u : 0u;
+#pragma unroll
+    for (int j = 0; j < 16; j++) w[j] = (pack2<T>(v[2 * j], v[2 * j + 1]) & mask) ^ sign;
 }
 
 // ---------------------------------------------------------------- checkpoints

@@ -32,18 +32,16 @@ constexpr int kNarrowGroup = 8;       // token tiles of a group at most
 constexpr int kNarrowWarps = 16;      // epilogue warps
 constexpr int kNarrowThreads = 64 + 32 * kNarrowWarps;
 constexpr int kPanel = 128 * 128;     // bytes of 128 rows of 64 elements
-constexpr int kNarrowBars = 2 + 2 * 10 + 2;
+constexpr int kNarrowBars = 2 + 2 * 7 + 2;
 constexpr int kNarrowSmem = (kNarrowGroup + 2 + 4) * kPanel + 8 * kNarrowBars + 16;
 
 struct NarrowArgs {
     CUtensorMap h, w;
     int64_t tokens, vocab;
     int inner, depth, group;  // depth: inner rounded up to 16; group: token tiles of a group
-    const int64_t *target;
+    const LossRow *rows;
     const float2 *lse;
-    const float *dloss;
     const int *shift;
-    int64_t ignore;
     void *dw;                 // dense rows
     float *acc_w;             // [vocab][depth] running sums, for several groups
     float *part_h;            // [block][tokens][depth]
@@ -93,8 +91,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (kNarrowGroup + 6) * kPanel);
     const unsigned bar = tc::smem_u32(bars);
     const unsigned hfull = bar, dhfull = bar + 8, wfull = bar + 16, wempty = bar + 32, sfull = bar + 48,
-                   sempty = bar + 64, zfull = bar + 80, zempty = bar + 96, dwfull = bar + 112, dwempty = bar + 128,
-                   dhempty = bar + 144, drain = bar + 152;
+                   sempty = bar + 64, zfull = bar + 80, dwfull = bar + 96, dwempty = bar + 112, dhempty = bar + 128,
+                   drain = bar + 136;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(bars + kNarrowBars);
     int *s_error = reinterpret_cast<int *>(s_tmem + 1);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 2);
@@ -109,7 +107,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             tc::mbar_init(sfull + 8 * i, 1);
             tc::mbar_init(sempty + 8 * i, kNarrowWarps);
             tc::mbar_init(zfull + 8 * i, kNarrowWarps);
-            tc::mbar_init(zempty + 8 * i, 1);
             tc::mbar_init(dwfull + 8 * i, 1);
             tc::mbar_init(dwempty + 8 * i, kNarrowWarps);
         }
@@ -206,7 +203,6 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         ptx::mma_own(dh, zk + (k >> 2) * (kPanel >> 4) + 2 * (k & 3), wb + 128 * k, idh, b > 0 || k > 0);
-                    ptx::commit(zempty + 8 * (n & 1));
                     if (++t == tiles) {
                         t = 0;
                         ptx::commit(wempty + 8 * (nb & 1));
@@ -231,24 +227,9 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         };
         const float unscale = p.shift ? ldexpf(1.0f, -*p.shift) : 1.0f;
         const bool vec = p.inner % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dw) & 15) == 0;
-        struct Row {
-            int64_t target = 0;
-            float x0 = 0.0f, x1 = 0.0f, g = 0.0f;
-            bool on = false;
-        };
         auto fetch = [&](int64_t m) {
-            Row q;
-            if (m < p.tokens) {
-                q.target = p.target[m];
-                q.on = q.target != p.ignore;
-                if (q.on) {
-                    q.g = q.target < 0 || q.target >= p.vocab ? NAN : p.dloss[m];
-                    if (p.shift) q.g = ldexpf(q.g, *p.shift);
-                    const float2 l = p.lse[m];
-                    q.x0 = l.x;
-                    q.x1 = l.y;
-                }
-            }
+            LossRow q = {0.0f, 0.0f, 0.0f, kNoTarget};
+            if (m < p.tokens) *reinterpret_cast<float4 *>(&q) = reinterpret_cast<const float4 *>(p.rows)[m];
             return q;
         };
         // dW of the block that was finished last: 16 of its columns a warp
@@ -293,44 +274,23 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         for (int g = 0; ok && g < groups; g++) {
             const int tiles = min(p.group, token_tiles - g * p.group);
             const int64_t first = (int64_t)g * p.group * 128 + r;
-            Row next = fetch(first);
+            LossRow next = fetch(first);
             for (int b = 0; ok && b < mine; b++) {
                 const int64_t block = blockIdx.x + (int64_t)b * gridDim.x;
                 for (int t = 0; t < tiles; t++, n++) {
-                    const Row row = next;
+                    const LossRow row = next;
                     next = fetch(first + (t + 1 < tiles ? t + 1 : 0) * 128);
-                    const float add = log2f(fabsf(row.g)) - row.x1 * kLog2e;
-                    const unsigned mask = row.on ? 0xffffffffu : 0u, sign = row.on && row.g < 0.0f ? 0x80008000u : 0u;
-                    const int64_t tg = row.target - block * 128 - quarter * 32;
-                    const int at = row.on && tg >= 0 && tg < 32 ? (int)tg : -1;
+                    // S was issued after the products that read this Z buffer last: it is free too
                     if (!(ok = wait_all(sfull + 8 * (n & 1), (n >> 1) & 1))) break;
                     tc::fence_after();
                     float v[32];
+                    unsigned w[16];
                     ptx::load32(tS + (n & 1) * 128 + lanes + quarter * 32, v);
                     ptx::wait32(v);
                     tc::fence_before();
                     __syncwarp();
                     if (lane == 0) tc::mbar_arrive(sempty + 8 * (n & 1));
-                    const bool any = __any_sync(0xffffffffu, at >= 0);
-                    float hot = 0.0f;
-                    if (any) {
-                        asm volatile("");
-                        float x = v[0];
-#pragma unroll
-                        for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        hot = expm1f(x - row.x0 - row.x1) * fabsf(row.g);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - row.x0, kLog2e, add));
-                    if (any) {
-                        asm volatile("");
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
-                    }
-                    unsigned w[16];
-#pragma unroll
-                    for (int j = 0; j < 16; j++) w[j] = (pack2<T>(v[2 * j], v[2 * j + 1]) & mask) ^ sign;
-                    if (!(ok = wait_all(zempty + 8 * (n & 1), ((n >> 1) & 1) ^ 1))) break;
+                    loss_z<T>(v, w, row, (int)(block * 128) + quarter * 32, p.lse, first + t * 128);
                     unsigned char *z = zbuf + (n & 1) * 2 * kPanel + (quarter >> 1) * kPanel + r * 128;
 #pragma unroll
                     for (int j = 0; j < 4; j++)

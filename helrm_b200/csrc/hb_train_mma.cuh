@@ -397,27 +397,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         const EpiArgs &e = p.e;
         unsigned cnt = 0;
         // What the loss needs to know of this lane's row, fetched a tile ahead.
-        struct Row {
-            int64_t target = -1;
-            float dloss = 0.0f;
-            float2 lse = {0.0f, 0.0f};
+        int64_t next_target = -1;
+        LossRow next_row = {0.0f, 0.0f, 0.0f, kNoTarget};
+        Item next = item(first_item);
+        auto fetch = [&] {
+            const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
+            if (EPI == EPI_LSE) next_target = m < p.M ? e.target[m] : -1;
+            if (EPI == EPI_Z && m < p.M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
-        auto fetch = [&](unsigned i) {
-            Row r;
-            if ((EPI == EPI_LSE || EPI == EPI_Z) && i < items) {
-                const int64_t m = (int64_t)item(i).mt * kRows + 128 * rank + 32 * quad + lane;
-                if (m < p.M) {
-                    r.target = e.target[m];
-                    if (EPI == EPI_Z) r.dloss = e.dloss[m], r.lse = e.lse[m];
-                }
-            }
-            return r;
-        };
-        Row next = fetch(first_item);
+        if (first_item < items) fetch();
         for (unsigned i = first_item; i < items; i += step, cnt++) {
-            const Item t = item(i);
-            const Row row = next;
-            next = fetch(i + step);
+            const Item t = next;
+            const int64_t target = next_target;
+            const LossRow row = next_row;
+            if (i + step < items) {
+                next = item(i + step);
+                fetch();
+            }
             const int buf = (int)(cnt & 1);
             const int64_t m0 = (int64_t)t.mt * kRows + 128 * rank + 32 * quad, m = m0 + lane;
             const unsigned acc = tmem + ((unsigned)(32 * quad) << 16) + buf * kCols;
@@ -491,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             } else if constexpr (EPI == EPI_LSE) {
                 constexpr int kWide = kCols / (kWarps / 4);  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
-                const int64_t tg = row.target - n0;
+                const int64_t tg = target - n0;
                 float top = -INFINITY, sum = 0.0f;
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
@@ -535,45 +531,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / (kWarps / 4);
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
-                // z = g exp(v - x0 - x1) = sign 2^((v - x0) log2(e) + c): the difference to the row's maximum is exact
-                // where it matters, and |g| costs nothing.  Sign and rows without a target go over the packed words.
-                const bool on = m < p.M && row.target != e.ignore;
-                float g = 0.0f;
-                if (on) {
-                    g = row.target < 0 || row.target >= e.vocab ? NAN : row.dloss;
-                    if (e.shift) g = ldexpf(g, *e.shift);
-                }
-                const float x0 = on ? row.lse.x : 0.0f, x1 = on ? row.lse.y : 0.0f;
-                const int64_t tg = row.target - e.col0 - n0;
-                const float add = log2f(fabsf(g)) - x1 * kLog2e;
-                const unsigned mask = on ? 0xffffffffu : 0u, sign = on && g < 0.0f ? 0x80008000u : 0u;
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
                     float v[32];
+                    unsigned w[16];
                     ptx::load32(acc + half * kWide + c * 32, v);
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    const int at = on && tg >= c * 32 && tg < c * 32 + 32 ? (int)tg - c * 32 : -1;
-                    const bool any = __any_sync(0xffffffffu, at >= 0);
-                    float hot = 0.0f;
-                    if (any) {
-                        asm volatile("");
-                        float x = v[0];
-#pragma unroll
-                        for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        hot = expm1f(x - x0 - x1) * fabsf(g);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - x0, kLog2e, add));
-                    if (any) {
-                        asm volatile("");
-#pragma unroll
-                        for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
-                    }
-                    unsigned w[16];
-#pragma unroll
-                    for (int j = 0; j < 16; j++) w[j] = (pack2<T>(v[2 * j], v[2 * j + 1]) & mask) ^ sign;
+                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, m);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, p.M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }
