@@ -264,7 +264,11 @@ static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
 template <class T>
 static void join(const float *acc, int parts, int64_t M, int64_t N, int64_t ld, const int *shift, void *out,
                  cudaStream_t s) {
-    k_join<T><<<blocks(M * (ld / 4), 256), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out), N);
+    if (parts > 8)
+        k_join<T, true><<<blocks(M * (ld / 4), 32), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out), N);
+    else
+        k_join<T, false><<<blocks(M * (ld / 4), 256), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out),
+                                                                   N);
     launched("join parts");
 }
 // D = A B^T (+ A1 B1^T), or with outputs = 2 also A1 B^T, as dense 16-bit rows

@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             tc::mbar_init(wfull + 8 * i, 1);
             tc::mbar_init(wempty + 8 * i, 1);
             tc::mbar_init(sfull + 8 * i, 1);
-            tc::mbar_init(sempty + 8 * i, kNarrowWarps);
-            tc::mbar_init(zfull + 8 * i, kNarrowWarps);
+            tc::mbar_init(sempty + 8 * i, kNarrowWarps / 2);
+            tc::mbar_init(zfull + 8 * i, kNarrowWarps / 2);
             tc::mbar_init(dwfull + 8 * i, 1);
             tc::mbar_init(dwempty + 8 * i, kNarrowWarps);
         }
@@ -219,7 +219,10 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue
-        const int quad = warp & 3, quarter = (warp - 2) >> 2;  // rows of the accumulators; a quarter of their columns
+        // Warps 2-9 take the even tiles, 10-17 the odd ones, each of them 64 columns: a warp that took a part of
+        // every tile would go through all of a tile's hand-offs within one tile's time (1024 x 131072 x 16: 118 us
+        // whether or not the exponentials were computed).
+        const int quad = warp & 3, quarter = (warp - 2) >> 2, set = quarter >> 1;
         const unsigned lanes = (unsigned)(32 * quad) << 16;
         const int r = 32 * quad + lane;  // row of a tile
         auto wait_all = [&](unsigned a, unsigned parity) {
@@ -247,11 +250,16 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         float4 *a = reinterpret_cast<float4 *>(p.acc_w + row * p.depth + c0);
 #pragma unroll
                         for (int k = 0; k < 4; k++) {
-                            if (g) {
-                                const float4 o = a[k];
+                            if (g == 0) {
+                                a[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+                            } else if (g + 1 < groups) {  // this lane alone adds here: the order is the groups'
+                                asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(a + k),
+                                             "f"(v[4 * k]), "f"(v[4 * k + 1]), "f"(v[4 * k + 2]), "f"(v[4 * k + 3])
+                                             : "memory");
+                            } else {
+                                const float4 o = __ldcg(a + k);
                                 v[4 * k] += o.x, v[4 * k + 1] += o.y, v[4 * k + 2] += o.z, v[4 * k + 3] += o.w;
                             }
-                            if (g + 1 < groups) a[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
                         }
                     }
                     if (g + 1 == groups) {
@@ -269,42 +277,63 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             if (lane == 0) tc::mbar_arrive(dwempty + 8 * (nb & 1));
             return true;
         };
-        unsigned n = 0, nb = 0;
+        unsigned n = 0, nb = 0;  // tiles and blocks so far; written: blocks whose dW this warp has written
         bool ok = true;
         for (int g = 0; ok && g < groups; g++) {
             const int tiles = min(p.group, token_tiles - g * p.group);
             const int64_t first = (int64_t)g * p.group * 128 + r;
-            LossRow next = fetch(first);
-            for (int b = 0; ok && b < mine; b++) {
-                const int64_t block = blockIdx.x + (int64_t)b * gridDim.x;
-                for (int t = 0; t < tiles; t++, n++) {
-                    const LossRow row = next;
-                    next = fetch(first + (t + 1 < tiles ? t + 1 : 0) * 128);
-                    // S was issued after the products that read this Z buffer last: it is free too
-                    if (!(ok = wait_all(sfull + 8 * (n & 1), (n >> 1) & 1))) break;
-                    tc::fence_after();
+            const unsigned nb0 = nb;  // the group's first block
+            unsigned written = nb;
+            auto write_until = [&](unsigned end) -> bool {
+                for (; written < end; written++)
+                    if (!write_dw(written, blockIdx.x + (int64_t)(written - nb0) * gridDim.x, g)) return false;
+                return true;
+            };
+            // this warp's tiles: every other one
+            auto tile_after = [&](int &b, int &t, int by) {
+                for (t += by; t >= tiles; t -= tiles) b++;
+            };
+            int b = 0, t = 0;
+            tile_after(b, t, (n & 1) != (unsigned)set);
+            LossRow next = fetch(first + t * 128);
+            const unsigned end = n + tiles * mine;
+            for (n += (n & 1) != (unsigned)set; n < end; n += 2) {
+                const LossRow row = next;
+                const int64_t m = first + t * 128;
+                const int col = (blockIdx.x + b * gridDim.x) * 128 + (quarter & 1) * 64;
+                const unsigned before = nb0 + b;
+                tile_after(b, t, 2);
+                next = fetch(first + t * 128);
+                // S was issued after the products that read this Z buffer last: it is free too
+                if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1))) break;
+                tc::fence_after();
+                unsigned char *z = zbuf + set * 2 * kPanel + (quarter & 1) * kPanel + r * 128;
+#pragma unroll 1
+                for (int c = 0; c < 2; c++) {
                     float v[32];
                     unsigned w[16];
-                    ptx::load32(tS + (n & 1) * 128 + lanes + quarter * 32, v);
+                    ptx::load32(tS + set * 128 + lanes + (quarter & 1) * 64 + c * 32, v);
                     ptx::wait32(v);
-                    tc::fence_before();
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(sempty + 8 * (n & 1));
-                    loss_z<T>(v, w, row, (int)(block * 128) + quarter * 32, p.lse, first + t * 128);
-                    unsigned char *z = zbuf + (n & 1) * 2 * kPanel + (quarter >> 1) * kPanel + r * 128;
+                    if (c) {
+                        tc::fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
+                    }
+                    loss_z<T>(v, w, row, col + c * 32, p.lse, m);
 #pragma unroll
                     for (int j = 0; j < 4; j++)
-                        *reinterpret_cast<uint4 *>(z + ((((quarter & 1) * 4 + j) ^ (r & 7)) << 4)) =
+                        *reinterpret_cast<uint4 *>(z + (((c * 4 + j) ^ (r & 7)) << 4)) =
                             make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(zfull + 8 * (n & 1));
-                    // the block before this one, while this one's products run
-                    if (t == 0 && b > 0 && !(ok = write_dw(nb - 1, block - gridDim.x, g))) break;
                 }
-                nb++;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(zfull + 8 * set);
+                // the blocks before this one, while this one's products run
+                if (!(ok = write_until(before))) break;
             }
-            if (ok) ok = write_dw(nb - 1, blockIdx.x + (int64_t)(mine - 1) * gridDim.x, g);
+            n = end;
+            nb = nb0 + mine;
+            if (ok) ok = write_until(nb);
             if (!ok || !(ok = wait_all(dhfull, (unsigned)g & 1))) break;
             tc::fence_after();
             const int c0 = quarter * 16;
