@@ -32,7 +32,7 @@ constexpr int kNarrowGroup = 8;       // token tiles of a group at most
 constexpr int kNarrowWarps = 16;      // epilogue warps
 constexpr int kNarrowThreads = 64 + 32 * kNarrowWarps;
 constexpr int kPanel = 128 * 128;     // bytes of 128 rows of 64 elements
-constexpr int kNarrowBars = 2 + 2 * 7 + 2;
+constexpr int kNarrowBars = 2 + 2 * 8 + 2;
 constexpr int kNarrowSmem = (kNarrowGroup + 2 + 4) * kPanel + 8 * kNarrowBars + 16;
 
 struct NarrowArgs {
@@ -91,8 +91,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + (kNarrowGroup + 6) * kPanel);
     const unsigned bar = tc::smem_u32(bars);
     const unsigned hfull = bar, dhfull = bar + 8, wfull = bar + 16, wempty = bar + 32, sfull = bar + 48,
-                   sempty = bar + 64, zfull = bar + 80, dwfull = bar + 96, dwempty = bar + 112, dhempty = bar + 128,
-                   drain = bar + 136;
+                   sempty = bar + 64, zfull = bar + 80, zempty = bar + 96, dwfull = bar + 112, dwempty = bar + 128,
+                   dhempty = bar + 144, drain = bar + 152;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(bars + kNarrowBars);
     int *s_error = reinterpret_cast<int *>(s_tmem + 1);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 2);
@@ -107,6 +107,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             tc::mbar_init(sfull + 8 * i, 1);
             tc::mbar_init(sempty + 8 * i, kNarrowWarps / 2);
             tc::mbar_init(zfull + 8 * i, kNarrowWarps / 2);
+            tc::mbar_init(zempty + 8 * i, 1);
             tc::mbar_init(dwfull + 8 * i, 1);
             tc::mbar_init(dwempty + 8 * i, kNarrowWarps);
         }
@@ -184,10 +185,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                     if (++ts == tiles) ts = 0, ws++;
                     return true;
                 };
-                ok = ok && issue_s();
+                // S runs ahead of the gradients' products by two tiles, so that an epilogue warp finds its next one
+                // without waiting for them; by one where a block has one tile only, since its rows of W are in one
+                // of two buffers that the products before have to release
+                const int ahead = tiles > 1 ? 2 : 1;
+                for (int j = 0; ok && j < ahead && j < all; j++) ok = issue_s();
                 int t = 0, b = 0;
                 for (int j = 0; ok && j < all; j++, n++) {
-                    if (j + 1 < all && !(ok = issue_s())) break;
+                    if (j + ahead < all && !(ok = issue_s())) break;
                     if (t == 0 && !(ok = tc::mbar_wait(dwempty + 8 * (nb & 1), ((nb >> 1) & 1) ^ 1, s_abort, s_error, 2,
                                                        kWaitNs)))
                         break;
@@ -203,6 +208,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
 #pragma unroll
                     for (int k = 0; k < 8; k++)
                         ptx::mma_own(dh, zk + (k >> 2) * (kPanel >> 4) + 2 * (k & 3), wb + 128 * k, idh, b > 0 || k > 0);
+                    ptx::commit(zempty + 8 * (n & 1));
                     if (++t == tiles) {
                         t = 0;
                         ptx::commit(wempty + 8 * (nb & 1));
@@ -304,8 +310,8 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 const unsigned before = nb0 + b;
                 tile_after(b, t, 2);
                 next = fetch(first + t * 128);
-                // S was issued after the products that read this Z buffer last: it is free too
-                if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1))) break;
+                if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1) && wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1)))
+                    break;
                 tc::fence_after();
                 unsigned char *z = zbuf + set * 2 * kPanel + (quarter & 1) * kPanel + r * 128;
 #pragma unroll 1
