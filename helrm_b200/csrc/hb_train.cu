@@ -489,7 +489,7 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         Product d;
         d.a = in.fit({h, tokens, inner, ldh});
         d.b = in.fit({wt, vocab, inner, ldw});
-        const int64_t parts = epi_warps(EPI_LSE) / 4 * (int64_t)blocks(vocab, kCols);
+        const int64_t parts = 2 * (int64_t)blocks(vocab, kCols);
         const int64_t joined = parts > kLossParts ? blocks(parts, kLossParts) : 0;
         float2 *part = w.take<float2>(parts * tokens), *few = w.take<float2>(joined * tokens);
         float *at = w.take<float>(tokens);

@@ -228,7 +228,7 @@ template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI), 1)
     k_mma_product(const __grid_constant__ ProductArgs p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-    constexpr int kWarps = epi_warps(EPI);
+    constexpr int kWarps = epi_warps(EPI), kSets = kWarps / 8;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *stage = smem + 2 * kStages * kOperand;
     uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kStageOut);
@@ -248,7 +248,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         }
         for (int i = 0; i < 2; i++) {
             tc::mbar_init(tfull + 8 * i, 1);
-            tc::mbar_init(tempty + 8 * i, 2 * kWarps);
+            tc::mbar_init(tempty + 8 * i, 16);  // 8 warps of both SMs
         }
         tc::mbar_init(drain, 1);
         *s_error = 0;
@@ -391,27 +391,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         __syncwarp();
     } else if (warp >= 4) {
         // ------------------------------------------------------------ epilogue
-        const int quad = warp & 3, half = (warp - 4) >> 2;  // half: or quarter, with 16 warps
+        // 8 warps take a tile, half of its columns each; 16 are two sets that take alternate tiles (with a quarter of
+        // every tile each, what a tile costs beside its logits counted twice)
+        const int quad = warp & 3, half = (warp - 4) >> 2 & 1, set = kSets > 1 ? (warp - 4) >> 3 : 0;
         unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
         const EpiArgs &e = p.e;
-        unsigned cnt = 0;
+        unsigned cnt = set;
         // What the loss needs to know of this lane's row, fetched a tile ahead.
         int64_t next_target = -1;
         LossRow next_row = {0.0f, 0.0f, 0.0f, kNoTarget};
-        Item next = item(first_item);
+        Item next = item(first_item + set * step);
         auto fetch = [&] {
             const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
             if (EPI == EPI_LSE) next_target = m < p.M ? e.target[m] : -1;
             if (EPI == EPI_Z && m < p.M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
-        if (first_item < items) fetch();
-        for (unsigned i = first_item; i < items; i += step, cnt++) {
+        if (first_item + set * step < items) fetch();
+        for (unsigned i = first_item + set * step; i < items; i += kSets * step, cnt += kSets) {
             const Item t = next;
             const int64_t target = next_target;
             const LossRow row = next_row;
-            if (i + step < items) {
-                next = item(i + step);
+            if (i + kSets * step < items) {
+                next = item(i + kSets * step);
                 fetch();
             }
             const int buf = (int)(cnt & 1);
@@ -485,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     }
                 }
             } else if constexpr (EPI == EPI_LSE) {
-                constexpr int kWide = kCols / (kWarps / 4);  // columns a warp
+                constexpr int kWide = kCols / 2;  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 const int64_t tg = target - n0;
                 float top = -INFINITY, sum = 0.0f;
@@ -527,9 +529,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + ((s0 + s1) + (s2 + s3));
                     top = mx;
                 }
-                if (m < p.M) e.part[((int64_t)t.nt * (kWarps / 4) + half) * p.M + m] = make_float2(top, sum);
+                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top, sum);
             } else if constexpr (EPI == EPI_Z) {
-                constexpr int kWide = kCols / (kWarps / 4);
+                constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
