@@ -108,12 +108,28 @@ def _stream(index: int) -> int:
 
 class _Plan:
     """The checked form of a call: the entry's leading arguments, the row
-    pitches of its matrices, the result's shape, and the workspace it needs
-    by which addresses are on 16-byte boundaries."""
-    __slots__ = ("head", "pitches", "shape", "needs")
+    pitches of its matrices, what it returns, and the workspace it needs by
+    which addresses are on 16-byte boundaries."""
+    __slots__ = ("head", "pitches", "out", "needs")
 
-    def __init__(self, head, pitches, shape):
-        self.head, self.pitches, self.shape, self.needs = head, pitches, shape, {}
+    def __init__(self, head, pitches, out):
+        self.head, self.pitches, self.out, self.needs = head, pitches, out, {}
+
+
+class _Out:
+    """A dense result (with its strides at hand torch allocates it fastest)."""
+    __slots__ = ("shape", "strides", "dtype", "device")
+
+    def __init__(self, shape, dtype, device):
+        self.shape, self.dtype, self.device = tuple(shape), dtype, device
+        n, strides = 1, []
+        for d in reversed(self.shape):
+            strides.insert(0, n)
+            n *= max(1, d)
+        self.strides = tuple(strides)
+
+    def new(self):
+        return torch.empty_strided(self.shape, self.strides, dtype=self.dtype, device=self.device)
 
 
 def _remember(key, plan):
@@ -133,7 +149,7 @@ def _run(name: str, like, needs, odd, *args):
         _capi.check(fn(*args, None, ctypes.byref(n), 0))
         need = needs[odd] = n.value
     if need:
-        ws = like.new_empty(need, dtype=torch.uint8)
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=like.device)
         rc = fn(*args, ws.data_ptr(), ctypes.byref(ctypes.c_size_t(need)), _stream(args[0]))
     else:  # any aligned address will do
         rc = fn(*args, 256, _NOTHING, _stream(args[0]))
@@ -163,11 +179,11 @@ def gated_forward(x, w_gate, w_up, activation: str = "silu"):
         if width < 1:
             raise ValueError("the weights have no rows")
         plan = _Plan((x.device.index, _DTYPES[x.dtype], act, xm.shape[0], inner, width),
-                     (_pitch(xm), _pitch(wg), _pitch(wu)), x.shape[:-1] + (width,))
+                     (_pitch(xm), _pitch(wg), _pitch(wu)), _Out(x.shape[:-1] + (width,), x.dtype, x.device))
         if xm.data_ptr() == x.data_ptr() and wg is w_gate and wu is w_up:
             _remember(key, plan)
         x, w_gate, w_up = xm, wg, wu  # the copies, where the strides asked for some
-    h = x.new_empty(plan.shape)
+    h = plan.out.new()
     px, pg, pu = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
     lx, lg, lu = plan.pitches
     _run("helrm_GatedForward", x, plan.needs, (px & 15, pg & 15, pu & 15), *plan.head, px, lx, pg, lg, pu, lu,
@@ -208,14 +224,16 @@ def gated_backward(dh, x, w_gate, w_up, activation: str = "silu", needs=(True, T
         if tuple(dh.shape) != shape[:-1] + (wg.shape[0],):
             raise ValueError(f"dh has shape {tuple(dh.shape)}, the block's result {shape[:-1] + (wg.shape[0],)}")
         plan = _Plan((dh.device.index, _DTYPES[dh.dtype], act, tokens, inner, width),
-                     (_pitch(dhm), pitch, _pitch(wg), _pitch(wu)), (shape, (width, inner)))
+                     (_pitch(dhm), pitch, _pitch(wg), _pitch(wu)),
+                     (_Out(shape, dh.dtype, dh.device), _Out((width, inner), dh.dtype, dh.device)))
         if (dhm.data_ptr() == dh.data_ptr() and (kept or xm.data_ptr() == x.data_ptr()) and wg is w_gate
                 and wu is w_up):
             _remember(key, plan)
         dh, x, w_gate, w_up = dhm, xm, wg, wu  # the copies, where the strides asked for some
-    dx = dh.new_empty(plan.shape[0]) if needs[0] else None
-    dwg = dh.new_empty(plan.shape[1]) if needs[1] else None
-    dwu = dh.new_empty(plan.shape[1]) if needs[2] else None
+    out_x, out_w = plan.out
+    dx = out_x.new() if needs[0] else None
+    dwg = out_w.new() if needs[1] else None
+    dwu = out_w.new() if needs[2] else None
     if any(needs):
         ld, lx, lg, lu = plan.pitches
         pd, pg, pu = dh.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
@@ -285,12 +303,13 @@ def pack_checkpoint(x) -> Checkpoint:
         rows, cols = m.shape
         groups = -(-cols // GROUP)
         plan = _Plan((x.device.index, _DTYPES[x.dtype], rows, cols), _pitch(m),
-                     ((rows, GROUP * groups), (rows, groups), tuple(x.shape), x.dtype))
+                     (_Out((rows, GROUP * groups), torch.int8, x.device), _Out((rows, groups), torch.uint8, x.device),
+                      tuple(x.shape), x.dtype))
         if m.data_ptr() == x.data_ptr():
             _remember(key, plan)
         x = m
-    shape_q, shape_e, shape, dtype = plan.shape
-    q, e = x.new_empty(shape_q, dtype=torch.int8), x.new_empty(shape_e, dtype=torch.uint8)
+    out_q, out_e, shape, dtype = plan.out
+    q, e = out_q.new(), out_e.new()
     rc = _entry("helrm_PackCheckpoint")(*plan.head, x.data_ptr(), plan.pitches, q.data_ptr(), e.data_ptr(),
                                         _stream(plan.head[0]))
     if rc:
@@ -310,9 +329,10 @@ def unpack_checkpoint(c: Checkpoint):
     except (AttributeError, TypeError):
         key = plan = None
     if plan is None:
-        plan = _Plan((q.device.index, _DTYPES.get(dtype), _check_checkpoint(c), shape[-1]), None, shape)
+        plan = _Plan((q.device.index, _DTYPES.get(dtype), _check_checkpoint(c), shape[-1]), None,
+                     _Out(shape, dtype, q.device))
         _remember(key, plan)
-    x = q.new_empty(shape, dtype=dtype)
+    x = plan.out.new()
     rc = _entry("helrm_UnpackCheckpoint")(*plan.head, q.data_ptr(), e.data_ptr(), x.data_ptr(),
                                           _stream(plan.head[0]))
     if rc:
@@ -331,10 +351,11 @@ def _targets(targets, lead, dev):
     return targets.to(torch.int64).contiguous()
 
 
-def _floats(t, name: str, lead, dev):
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != dev or t.shape != lead:
-        raise ValueError(f"{name} is not a float32 tensor of shape {tuple(lead)} on {dev}")
-    return t.contiguous()
+def _floats(t, name: str, like: _Out):
+    if (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != like.device
+            or t.shape != like.shape):
+        raise ValueError(f"{name} is not a float32 tensor of shape {like.shape} on {like.device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _loss_call(h, w, targets):
@@ -354,7 +375,9 @@ def _loss_call(h, w, targets):
         lead = h.shape[:-1]
         t = _targets(targets, lead, h.device)
         plan = _Plan((h.device.index, _DTYPES[h.dtype], hm.shape[0], hm.shape[1], wm.shape[0]),
-                     (_pitch(hm), _pitch(wm)), (lead, h.shape, wm.shape, h.device))
+                     (_pitch(hm), _pitch(wm)),
+                     (_Out(lead, torch.float32, h.device), _Out(lead + (2,), torch.float32, h.device),
+                      _Out(h.shape, h.dtype, h.device), _Out(wm.shape, h.dtype, h.device)))
         if hm.data_ptr() == h.data_ptr() and wm is w:
             _remember(key, plan)
         return hm, wm, t, plan
@@ -370,8 +393,7 @@ def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
     w [vocab, inner], targets [...].  Rows whose target is ignore_index have
     loss 0, other targets outside the vocabulary NaN."""
     h, w, t, plan = _loss_call(h, w, targets)
-    lead = plan.shape[0]
-    loss, lse = h.new_empty(lead, dtype=torch.float32), h.new_empty(lead + (2,), dtype=torch.float32)
+    loss, lse = plan.out[0].new(), plan.out[1].new()
     ph, pw = h.data_ptr(), w.data_ptr()
     _run("helrm_VocabularyLossForward", h, plan.needs, (ph & 15, pw & 15), *plan.head, ph, plan.pitches[0], pw,
          plan.pitches[1], t.data_ptr(), int(ignore_index), loss.data_ptr(), lse.data_ptr())
@@ -382,10 +404,10 @@ def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100
     """(dh, dw) from dloss [...] (float32) and vocabulary_loss_forward's lse.
     needs: which of the two are wanted (None in their place)."""
     h, w, t, plan = _loss_call(h, w, targets)
-    lead, shape, shape_w, dev = plan.shape
-    g, l = _floats(dloss, "dloss", lead, dev), _floats(lse, "lse", lead + (2,), dev)
-    dh = h.new_empty(shape) if needs[0] else None
-    dw = h.new_empty(shape_w) if needs[1] else None
+    out_loss, out_lse, out_h, out_w = plan.out
+    g, l = _floats(dloss, "dloss", out_loss), _floats(lse, "lse", out_lse)
+    dh = out_h.new() if needs[0] else None
+    dw = out_w.new() if needs[1] else None
     if any(needs):
         ph, pw = h.data_ptr(), w.data_ptr()
         _run("helrm_VocabularyLossBackward", h, plan.needs, (ph & 15, pw & 15, bool(needs[0]), bool(needs[1])),
