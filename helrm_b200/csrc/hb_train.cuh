@@ -297,29 +297,33 @@ __global__ void __launch_bounds__(kCkptThreads) k_pack(const T *__restrict__ x, 
 #pragma unroll
     for (int i = 0; i < kCkptRows; i++) {
         const unsigned w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-        float f[8];
-        unsigned top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float2 t = unpack2<T>(w[k]);
-            f[2 * k] = t.x, f[2 * k + 1] = t.y;
-            top = max(top, max(__float_as_uint(t.x) & 0x7fffffffu, __float_as_uint(t.y) & 0x7fffffffu));
-        }
+        // magnitudes of both 16-bit types are ordered like their bits
+        unsigned mx = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                               __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
         // a group lies in four neighbouring lanes: per_block and the block's first chunk are multiples of 4
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const unsigned top = __float_as_uint(unpack2<T>(max(mx & 0xffffu, mx >> 16)).x);
         // top = f 2^E with 1 <= f < 2; max <= 127 s = (127/64) 2^(e+6)
         int E = (int)(top >> 23) - ((top & 0x7fffffu) > 0x7e0000u ? 5 : 6);  // biased by 127
         E = max(E, least);
         const float inv = __uint_as_float((unsigned)(254 - E) << 23);
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const float2 t = unpack2<T>(w[k]);
+            f[2 * k] = t.x * inv, f[2 * k + 1] = t.y * inv;
+        }
+        if (__any_sync(0xffffffffu, E == most)) {
+            asm volatile("");
+#pragma unroll
+            for (int k = 0; k < 8; k++)  // 64 s would be past the type's range
+                if (E == most) f[k] = fminf(fmaxf(f[k], -63.0f), 63.0f);
+        }
         // x / s is exact; adding 1.5 2^23 leaves it rounded, halves to even, in the low byte
         unsigned b[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            float y = f[k] * inv;
-            if (E == most) y = fminf(fmaxf(y, -63.0f), 63.0f);  // 64 s would be past the type's range
-            b[k] = __float_as_uint(y + 12582912.0f);
-        }
+        for (int k = 0; k < 8; k++) b[k] = __float_as_uint(f[k] + 12582912.0f);
         uint2 o;
         o.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
         o.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
