@@ -30,9 +30,9 @@ namespace train {
 constexpr int kNarrow = 64;           // features at most
 constexpr int kNarrowGroup = 8;       // token tiles of a group at most
 constexpr int kNarrowWarps = 16;      // epilogue warps
-constexpr int kNarrowThreads = 64 + 32 * kNarrowWarps;
+constexpr int kNarrowThreads = 96 + 32 * kNarrowWarps;
 constexpr int kPanel = 128 * 128;     // bytes of 128 rows of 64 elements
-constexpr int kNarrowBars = 2 + 2 * 8 + 2;
+constexpr int kNarrowBars = 2 + 2 * 8 + 4;
 constexpr int kNarrowSmem = (kNarrowGroup + 2 + 4) * kPanel + 8 * kNarrowBars + 16;
 
 struct NarrowArgs {
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
     const unsigned bar = tc::smem_u32(bars);
     const unsigned hfull = bar, dhfull = bar + 8, wfull = bar + 16, wempty = bar + 32, sfull = bar + 48,
                    sempty = bar + 64, zfull = bar + 80, zempty = bar + 96, dwfull = bar + 112, dwempty = bar + 128,
-                   dhempty = bar + 144, drain = bar + 152;
+                   dhempty = bar + 144, drain = bar + 152, drain2 = bar + 160;
     unsigned *s_tmem = reinterpret_cast<unsigned *>(bars + kNarrowBars);
     int *s_error = reinterpret_cast<int *>(s_tmem + 1);
     volatile int *s_abort = reinterpret_cast<volatile int *>(s_tmem + 2);
@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         }
         tc::mbar_init(dhempty, kNarrowWarps);
         tc::mbar_init(drain, 1);
+        tc::mbar_init(drain2, 1);
         *s_error = 0;
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -156,45 +157,24 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         }
         __syncwarp();
     } else if (warp == 1) {
-        // ------------------------------------------------------------ MMA
+        // ------------------------------------------------------------ MMA of the gradients
         if (lane == 0) {
             constexpr unsigned kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr unsigned kBase = (1u << 4) | kType | ((128u >> 4) << 24);
-            const unsigned ids = kBase | ((128u >> 3) << 17);                                        // S
             const unsigned idw = kBase | (1u << 15) | (1u << 16) | ((unsigned)(p.depth >> 3) << 17);  // dW
             const unsigned idh = kBase | (1u << 16) | ((unsigned)(p.depth >> 3) << 17);               // dH
-            const int steps = p.depth / 16;
-            unsigned ns = 0, n = 0, nb = 0, ws = 0;  // S issued, tiles done, blocks done, W blocks taken by S
+            unsigned n = 0, nb = 0;  // tiles and blocks done
             bool ok = true;
             for (int g = 0; ok && g < groups; g++) {
                 const int tiles = min(p.group, token_tiles - g * p.group), all = tiles * mine;
                 ok = tc::mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2, kWaitNs) &&
                      (g == 0 || tc::mbar_wait(dhempty, (unsigned)(g - 1) & 1, s_abort, s_error, 2, kWaitNs));
-                int ts = 0;  // token tile of the next S
-                auto issue_s = [&]() -> bool {
-                    if (ts == 0 && !tc::mbar_wait(wfull + 8 * (ws & 1), (ws >> 1) & 1, s_abort, s_error, 2, kWaitNs))
-                        return false;
-                    if (!tc::mbar_wait(sempty + 8 * (ns & 1), ((ns >> 1) & 1) ^ 1, s_abort, s_error, 2, kWaitNs))
-                        return false;
-                    tc::fence_after();
-                    const uint64_t a = ptx::descriptor(sH + ts * kPanel), b = ptx::descriptor(sW + (ws & 1) * kPanel);
-                    for (int k = 0; k < steps; k++)
-                        ptx::mma_own(tS + (ns & 1) * 128, a + 2 * k, b + 2 * k, ids, k > 0);
-                    ptx::commit(sfull + 8 * (ns & 1));
-                    ns++;
-                    if (++ts == tiles) ts = 0, ws++;
-                    return true;
-                };
-                // S runs ahead of the gradients' products by two tiles, so that an epilogue warp finds its next one
-                // without waiting for them; by one where a block has one tile only, since its rows of W are in one
-                // of two buffers that the products before have to release
-                const int ahead = tiles > 1 ? 2 : 1;
-                for (int j = 0; ok && j < ahead && j < all; j++) ok = issue_s();
                 int t = 0, b = 0;
                 for (int j = 0; ok && j < all; j++, n++) {
-                    if (j + ahead < all && !(ok = issue_s())) break;
-                    if (t == 0 && !(ok = tc::mbar_wait(dwempty + 8 * (nb & 1), ((nb >> 1) & 1) ^ 1, s_abort, s_error, 2,
-                                                       kWaitNs)))
+                    if (t == 0 &&
+                        !(ok = tc::mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2, kWaitNs) &&
+                               tc::mbar_wait(dwempty + 8 * (nb & 1), ((nb >> 1) & 1) ^ 1, s_abort, s_error, 2,
+                                             kWaitNs)))
                         break;
                     if (!(ok = tc::mbar_wait(zfull + 8 * (n & 1), (n >> 1) & 1, s_abort, s_error, 2, kWaitNs))) break;
                     tc::fence_after();
@@ -223,12 +203,44 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             tc::mbar_wait(drain, 0, nullptr, s_error, 8, kWaitNs);
         }
         __syncwarp();
+    } else if (warp == 2) {
+        // ------------------------------------------------------------ MMA of S
+        // A thread of its own: S of a tile to come never waits behind the hand-off of a finished Z (one thread for
+        // all three products: 83 us at 1024 x 131072 x 16).
+        if (lane == 0) {
+            constexpr unsigned kType = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            const unsigned ids = (1u << 4) | kType | ((128u >> 4) << 24) | ((128u >> 3) << 17);
+            const int steps = p.depth / 16;
+            unsigned n = 0, nb = 0;
+            bool ok = true;
+            for (int g = 0; ok && g < groups; g++) {
+                const int tiles = min(p.group, token_tiles - g * p.group);
+                ok = tc::mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2, kWaitNs);
+                for (int b = 0; ok && b < mine; b++, nb++) {
+                    if (!(ok = tc::mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2, kWaitNs))) break;
+                    const uint64_t wd = ptx::descriptor(sW + (nb & 1) * kPanel);
+                    for (int t = 0; t < tiles; t++, n++) {
+                        if (!(ok = tc::mbar_wait(sempty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, s_abort, s_error, 2,
+                                                 kWaitNs)))
+                            break;
+                        tc::fence_after();
+                        const uint64_t hd = ptx::descriptor(sH + t * kPanel);
+                        for (int k = 0; k < steps; k++)
+                            ptx::mma_own(tS + (n & 1) * 128, hd + 2 * k, wd + 2 * k, ids, k > 0);
+                        ptx::commit(sfull + 8 * (n & 1));
+                    }
+                }
+            }
+            ptx::commit(drain2);
+            tc::mbar_wait(drain2, 0, nullptr, s_error, 8, kWaitNs);
+        }
+        __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue
-        // Warps 2-9 take the even tiles, 10-17 the odd ones, each of them 64 columns: a warp that took a part of
+        // Warps 3-10 take the even tiles, 11-18 the odd ones, each of them 64 columns: a warp that took a part of
         // every tile would go through all of a tile's hand-offs within one tile's time (1024 x 131072 x 16: 118 us
         // whether or not the exponentials were computed).
-        const int quad = warp & 3, quarter = (warp - 2) >> 2, set = quarter >> 1;
+        const int quad = warp & 3, quarter = (warp - 3) >> 2, set = quarter >> 1;
         const unsigned lanes = (unsigned)(32 * quad) << 16;
         const int r = 32 * quad + lane;  // row of a tile
         auto wait_all = [&](unsigned a, unsigned parity) {
