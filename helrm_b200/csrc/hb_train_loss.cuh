@@ -142,13 +142,13 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             for (int g = 0; ok && g < groups; g++) {
                 const int tiles = min(p.group, token_tiles - g * p.group);
                 // the group before has read its H
-                if (g && !(ok = tc::mbar_wait(dhfull, (unsigned)(g - 1) & 1, s_abort, s_error, 1, kWaitNs))) break;
+                if (g && !(ok = mbar_wait(dhfull, (unsigned)(g - 1) & 1, s_abort, s_error, 1))) break;
                 tc::mbar_arrive_tx(hfull, tiles * kPanel);
                 for (int t = 0; t < tiles; t++)
                     ptx::tma_load_own(sH + t * kPanel, &p.h, 0, (g * p.group + t) * 128, hfull);
                 for (int b = 0; b < mine; b++, nw++) {
                     const unsigned s = nw & 1;
-                    if (!(ok = tc::mbar_wait(wempty + 8 * s, ((nw >> 1) & 1) ^ 1, s_abort, s_error, 1, kWaitNs))) break;
+                    if (!(ok = mbar_wait(wempty + 8 * s, ((nw >> 1) & 1) ^ 1, s_abort, s_error, 1))) break;
                     tc::mbar_arrive_tx(wfull + 8 * s, kPanel);
                     ptx::tma_load_own(sW + s * kPanel, &p.w, 0, ((int)blockIdx.x + b * (int)gridDim.x) * 128,
                                       wfull + 8 * s);
@@ -167,16 +167,15 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             bool ok = true;
             for (int g = 0; ok && g < groups; g++) {
                 const int tiles = min(p.group, token_tiles - g * p.group), all = tiles * mine;
-                ok = tc::mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2, kWaitNs) &&
-                     (g == 0 || tc::mbar_wait(dhempty, (unsigned)(g - 1) & 1, s_abort, s_error, 2, kWaitNs));
+                ok = mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2) &&
+                     (g == 0 || mbar_wait(dhempty, (unsigned)(g - 1) & 1, s_abort, s_error, 2));
                 int t = 0, b = 0;
                 for (int j = 0; ok && j < all; j++, n++) {
                     if (t == 0 &&
-                        !(ok = tc::mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2, kWaitNs) &&
-                               tc::mbar_wait(dwempty + 8 * (nb & 1), ((nb >> 1) & 1) ^ 1, s_abort, s_error, 2,
-                                             kWaitNs)))
+                        !(ok = mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2) &&
+                               mbar_wait(dwempty + 8 * (nb & 1), ((nb >> 1) & 1) ^ 1, s_abort, s_error, 2)))
                         break;
-                    if (!(ok = tc::mbar_wait(zfull + 8 * (n & 1), (n >> 1) & 1, s_abort, s_error, 2, kWaitNs))) break;
+                    if (!(ok = mbar_wait(zfull + 8 * (n & 1), (n >> 1) & 1, s_abort, s_error, 2))) break;
                     tc::fence_after();
                     const unsigned z = sZ + (n & 1) * 2 * kPanel;
                     // Z MN-major: the vocabulary's two 64-entry panels are kPanel bytes apart
@@ -200,7 +199,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 if (ok) ptx::commit(dhfull);
             }
             ptx::commit(drain);
-            tc::mbar_wait(drain, 0, nullptr, s_error, 8, kWaitNs);
+            mbar_wait(drain, 0, nullptr, s_error, 8);
         }
         __syncwarp();
     } else if (warp == 2) {
@@ -215,13 +214,12 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
             bool ok = true;
             for (int g = 0; ok && g < groups; g++) {
                 const int tiles = min(p.group, token_tiles - g * p.group);
-                ok = tc::mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2, kWaitNs);
+                ok = mbar_wait(hfull, (unsigned)g & 1, s_abort, s_error, 2);
                 for (int b = 0; ok && b < mine; b++, nb++) {
-                    if (!(ok = tc::mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2, kWaitNs))) break;
+                    if (!(ok = mbar_wait(wfull + 8 * (nb & 1), (nb >> 1) & 1, s_abort, s_error, 2))) break;
                     const uint64_t wd = ptx::descriptor(sW + (nb & 1) * kPanel);
                     for (int t = 0; t < tiles; t++, n++) {
-                        if (!(ok = tc::mbar_wait(sempty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, s_abort, s_error, 2,
-                                                 kWaitNs)))
+                        if (!(ok = mbar_wait(sempty + 8 * (n & 1), ((n >> 1) & 1) ^ 1, s_abort, s_error, 2)))
                             break;
                         tc::fence_after();
                         const uint64_t hd = ptx::descriptor(sH + t * kPanel);
@@ -232,7 +230,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 }
             }
             ptx::commit(drain2);
-            tc::mbar_wait(drain2, 0, nullptr, s_error, 8, kWaitNs);
+            mbar_wait(drain2, 0, nullptr, s_error, 8);
         }
         __syncwarp();
     } else {
@@ -244,7 +242,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         const unsigned lanes = (unsigned)(32 * quad) << 16;
         const int r = 32 * quad + lane;  // row of a tile
         auto wait_all = [&](unsigned a, unsigned parity) {
-            return __all_sync(0xffffffffu, tc::mbar_wait(a, parity, s_abort, s_error, 4, kWaitNs));
+            return __all_sync(0xffffffffu, mbar_wait(a, parity, s_abort, s_error, 4));
         };
         const float unscale = p.shift ? ldexpf(1.0f, -*p.shift) : 1.0f;
         const bool vec = p.inner % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dw) & 15) == 0;
@@ -322,8 +320,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 const unsigned before = nb0 + b;
                 tile_after(b, t, 2);
                 next = fetch(first + t * 128);
-                if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1) && wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1)))
-                    break;
+                if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1))) break;
                 tc::fence_after();
                 unsigned char *z = zbuf + set * 2 * kPanel + (quarter & 1) * kPanel + r * 128;
 #pragma unroll 1
@@ -338,11 +335,14 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
                     }
                     loss_z<T>(v, w, row, col + c * 32, p.lse, m);
+                    // the products that read this buffer two tiles ago
+                    if (!c && !(ok = wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1))) break;
 #pragma unroll
                     for (int j = 0; j < 4; j++)
                         *reinterpret_cast<uint4 *>(z + (((c * 4 + j) ^ (r & 7)) << 4)) =
                             make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
                 }
+                if (!ok) break;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(zfull + 8 * set);

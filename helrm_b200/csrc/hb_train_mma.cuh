@@ -58,6 +58,26 @@ struct ProductArgs {
     int *error;            // host memory
 };
 
+// Bounded wait for a barrier's phase, as tc::mbar_wait, except that a wait of
+// ordinary length reads no clock.
+__device__ __forceinline__ bool mbar_wait(unsigned a, unsigned parity, volatile int *abort, int *err, int code) {
+    if (tc::mbar_try(a, parity)) return true;
+    unsigned long long t0 = 0;
+    for (unsigned it = 1;; it++) {
+        if (tc::mbar_try(a, parity)) return true;
+        if (abort && *abort) return false;
+        if ((it & 255) == 0) {
+            const unsigned long long t = tc::gtimer();
+            if (t0 == 0) t0 = t;
+            if (t - t0 > kWaitNs) {
+                if (abort) *abort = 1;
+                atomicOr(err, code);
+                return false;
+            }
+        }
+    }
+}
+
 namespace ptx {
 __device__ __forceinline__ unsigned rank() {
     unsigned r;
@@ -314,7 +334,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int m = t.mt * kRows + 128 * (int)rank;
                 const int n = kDual ? t.nt * 128 : t.nt * kCols + 128 * (int)rank;
                 for (int k = t.k0; k < t.k1; k++) {
-                    if (!tc::mbar_wait(empty + 8 * s, ph ^ 1, s_abort, s_error, 1, kWaitNs)) {
+                    if (!mbar_wait(empty + 8 * s, ph ^ 1, s_abort, s_error, 1)) {
                         ok = false;
                         break;
                     }
@@ -346,7 +366,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             for (int i = 0; ok && i < kStages && i < loads; i++) {
                 if (s == 0) ph ^= 1;
                 s = s == 0 ? kStages - 1 : s - 1;
-                ok = tc::mbar_wait(empty + 8 * s, ph, s_abort, s_error, 1, kWaitNs);
+                ok = mbar_wait(empty + 8 * s, ph, s_abort, s_error, 1);
             }
         }
         __syncwarp();
@@ -366,11 +386,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             for (unsigned i = first_item; ok && i < items; i += step, n++) {
                 const Item t = item(i);
                 const int buf = (int)(n & 1);
-                if (!tc::mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2, kWaitNs)) break;
+                if (!mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2)) break;
                 tc::fence_after();
                 const unsigned d = tmem + buf * kCols;
                 for (int k = t.k0; k < t.k1; k++) {
-                    if (!tc::mbar_wait(full + 8 * s, ph, s_abort, s_error, 2, kWaitNs)) {
+                    if (!mbar_wait(full + 8 * s, ph, s_abort, s_error, 2)) {
                         ok = false;
                         break;
                     }
@@ -386,7 +406,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             }
             // after a failure too, no MMA is left in flight
             ptx::commit_own(drain);
-            tc::mbar_wait(drain, 0, nullptr, s_error, 8, kWaitNs);
+            mbar_wait(drain, 0, nullptr, s_error, 8);
         }
         __syncwarp();
     } else if (warp >= 4) {
@@ -424,8 +444,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 __syncwarp();
                 if (lane == 0) ptx::arrive_cluster(bar_empty + 8 * buf);
             };
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(tfull + 8 * buf, (unsigned)((cnt >> 1) & 1), s_abort, s_error,
-                                                       4, kWaitNs)))
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((cnt >> 1) & 1), s_abort, s_error,
+                                                       4)))
                 break;
             tc::fence_after();
             if constexpr (kDual) {
