@@ -36,9 +36,23 @@ struct DeviceGuard {
     }
 };
 
-static void launched(const char *what) {
+// Launches a kernel that may start before the one in front of it in the stream
+// has ended (each waits for that itself, after_previous): five short kernels in
+// a row cost the product's set-up once instead of five times.
+template <class... P, class... A>
+static void start(const char *what, void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.dynamicSmemBytes = (size_t)smem;
+    c.stream = s;
+    cudaLaunchAttribute at[1] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = at;
+    c.numAttrs = 1;
+    cuda_check(cudaLaunchKernelEx(&c, kernel, P(args)...), what);
     count_launches(1);
-    cuda_check(cudaGetLastError(), what);
 }
 
 static void require(bool ok, const char *msg) {
@@ -179,8 +193,7 @@ struct Operands {
             if (n > most) most = n;
         }
         const unsigned grid = blocks(most, 256) < 8u * 148 ? blocks(most, 256) : 8u * 148;
-        k_repitch<<<dim3(grid ? grid : 1, (unsigned)copies.size()), 256, 0, s>>>(p);
-        launched("copy to aligned rows");
+        start("copy to aligned rows", k_repitch, dim3(grid ? grid : 1, (unsigned)copies.size()), 256, 0, s, p);
     }
 };
 
@@ -200,8 +213,7 @@ static void read_checkpoint(const int8_t *q, const uint8_t *ex, int64_t rows, in
                             cudaStream_t s) {
     dim3 grid;
     const CkptPlan p = ckpt_plan(rows, cols, fits_vectors(x, ldx), grid);
-    k_unpack<T><<<grid, kCkptThreads, 0, s>>>(q, ex, p, x, ldx);
-    launched("read checkpoint");
+    start("read checkpoint", k_unpack<T>, grid, kCkptThreads, 0, s, q, ex, p, x, ldx);
 }
 
 static CUtensorMap tensor_map(const Matrix &m, bool bf16, int major) {
@@ -249,9 +261,8 @@ static void launch(const Product &d, cudaStream_t s) {
     raise_shared_memory<k_mma_product<T, AMAJ, BMAJ, EPI, ACT>>(kProductSmem);
     const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
     require(items < (int64_t)1 << 31, "more than 2^31 tiles in one product");
-    kernel<<<dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
-             kProductSmem, s>>>(p);
-    launched("training product");
+    start("training product", kernel, dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
+          kProductSmem, s, p);
 }
 
 // Parts of the depth for a product of few tiles: enough to give every SM pair
@@ -264,12 +275,11 @@ static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
 template <class T>
 static void join(const float *acc, int parts, int64_t M, int64_t N, int64_t ld, const int *shift, void *out,
                  cudaStream_t s) {
+    T *o = static_cast<T *>(out);
     if (parts > 8)
-        k_join<T, true><<<blocks(M * (ld / 4), 32), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out), N);
+        start("join parts", k_join<T, true>, blocks(M * (ld / 4), 32), 256, 0, s, acc, parts, M, N, ld, shift, o, N);
     else
-        k_join<T, false><<<blocks(M * (ld / 4), 256), 256, 0, s>>>(acc, parts, M, N, ld, shift, static_cast<T *>(out),
-                                                                   N);
-    launched("join parts");
+        start("join parts", k_join<T, false>, blocks(M * (ld / 4), 256), 256, 0, s, acc, parts, M, N, ld, shift, o, N);
 }
 // D = A B^T (+ A1 B1^T), or with outputs = 2 also A1 B^T, as dense 16-bit rows
 // at out[0], out[1]; the sums of a split depth are joined in acc.
@@ -453,9 +463,9 @@ HB_API int helrm_PackCheckpoint(int device, int dtype, int64_t tokens, int64_t i
         const CkptPlan p = ckpt_plan(tokens, inner, fits_vectors(x, tokens > 1 ? ldx : pitch(inner)), grid);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
-            k_pack<T><<<grid, kCkptThreads, 0, (cudaStream_t)stream>>>(static_cast<const T *>(x), ldx, p, q, ex);
+            start("pack checkpoint", k_pack<T>, grid, kCkptThreads, 0, (cudaStream_t)stream, static_cast<const T *>(x), ldx,
+                  p, q, ex);
         });
-        launched("pack checkpoint");
     });
 }
 
@@ -502,15 +512,13 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         d.e.at = at;
         d.e.target = targets;
         by_dtype(dtype, [&](auto t) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_LSE, 0>(d, s); });
-        if (joined) {
-            k_loss<false><<<dim3(blocks(tokens, 32), (unsigned)joined), 1024, 0, s>>>(
-                part, parts, nullptr, nullptr, 0, 0, tokens, nullptr, few);
-            launched("loss");
-        }
-        k_loss<true><<<blocks(tokens, 32), 1024, 0, s>>>(joined ? few : part, joined ? joined : parts, at, targets,
-                                                         ignore_index, vocab, tokens, loss,
-                                                         reinterpret_cast<float2 *>(lse));
-        launched("loss");
+        const float *none = nullptr;
+        const int64_t *no_targets = nullptr;
+        if (joined)
+            start("loss", k_loss<false>, dim3(blocks(tokens, 32), (unsigned)joined), 1024, 0, s, part, parts, none,
+                  no_targets, (int64_t)0, (int64_t)0, tokens, (float *)nullptr, few);
+        start("loss", k_loss<true>, blocks(tokens, 32), 1024, 0, s, joined ? few : part, joined ? joined : parts, at,
+              targets, ignore_index, vocab, tokens, loss, reinterpret_cast<float2 *>(lse));
     });
 }
 
@@ -533,12 +541,10 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         if (dtype != HELRM_FP16) shift = nullptr;
         auto prepare = [&](cudaStream_t s) {
             if (shift) {
-                k_loss_shift<<<1, 1024, 0, s>>>(dloss, targets, ignore_index, tokens, shift);
-                launched("loss shift");
+                start("loss shift", k_loss_shift, 1, 1024, 0, s, dloss, targets, ignore_index, tokens, shift);
             }
-            k_loss_rows<<<blocks(tokens, 256), 256, 0, s>>>(dloss, targets, reinterpret_cast<const float2 *>(lse),
-                                                            ignore_index, vocab, tokens, shift, rows);
-            launched("loss rows");
+            start("loss rows", k_loss_rows, blocks(tokens, 256), 256, 0, s, dloss, targets,
+                  reinterpret_cast<const float2 *>(lse), ignore_index, vocab, tokens, shift, rows);
         };
         const Narrow nr = narrow(tokens, inner, vocab);
         if (nr.on) {
@@ -570,8 +576,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 a.part_h = part;
                 a.error = runtime().error;
                 raise_shared_memory<k_loss_grads_narrow<T>>(kNarrowSmem);
-                k_loss_grads_narrow<T><<<nr.grid, kNarrowThreads, kNarrowSmem, s>>>(a);
-                launched("loss gradients");
+                start("loss gradients", k_loss_grads_narrow<T>, nr.grid, kNarrowThreads, kNarrowSmem, s, a);
                 if (dh) join<T>(part, nr.grid, tokens, inner, nr.depth, a.shift, dh, s);
             });
             return;

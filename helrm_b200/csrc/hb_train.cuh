@@ -46,6 +46,15 @@ template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(unsigned v)
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&v));
 }
 
+// Every kernel here starts while the one before it in the stream ends: it sets
+// itself up, lets the next one do the same, and touches no memory of others
+// until all of that one's work is visible.  Kernel pointers carry no
+// __restrict__, which would let a load move above the wait.
+__device__ __forceinline__ void after_previous() {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -139,10 +148,11 @@ struct EpiArgs {
 // (1024 rows, 7814 parts: 133 us in one pass).
 constexpr int kLossParts = 512;
 template <bool LAST>
-__global__ void __launch_bounds__(1024) k_loss(const float2 *__restrict__ part, int64_t parts,
-                                               const float *__restrict__ at, const int64_t *__restrict__ target,
-                                               int64_t ignore, int64_t vocab, int64_t M, float *__restrict__ loss,
-                                               float2 *__restrict__ lse) {
+__global__ void __launch_bounds__(1024) k_loss(const float2 *part, int64_t parts,
+                                               const float *at, const int64_t *target,
+                                               int64_t ignore, int64_t vocab, int64_t M, float *loss,
+                                               float2 *lse) {
+    after_previous();
     __shared__ float2 red[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t m = (int64_t)blockIdx.x * 32 + lane;
@@ -183,9 +193,10 @@ struct LossRow {
     int target;
 };
 constexpr int kNoTarget = -2147483647 - 1;
-__global__ void k_loss_rows(const float *__restrict__ dloss, const int64_t *__restrict__ target,
-                            const float2 *__restrict__ lse, int64_t ignore, int64_t vocab, int64_t M,
-                            const int *__restrict__ shift, LossRow *__restrict__ rows) {
+__global__ void k_loss_rows(const float *dloss, const int64_t *target,
+                            const float2 *lse, int64_t ignore, int64_t vocab, int64_t M,
+                            const int *shift, LossRow *rows) {
+    after_previous();
     const int64_t m = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (m >= M) return;
     LossRow r = {0.0f, 0.0f, 0.0f, kNoTarget};
@@ -203,8 +214,9 @@ __global__ void k_loss_rows(const float *__restrict__ dloss, const int64_t *__re
 
 // fp16 only: the power of two that brings the largest |dloss| of a row that
 // takes part to [2^14, 2^15), so that Z keeps the probabilities down to 2^-38.
-__global__ void k_loss_shift(const float *__restrict__ dloss, const int64_t *__restrict__ target, int64_t ignore,
-                             int64_t M, int *__restrict__ shift) {
+__global__ void k_loss_shift(const float *dloss, const int64_t *target, int64_t ignore,
+                             int64_t M, int *shift) {
+    after_previous();
     __shared__ float red[32];
     float top = 0.0f;
     for (int64_t m = threadIdx.x; m < M; m += blockDim.x)
@@ -222,7 +234,7 @@ __global__ void k_loss_shift(const float *__restrict__ dloss, const int64_t *__r
 // packed in 16 words.  The target's exp(..) - 1 is formed without cancellation.
 template <class T>
 __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col,
-                                       const float2 *__restrict__ lse, int64_t m) {
+                                       const float2 *lse, int64_t m) {
     const int at = r.target >= col && r.target < col + 32 ? r.target - col : -1;
     const bool any = __any_sync(0xffffffffu, at >= 0);
     float hot = 0.0f;
@@ -279,8 +291,9 @@ __device__ __forceinline__ void store8(unsigned short *row, int64_t col, int64_t
 }
 
 template <class T>
-__global__ void __launch_bounds__(kCkptThreads) k_pack(const T *__restrict__ x, int64_t ldx, CkptPlan p,
-                                                       int8_t *__restrict__ q, uint8_t *__restrict__ ex) {
+__global__ void __launch_bounds__(kCkptThreads) k_pack(const T *x, int64_t ldx, CkptPlan p,
+                                                       int8_t *q, uint8_t *ex) {
+    after_previous();
     const int r = threadIdx.x / p.per_block, c = blockIdx.y * p.per_block + threadIdx.x % p.per_block;
     const bool on = r < p.rows_block && c < p.chunks;
     uint4 v[kCkptRows];
@@ -339,8 +352,9 @@ __global__ void __launch_bounds__(kCkptThreads) k_pack(const T *__restrict__ x, 
 }
 
 template <class T>
-__global__ void __launch_bounds__(kCkptThreads) k_unpack(const int8_t *__restrict__ q, const uint8_t *__restrict__ ex,
-                                                         CkptPlan p, T *__restrict__ x, int64_t ldx) {
+__global__ void __launch_bounds__(kCkptThreads) k_unpack(const int8_t *q, const uint8_t *ex,
+                                                         CkptPlan p, T *x, int64_t ldx) {
+    after_previous();
     const int r = threadIdx.x / p.per_block, c = blockIdx.y * p.per_block + threadIdx.x % p.per_block;
     if (r >= p.rows_block || c >= p.chunks) return;
     uint2 v[kCkptRows];

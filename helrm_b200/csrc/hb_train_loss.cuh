@@ -128,6 +128,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
     __syncthreads();
     tc::fence_after();
     const unsigned tmem = *s_tmem;
+    after_previous();
     const unsigned tS = tmem, tDW = tmem + 256, tDH = tmem + 384;
 
     const int token_tiles = (int)((p.tokens + 127) / 128), groups = (token_tiles + p.group - 1) / p.group;

@@ -286,6 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     ptx::cluster_sync();
     tc::fence_after();
     const unsigned tmem = *s_tmem;
+    after_previous();
 
     // The launch has fewer than 2^31 items, so that all of this is 32-bit
     // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
@@ -592,8 +593,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 // are added up in order (148 parts of 1024 x 16: 37 us with a thread going
 // through all of them).
 template <class T, bool MANY>
-__global__ void __launch_bounds__(256) k_join(const float *__restrict__ acc, int parts, int64_t M, int64_t N,
-                                              int64_t ld, const int *shift, T *__restrict__ out, int64_t ldo) {
+__global__ void __launch_bounds__(256) k_join(const float *acc, int parts, int64_t M, int64_t N,
+                                              int64_t ld, const int *shift, T *out, int64_t ldo) {
+    after_previous();
     __shared__ float4 red[MANY ? 8 : 1][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t per = ld / 4, i = MANY ? (int64_t)blockIdx.x * 32 + lane : (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -632,6 +634,7 @@ struct Repitch {
     int64_t ld[4], rows[4], cols[4];
 };
 __global__ void k_repitch(const __grid_constant__ Repitch p) {
+    after_previous();
     const int k = blockIdx.y;
     const int64_t per = (p.cols[k] + 7) / 8, n = p.rows[k] * per;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
