@@ -130,6 +130,7 @@ struct EpiArgs {
     int first = 1;                      // 0: added to what acc holds
     float2 *part = nullptr;             // EPI_LSE: (max, sum) of each warp's columns, [part][row]
     float *at = nullptr;                // EPI_LSE: the target's logit
+    float grow = 1.0f;                  // EPI_LSE, EPI_Z: what a logit is multiplied by (logit_scale)
     const int64_t *target = nullptr;
     const float2 *lse = nullptr;        // EPI_Z: the row's (maximum, log of the sum relative to it)
     const struct LossRow *rows = nullptr;
@@ -234,7 +235,7 @@ __global__ void k_loss_shift(const float *dloss, const int64_t *target, int64_t 
 // packed in 16 words.  The target's exp(..) - 1 is formed without cancellation.
 template <class T>
 __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col,
-                                       const float2 *lse, int64_t m) {
+                                       const float2 *lse, int64_t m, float grow) {
     const int at = r.target >= col && r.target < col + 32 ? r.target - col : -1;
     const bool any = __any_sync(0xffffffffu, at >= 0);
     float hot = 0.0f;
@@ -243,10 +244,10 @@ __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const 
         float x = v[0];
 #pragma unroll
         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-        if (at >= 0) hot = expm1f(x - r.max - lse[m].y) * fabsf(r.g);
+        if (at >= 0) hot = expm1f(fmaf(x, grow, -r.max) - lse[m].y) * fabsf(r.g);
     }
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(v[j] - r.max, kLog2e, r.add));
+    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(fmaf(v[j], grow, -r.max), kLog2e, r.add));
     if (any) {
         asm volatile("");
 #pragma unroll

@@ -512,6 +512,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 const int64_t tg = target - n0;
                 float top = -INFINITY, sum = 0.0f;
+                const float log2e = kLog2e * e.grow;
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
                     float v[32];
@@ -531,7 +532,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        if (at >= 0) e.at[m] = x;
+                        if (at >= 0) e.at[m] = x * e.grow;
                     }
                     float m0 = v[0], m1 = v[1];
 #pragma unroll
@@ -542,15 +543,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        s0 += ex2((v[j] - ref) * kLog2e);
-                        s1 += ex2((v[j + 1] - ref) * kLog2e);
-                        s2 += ex2((v[j + 2] - ref) * kLog2e);
-                        s3 += ex2((v[j + 3] - ref) * kLog2e);
+                        s0 += ex2((v[j] - ref) * log2e);
+                        s1 += ex2((v[j + 1] - ref) * log2e);
+                        s2 += ex2((v[j + 2] - ref) * log2e);
+                        s3 += ex2((v[j + 3] - ref) * log2e);
                     }
-                    sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + ((s0 + s1) + (s2 + s3));
+                    sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + ((s0 + s1) + (s2 + s3));
                     top = mx;
                 }
-                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top, sum);
+                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top * e.grow, sum);
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
@@ -562,7 +563,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, m);
+                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, m, e.grow);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, p.M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }
