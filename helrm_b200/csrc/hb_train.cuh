@@ -66,6 +66,36 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 constexpr float kLog2e = 1.4426950408889634f;
+// Two 32-bit operations in one instruction, on neighbouring registers; each
+// half is rounded as the single operation is.
+__device__ __forceinline__ uint64_t join2(float lo, float hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+    return v;
+}
+__device__ __forceinline__ void split2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 // 1 / (1 + exp(-g)), within a few units of 2^-23: a division takes a slow path
 // for small numerators (gated 64 x 432 x 512: 17.8 us with it, 8.1 without)
 __device__ __forceinline__ float sigmoid(float g) { return rcp(1.0f + ex2(-kLog2e * g)); }
@@ -246,8 +276,14 @@ __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const 
         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
         if (at >= 0) hot = expm1f(fmaf(x, grow, -r.max) - lse[m].y) * fabsf(r.g);
     }
+    const uint64_t grow2 = join2(grow, grow), max2 = join2(-r.max, -r.max), log2 = join2(kLog2e, kLog2e),
+                   more2 = join2(r.add, r.add);
 #pragma unroll
-    for (int j = 0; j < 32; j++) v[j] = ex2(fmaf(fmaf(v[j], grow, -r.max), kLog2e, r.add));
+    for (int j = 0; j < 32; j += 2) {
+        split2(fma2(fma2(join2(v[j], v[j + 1]), grow2, max2), log2, more2), v[j], v[j + 1]);
+        v[j] = ex2(v[j]);
+        v[j + 1] = ex2(v[j + 1]);
+    }
     if (any) {
         asm volatile("");
 #pragma unroll

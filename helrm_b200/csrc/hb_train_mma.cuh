@@ -534,21 +534,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
                         if (at >= 0) e.at[m] = x * e.grow;
                     }
-                    float m0 = v[0], m1 = v[1];
+                    float m0 = max3(top, v[0], v[1]), m1 = v[2];
 #pragma unroll
-                    for (int j = 2; j < 32; j += 2) m0 = fmaxf(m0, v[j]), m1 = fmaxf(m1, v[j + 1]);
-                    const float mx = fmaxf(fmaxf(m0, m1), top);
+                    for (int j = 3; j < 31; j += 4) {
+                        m0 = max3(m0, v[j], v[j + 1]);
+                        m1 = max3(m1, v[j + 2], v[j + 3]);
+                    }
+                    const float mx = max3(m0, m1, v[31]);
                     // a row of minus infinities so far: relative to 0, nothing to add
                     const float ref = mx == -INFINITY ? 0.0f : mx;
-                    float s0 = 0.0f, s1 = 0.0f, s2 = 0.0f, s3 = 0.0f;
+                    const uint64_t ref2 = join2(-ref, -ref), log2 = join2(log2e, log2e);
+                    uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        s0 += ex2((v[j] - ref) * log2e);
-                        s1 += ex2((v[j + 1] - ref) * log2e);
-                        s2 += ex2((v[j + 2] - ref) * log2e);
-                        s3 += ex2((v[j + 3] - ref) * log2e);
+                        float x[4];
+                        split2(mul2(add2(join2(v[j], v[j + 1]), ref2), log2), x[0], x[1]);
+                        split2(mul2(add2(join2(v[j + 2], v[j + 3]), ref2), log2), x[2], x[3]);
+                        sum0 = add2(sum0, join2(ex2(x[0]), ex2(x[1])));
+                        sum1 = add2(sum1, join2(ex2(x[2]), ex2(x[3])));
                     }
-                    sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + ((s0 + s1) + (s2 + s3));
+                    float s0, s1;
+                    split2(add2(sum0, sum1), s0, s1);
+                    sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + (s0 + s1);
                     top = mx;
                 }
                 if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top * e.grow, sum);
