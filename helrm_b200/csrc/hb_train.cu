@@ -236,6 +236,8 @@ struct Product {
     Matrix a, b, a1, b1;
     int64_t M = 0, N = 0, K = 0, K1 = 0;
     int outputs = 1, splits = 1;
+    const LossPlan *plan = nullptr;
+    bool plan_k = false;
     EpiArgs e;
 };
 template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
@@ -255,6 +257,8 @@ static void launch(const Product &d, cudaStream_t s) {
     p.splits = d.splits;
     p.kb = (int)blocks(d.K, kDepth);
     p.kb1 = (int)blocks(d.K1, kDepth);
+    p.plan = d.plan;
+    p.plan_k = d.plan_k;
     p.e = d.e;
     p.error = runtime().error;
     auto kernel = k_mma_product<T, AMAJ, BMAJ, EPI, ACT>;
@@ -273,13 +277,12 @@ static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
     return n > 1 ? (int)n : 1;
 }
 template <class T>
-static void join(const float *acc, int parts, int64_t M, int64_t N, int64_t ld, const int *shift, void *out,
-                 cudaStream_t s) {
+static void join(const JoinArgs &j, void *out, cudaStream_t s) {
     T *o = static_cast<T *>(out);
-    if (parts > 8)
-        start("join parts", k_join<T, true>, blocks(M * (ld / 4), 32), 256, 0, s, acc, parts, M, N, ld, shift, o, N);
+    if (j.parts > 8)
+        start("join parts", k_join<T, true>, blocks(j.M * (j.ld / 4), 32), 256, 0, s, j, o);
     else
-        start("join parts", k_join<T, false>, blocks(M * (ld / 4), 256), 256, 0, s, acc, parts, M, N, ld, shift, o, N);
+        start("join parts", k_join<T, false>, blocks(j.M * (j.ld / 4), 256), 256, 0, s, j, o);
 }
 // D = A B^T (+ A1 B1^T), or with outputs = 2 also A1 B^T, as dense 16-bit rows
 // at out[0], out[1]; the sums of a split depth are joined in acc.
@@ -297,7 +300,8 @@ static void product_out(Product d, void *const *out, float *acc, cudaStream_t s)
     d.e.ldo = pad(d.N, 4);
     launch<T, AMAJ, BMAJ, EPI_SUM, 0>(d, s);
     for (int i = 0; i < d.outputs; i++)
-        join<T>(acc + (int64_t)i * d.splits * d.M * d.e.ldo, d.splits, d.M, d.N, d.e.ldo, d.e.shift, out[i], s);
+        join<T>({acc + (int64_t)i * d.splits * d.M * d.e.ldo, d.splits, d.M, d.M, d.N, d.e.ldo, d.e.plan, nullptr},
+                out[i], s);
 }
 static int64_t sums(int64_t M, int64_t N, int splits, int outputs) {
     return splits > 1 ? (int64_t)outputs * splits * M * pad(N, 4) : 0;
@@ -547,21 +551,25 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         require(dh || dw, "no output is asked for");
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
-        const Matrix mh = in.fit({h, tokens, inner, ldh}), mw = in.fit({wt, vocab, inner, ldw});
-        LossRow *rows = w.take<LossRow>(tokens);
-        int *shift = w.take<int>(dtype == HELRM_FP16 ? 1 : 0);
-        if (dtype != HELRM_FP16) shift = nullptr;
+        const Matrix mw = in.fit({wt, vocab, inner, ldw});
+        const bool scaled = dtype == HELRM_FP16;
+        const int64_t cap = pad(tokens, 256);  // the rows that take part, filled up
+        uint16_t *hc = w.take<uint16_t>(cap * pitch(inner));
+        const Matrix mh{hc, cap, inner, pitch(inner)};
+        LossRow *rows = w.take<LossRow>(cap);
+        int *src = w.take<int>(cap), *pos = w.take<int>(tokens);
+        LossPlan *plan = w.take<LossPlan>(1);
         auto prepare = [&](cudaStream_t s) {
-            if (shift) {
-                start("loss shift", k_loss_shift, 1, 1024, 0, s, dloss, targets, ignore_index, tokens, shift);
-            }
-            start("loss rows", k_loss_rows, blocks(tokens, 256), 256, 0, s, dloss, targets,
-                  reinterpret_cast<const float2 *>(lse), ignore_index, vocab, tokens, shift, rows);
+            in.copy(s);
+            start("loss rows", k_loss_plan, 1, 1024, 0, s, dloss, targets, reinterpret_cast<const float2 *>(lse),
+                  ignore_index, vocab, tokens, (int)scaled, rows, src, pos, plan);
+            start("loss rows", k_loss_gather, blocks(cap, 8), 256, 0, s, static_cast<const unsigned short *>(h), ldh,
+                  inner, fits_vectors(h, ldh), src, plan, hc, pitch(inner));
         };
         const Narrow nr = narrow(tokens, inner, vocab);
         if (nr.on) {
             const int groups = (int)blocks(blocks(tokens, 128), nr.group);
-            float *part = w.take<float>((int64_t)nr.grid * tokens * nr.depth);
+            float *part = w.take<float>((int64_t)nr.grid * cap * nr.depth);
             float *acc = w.take<float>(groups > 1 ? vocab * nr.depth : 0);
             void *dws = dw ? dw : w.take<uint16_t>(vocab * inner);
             if (sized(w, ws_bytes)) return;
@@ -571,34 +579,33 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
                 return;
             }
-            in.copy(s);
             prepare(s);
             by_dtype(dtype, [&](auto t) {
                 typedef decltype(t) T;
                 NarrowArgs a;
                 a.h = tensor_map(mh, std::is_same<T, __nv_bfloat16>::value, K_MAJOR);
                 a.w = tensor_map(mw, std::is_same<T, __nv_bfloat16>::value, K_MAJOR);
-                a.tokens = tokens, a.vocab = vocab;
+                a.capacity = cap, a.vocab = vocab;
                 a.inner = (int)inner, a.depth = nr.depth, a.group = nr.group;
                 a.rows = rows;
                 a.lse = reinterpret_cast<const float2 *>(lse);
-                a.shift = shift;
+                a.src = src;
+                a.plan = plan;
                 a.dw = dws;
                 a.acc_w = acc;
                 a.part_h = part;
                 a.error = runtime().error;
                 raise_shared_memory<k_loss_grads_narrow<T>>(kNarrowSmem);
                 start("loss gradients", k_loss_grads_narrow<T>, nr.grid, kNarrowThreads, kNarrowSmem, s, a);
-                if (dh) join<T>(part, nr.grid, tokens, inner, nr.depth, a.shift, dh, s);
+                if (dh) join<T>({part, nr.grid, cap, tokens, inner, nr.depth, plan, pos}, dh, s);
             });
             return;
         }
-        const int64_t cols = piece_columns(tokens, vocab), ldz = pitch(cols), lda = pad(inner, 4);
-        uint16_t *z = w.take<uint16_t>(tokens * ldz);
-        // dh over several pieces is a 32-bit sum; the parts of a piece's depth each keep their own
-        const int parts_h = dh ? parts_for(tokens, inner, cols, 1) : 1, parts_w = dw ? parts_for(cols, inner, tokens, 1) : 1;
-        const bool summed = dh && (cols < vocab || parts_h > 1);
-        float *acc = w.take<float>(summed ? parts_h * tokens * lda : 0);
+        const int64_t cols = piece_columns(cap, vocab), ldz = pitch(cols), lda = pad(inner, 4);
+        uint16_t *z = w.take<uint16_t>(cap * ldz);
+        // dh is a 32-bit sum over the pieces, for each part of a piece's depth, of the rows that take part
+        const int parts_h = dh ? parts_for(cap, inner, cols, 1) : 1, parts_w = dw ? parts_for(cols, inner, cap, 1) : 1;
+        float *acc = w.take<float>(dh ? parts_h * cap * lda : 0);
         float *acc_w = w.take<float>(sums(cols, inner, parts_w, 1));
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
@@ -607,21 +614,21 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
             return;
         }
-        in.copy(s);
         prepare(s);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             for (int64_t c0 = 0; c0 < vocab; c0 += cols) {
                 const int64_t n = vocab - c0 < cols ? vocab - c0 : cols;
-                const Matrix mc{static_cast<const T *>(mw.p) + c0 * mw.ld, n, inner, mw.ld}, mz{z, tokens, n, ldz};
+                const Matrix mc{static_cast<const T *>(mw.p) + c0 * mw.ld, n, inner, mw.ld}, mz{z, cap, n, ldz};
                 Product d;
                 d.a = mh, d.b = mc;
-                d.M = tokens, d.N = n, d.K = inner;
-                d.e.shift = shift;
+                d.M = cap, d.N = n, d.K = inner;
+                d.plan = plan;
                 d.e.o0 = z;
                 d.e.ldo = ldz;
                 d.e.vec = 1;
                 d.e.rows = rows;
+                d.e.src = src;
                 d.e.lse = reinterpret_cast<const float2 *>(lse);
                 d.e.col0 = c0;
                 d.e.grow = logit_scale(inner);
@@ -629,30 +636,28 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 if (dw) {
                     Product g;
                     g.a = mz, g.b = mh;
-                    g.M = n, g.N = inner, g.K = tokens;
+                    g.M = n, g.N = inner, g.K = cap;
                     g.splits = parts_w;
-                    g.e.shift = shift;
+                    g.plan = plan;
+                    g.plan_k = true;
+                    g.e.plan = plan;
                     void *out = static_cast<T *>(dw) + c0 * inner;
                     product_out<T, MN_MAJOR, MN_MAJOR>(g, &out, acc_w, s);
                 }
                 if (dh) {
                     Product g;
                     g.a = mz, g.b = mc;
-                    g.M = tokens, g.N = inner, g.K = n;
-                    g.e.shift = shift;
-                    if (summed) {
-                        // the last piece may be too short for every part: those keep their sums
-                        g.splits = parts_h < (int)blocks(n, kDepth) ? parts_h : (int)blocks(n, kDepth);
-                        g.e.acc = acc;
-                        g.e.ldo = lda;
-                        g.e.first = c0 == 0;
-                        launch<T, K_MAJOR, MN_MAJOR, EPI_SUM, 0>(g, s);
-                    } else {
-                        product_out<T, K_MAJOR, MN_MAJOR>(g, &dh, nullptr, s);
-                    }
+                    g.M = cap, g.N = inner, g.K = n;
+                    g.plan = plan;
+                    // the last piece may be too short for every part: those keep their sums
+                    g.splits = parts_h < (int)blocks(n, kDepth) ? parts_h : (int)blocks(n, kDepth);
+                    g.e.acc = acc;
+                    g.e.ldo = lda;
+                    g.e.first = c0 == 0;
+                    launch<T, K_MAJOR, MN_MAJOR, EPI_SUM, 0>(g, s);
                 }
             }
-            if (summed) join<T>(acc, parts_h, tokens, inner, lda, shift, dh, s);
+            if (dh) join<T>({acc, parts_h, cap, tokens, inner, lda, plan, pos}, dh, s);
         });
     });
 }

@@ -37,11 +37,12 @@ constexpr int kNarrowSmem = (kNarrowGroup + 2 + 4) * kPanel + 8 * kNarrowBars + 
 
 struct NarrowArgs {
     CUtensorMap h, w;
-    int64_t tokens, vocab;
+    int64_t capacity, vocab;  // capacity: rows of h and of a block's partial sums
     int inner, depth, group;  // depth: inner rounded up to 16; group: token tiles of a group
     const LossRow *rows;
     const float2 *lse;
-    const int *shift;
+    const int *src;
+    const LossPlan *plan;
     void *dw;                 // dense rows
     float *acc_w;             // [vocab][depth] running sums, for several groups
     float *part_h;            // [block][tokens][depth]
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
     after_previous();
     const unsigned tS = tmem, tDW = tmem + 256, tDH = tmem + 384;
 
-    const int token_tiles = (int)((p.tokens + 127) / 128), groups = (token_tiles + p.group - 1) / p.group;
+    const int token_tiles = max(1, (p.plan->count + 127) / 128), groups = (token_tiles + p.group - 1) / p.group;
     const int blocks_all = (int)((p.vocab + 127) / 128);
     const int mine = (blocks_all - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
 
@@ -245,11 +246,11 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         auto wait_all = [&](unsigned a, unsigned parity) {
             return __all_sync(0xffffffffu, mbar_wait(a, parity, s_abort, s_error, 4));
         };
-        const float unscale = p.shift ? ldexpf(1.0f, -*p.shift) : 1.0f;
+        const float unscale = ldexpf(1.0f, -p.plan->shift);
         const bool vec = p.inner % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dw) & 15) == 0;
-        auto fetch = [&](int64_t m) {
-            LossRow q = {0.0f, 0.0f, 0.0f, kNoTarget};
-            if (m < p.tokens) *reinterpret_cast<float4 *>(&q) = reinterpret_cast<const float4 *>(p.rows)[m];
+        auto fetch = [&](int64_t m) {  // the rows that fill up the last tile are there
+            LossRow q;
+            *reinterpret_cast<float4 *>(&q) = reinterpret_cast<const float4 *>(p.rows)[m];
             return q;
         };
         // dW of the block that was finished last: 16 of its columns a warp
@@ -335,7 +336,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
                     }
-                    loss_z<T>(v, w, row, col + c * 32, p.lse, m, 1.0f);
+                    loss_z<T>(v, w, row, col + c * 32, p.lse, p.src, m, 1.0f);
                     // the products that read this buffer two tiles ago
                     if (!c && !(ok = wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1))) break;
 #pragma unroll
@@ -362,11 +363,9 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 float v[16];
                 ptx::load16(tDH + t * p.depth + lanes + c0, v);
                 ptx::wait16(v);
-                if (m < p.tokens) {
-                    float4 *o = reinterpret_cast<float4 *>(p.part_h + ((int64_t)blockIdx.x * p.tokens + m) * p.depth + c0);
+                float4 *o = reinterpret_cast<float4 *>(p.part_h + ((int64_t)blockIdx.x * p.capacity + m) * p.depth + c0);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) o[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-                }
+                for (int k = 0; k < 4; k++) o[k] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
             }
             tc::fence_before();
             __syncwarp();

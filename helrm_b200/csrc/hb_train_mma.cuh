@@ -54,6 +54,8 @@ struct ProductArgs {
     int outputs;           // 2: a second product A1 B^T into o1
     int splits;            // the depth in this many parts, each with a partial sum of its own
     int kb, kb1;           // slices of (A, B), and after them of (A1, B1)
+    const LossPlan *plan;  // not NULL: the rows that take part, known on the device only, are
+    int plan_k;            // 0: the rows of the tiles, 1: the depth
     EpiArgs e;
     int *error;            // host memory
 };
@@ -290,9 +292,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 
     // The launch has fewer than 2^31 items, so that all of this is 32-bit
     // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
-    const unsigned tiles = (unsigned)p.tiles_m * p.tiles_n;
+    int tiles_m = p.tiles_m, kb = p.kb;
+    int64_t M = p.M;
+    if (p.plan) {
+        const int n = p.plan->filled;
+        if (p.plan_k)
+            kb = n / kDepth;
+        else
+            tiles_m = n / kRows, M = n;
+    }
+    const unsigned tiles = (unsigned)tiles_m * p.tiles_n;
     const unsigned items = tiles * p.splits * p.outputs;
-    const int depth = p.kb + p.kb1;
+    const int depth = kb + p.kb1;
     const unsigned first_item = blockIdx.x >> 1, step = gridDim.x >> 1;
     struct Item {
         int out, split, mt, nt, k0, k1;
@@ -311,8 +322,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             t.k0 = (int)((int64_t)depth * t.split / p.splits);
             t.k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
         }
-        const unsigned per = 8u * p.tiles_n, g = p.tiles_m > 8 ? i / per : 0;
-        const unsigned r = i - g * per, h = p.tiles_m - g * 8;
+        const unsigned per = 8u * p.tiles_n, g = tiles_m > 8 ? i / per : 0;
+        const unsigned r = i - g * per, h = tiles_m - g * 8;
         if (h >= 8) {
             t.mt = g * 8 + (r & 7);
             t.nt = r >> 3;
@@ -341,8 +352,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     }
                     if (rank == 0) tc::mbar_arrive_tx(full + 8 * s, 4 * kOperand);
                     const unsigned bar = ptx::of_first(full + 8 * s);
-                    const bool second = k >= p.kb;
-                    const int x = (second ? k - p.kb : k) * kDepth;
+                    const bool second = k >= kb;
+                    const int x = (second ? k - kb : k) * kDepth;
                     const CUtensorMap *ma = second || t.out ? &p.a1 : &p.a;
                     const CUtensorMap *mb = second || (kDual && rank) ? &p.b1 : &p.b;
                     const unsigned da = sA + s * kOperand, db = sB + s * kOperand;
@@ -379,7 +390,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                                    ((unsigned)AMAJ << 15) | ((unsigned)BMAJ << 16) | ((kCols >> 3) << 17) |
                                    ((kRows >> 4) << 24);
             // 16 of k: 32 bytes along a row, or 16 rows of 128 bytes
-            constexpr unsigned ka = AMAJ == K_MAJOR ? 32 : 2048, kb = BMAJ == K_MAJOR ? 32 : 2048;
+            constexpr unsigned step_a = AMAJ == K_MAJOR ? 32 : 2048, step_b = BMAJ == K_MAJOR ? 32 : 2048;
             int s = 0;
             unsigned ph = 0;
             unsigned n = 0;
@@ -399,7 +410,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     const uint64_t da = ptx::descriptor(sA + s * kOperand), db = ptx::descriptor(sB + s * kOperand);
 #pragma unroll
                     for (int j = 0; j < kDepth / 16; j++)
-                        ptx::mma(d, da + ((j * ka) >> 4), db + ((j * kb) >> 4), idesc, k > t.k0 || j > 0);
+                        ptx::mma(d, da + ((j * step_a) >> 4), db + ((j * step_b) >> 4), idesc, k > t.k0 || j > 0);
                     ptx::commit_both(empty + 8 * s);
                     if (++s == kStages) s = 0, ph ^= 1;
                 }
@@ -425,8 +436,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         Item next = item(first_item + set * step);
         auto fetch = [&] {
             const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
-            if (EPI == EPI_LSE) next_target = m < p.M ? e.target[m] : -1;
-            if (EPI == EPI_Z && m < p.M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
+            if (EPI == EPI_LSE) next_target = m < M ? e.target[m] : -1;
+            if (EPI == EPI_Z && m < M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
         if (first_item + set * step < items) fetch();
         for (unsigned i = first_item + set * step; i < items; i += kSets * step, cnt += kSets) {
@@ -461,7 +472,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::load32(acc + col, g);
                     ptx::load32(acc + 128 + col, u);
                     if constexpr (EPI == EPI_GATED_BWD)
-                        load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, p.M, n0 + col, p.N, vdh, lane);
+                        load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, M, n0 + col, p.N, vdh, lane);
                     ptx::wait32(g);
                     ptx::wait32(u);
                     if (c == 1) release();
@@ -469,7 +480,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 #pragma unroll
                         for (int j = 0; j < 16; j++)
                             w[j] = pack2<T>(act_f<ACT>(g[2 * j]) * u[2 * j], act_f<ACT>(g[2 * j + 1]) * u[2 * j + 1]);
-                        store_block<T>(st, w, o0, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, p.N, vec, lane);
                     } else {
                         unsigned wu[16];
 #pragma unroll
@@ -481,13 +492,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                             w[j] = pack2<T>(dh.x * u[2 * j] * d0, dh.y * u[2 * j + 1] * d1);
                             wu[j] = pack2<T>(dh.x * a0, dh.y * a1);
                         }
-                        store_block<T>(st, w, o0, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
-                        store_block<T>(st, wu, o1, e.ldo, m0, p.M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, wu, o1, e.ldo, m0, M, n0 + col, p.N, vec, lane);
                     }
                 }
             } else if constexpr (EPI == EPI_STORE || EPI == EPI_SUM) {
                 const int64_t n0 = (int64_t)t.nt * kCols;
-                const float scale = EPI == EPI_STORE && e.shift ? ldexpf(1.0f, -*e.shift) : 1.0f;
+                const float scale = EPI == EPI_STORE && e.plan ? ldexpf(1.0f, -e.plan->shift) : 1.0f;
+                const bool nothing = t.k0 == t.k1;  // a part of a depth that turned out short: no product ran
 #pragma unroll 1
                 for (int c = 0; c < 4; c++) {
                     const int col = half * 128 + c * 32;
@@ -496,15 +508,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::wait32(v);
                     if (c == 3) release();
                     if (n0 + col >= p.N) continue;
+                    if (nothing) {
+#pragma unroll
+                        for (int j = 0; j < 32; j++) v[j] = 0.0f;
+                    }
                     if constexpr (EPI == EPI_STORE) {
                         unsigned w[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) w[j] = pack2<T>(v[2 * j] * scale, v[2 * j + 1] * scale);
-                        store_block<T>(st, w, static_cast<T *>(t.out ? e.o1 : e.o0), e.ldo, m0, p.M, n0 + col, p.N,
+                        store_block<T>(st, w, static_cast<T *>(t.out ? e.o1 : e.o0), e.ldo, m0, M, n0 + col, p.N,
                                        e.vec & 1, lane);
                     } else {
                         float *o = e.acc + ((int64_t)t.out * p.splits + t.split) * p.M * e.ldo;
-                        store_sums(st, v, o, e.ldo, m0, p.M, n0 + col, !e.first, lane);
+                        store_sums(st, v, o, e.ldo, m0, M, n0 + col, !e.first, lane);
                     }
                 }
             } else if constexpr (EPI == EPI_LSE) {
@@ -558,7 +574,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + (s0 + s1);
                     top = mx;
                 }
-                if (m < p.M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top * e.grow, sum);
+                if (m < M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top * e.grow, sum);
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
@@ -570,8 +586,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, m, e.grow);
-                    store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, p.M, n0 + c * 32, p.N, e.vec & 1, lane);
+                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, e.src, m, e.grow);
+                    store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }
         }
@@ -597,40 +613,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 }
 
 // out[m][n] = 16-bit (2^-shift * sum over the parts of acc[part][m][n]), four
-// columns a lane.  MANY: the 8 warps of a block take every 8th part each and
-// are added up in order (148 parts of 1024 x 16: 37 us with a thread going
-// through all of them).
+// columns a lane; with pos the sums are those of row pos[m], or none (-1).
+// MANY: the 8 warps of a block take every 8th part each and are added up in
+// order (148 parts of 1024 x 16: 37 us with a thread going through all of them).
+struct JoinArgs {
+    const float *acc;
+    int parts;
+    int64_t rows, M, N, ld;  // rows of a part, rows and columns of the result, pitch of acc
+    const LossPlan *plan;    // not NULL: its shift
+    const int *pos;
+};
 template <class T, bool MANY>
-__global__ void __launch_bounds__(256) k_join(const float *acc, int parts, int64_t M, int64_t N,
-                                              int64_t ld, const int *shift, T *out, int64_t ldo) {
+__global__ void __launch_bounds__(256) k_join(JoinArgs p, T *out) {
     after_previous();
     __shared__ float4 red[MANY ? 8 : 1][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t per = ld / 4, i = MANY ? (int64_t)blockIdx.x * 32 + lane : (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (!MANY && i >= M * per) return;
+    const int64_t per = p.ld / 4, i = MANY ? (int64_t)blockIdx.x * 32 + lane : (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (!MANY && i >= p.M * per) return;
+    const int64_t m = i / per, c = i - m * per;
+    int64_t from = -1;
+    if (i < p.M * per) from = p.pos ? p.pos[m] : m;
     float4 s = make_float4(0, 0, 0, 0);
     auto add = [&](const float4 &v) { s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w; };
-    if (i < M * per) {
+    if (from >= 0) {
+        const float4 *a = reinterpret_cast<const float4 *>(p.acc) + from * per + c;
 #pragma unroll 4
-        for (int k = MANY ? warp : 0; k < parts; k += MANY ? 8 : 1)
-            add(reinterpret_cast<const float4 *>(acc)[k * M * per + i]);
+        for (int k = MANY ? warp : 0; k < p.parts; k += MANY ? 8 : 1) add(a[k * p.rows * per]);
     }
     if (MANY) {
         red[warp][lane] = s;
         __syncthreads();
-        if (warp || i >= M * per) return;
+        if (warp || i >= p.M * per) return;
         for (int k = 1; k < 8; k++) add(red[k][lane]);
     }
-    const int64_t m = i / per, n = (i - m * per) * 4;
-    const float scale = shift ? ldexpf(1.0f, -*shift) : 1.0f;
+    const int64_t n = c * 4;
+    const float scale = p.plan ? ldexpf(1.0f, -p.plan->shift) : 1.0f;
     const float v[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
-    T *o = out + m * ldo + n;
-    if (ldo % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 7) == 0 && n + 4 <= N) {
+    T *o = out + m * p.N + n;
+    if (p.N % 4 == 0 && n < p.N && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
         *reinterpret_cast<uint2 *>(o) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
     } else {
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            if (n + j < N) o[j] = from_f<T>(v[j]);
+            if (n + j < p.N) o[j] = from_f<T>(v[j]);
     }
 }
 

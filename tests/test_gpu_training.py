@@ -394,6 +394,33 @@ def test_loss_every_row_ignored(tr):
         assert not dh.any() and not dw.any() and torch.isfinite(dh).all() and torch.isfinite(dw).all()
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("shape", [(300, 72, 500), (5000, 40, 300), (200, 24, 19000), (4100, 16, 19001), (9000, 100, 130)])
+def test_loss_ignored_rows_reach_nothing(tr, shape, dt):
+    """Most rows are ignored and hold infinities and NaN: the gradients are those of the others alone."""
+    n, k, v = shape
+    dt = DTYPES[dt]
+    h, w = rand(n, k, dtype=dt), rand(v, k, dtype=dt, std=k ** -0.5, seed=1)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    t = torch.randint(0, v, (n,), generator=gen, device="cuda")
+    out = torch.rand(n, generator=gen, device="cuda") < 0.7
+    out[n // 3:n // 2] = True
+    out[n - 1] = False
+    t[out] = -100
+    g = (0.5 + torch.rand(n, generator=gen, device="cuda")) / n * (1024.0 if dt == torch.float16 else 1.0)
+    bad = h.clone()
+    bad[out] = torch.tensor([float("nan"), float("inf"), float("-inf")], device="cuda", dtype=dt)[
+        torch.randint(0, 3, (int(out.sum()), 1), generator=gen, device="cuda")].expand(-1, k)
+    loss, lse = tr.vocabulary_loss_forward(bad, w, t)
+    assert not loss[out].any() and torch.isfinite(loss).all()
+    dh, dw = tr.vocabulary_loss_backward(g, bad, w, t, lse)
+    assert not dh[out].any() and torch.isfinite(dh).all() and torch.isfinite(dw).all()
+    keep = ~out
+    wdh, wdw = loss_grads(g[keep], h[keep], w, t[keep])
+    within(dh[keep].contiguous(), wdh, "dh")
+    within(dw, wdw, "dw")
+
+
 def test_loss_target_out_of_range(tr):
     h, w = rand(6, 24, dtype=torch.bfloat16), rand(50, 24, dtype=torch.bfloat16)
     t = torch.tensor([0, 49, 50, -1, -100, 3], device="cuda")
