@@ -561,10 +561,12 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         LossPlan *plan = w.take<LossPlan>(1);
         auto prepare = [&](cudaStream_t s) {
             in.copy(s);
-            start("loss rows", k_loss_plan, 1, 1024, 0, s, dloss, targets, reinterpret_cast<const float2 *>(lse),
-                  ignore_index, vocab, tokens, (int)scaled, rows, src, pos, plan);
-            start("loss rows", k_loss_gather, blocks(cap, 8), 256, 0, s, static_cast<const unsigned short *>(h), ldh,
-                  inner, fits_vectors(h, ldh), src, plan, hc, pitch(inner));
+            LossRows r = {dloss, targets, reinterpret_cast<const float2 *>(lse), ignore_index, vocab, tokens,
+                          static_cast<const unsigned short *>(h), ldh, inner, fits_vectors(h, ldh), scaled, 0, rows, src,
+                          pos, plan, hc, pitch(inner)};
+            // 32 rows a block, or at most 512 blocks
+            r.per = (int)(cap > 32 * 512 ? pad(blocks(cap, 512), 32) : 32);
+            start("loss rows", k_loss_rows, blocks(cap, r.per), 1024, 0, s, r);
         };
         const Narrow nr = narrow(tokens, inner, vocab);
         if (nr.on) {

@@ -257,36 +257,53 @@ struct LossPlan {
     int count;   // rows that take part
     int shift;   // fp16: Z is scaled by 2^shift
 };
-// One block: a pass over the targets, each thread four of them at a time.
-// scaled (fp16): the power of two that brings the largest |dloss| of a row that
-// takes part to [2^14, 2^15), so that Z keeps the probabilities down to 2^-38.
-__global__ void __launch_bounds__(1024) k_loss_plan(const float *dloss, const int64_t *target, const float2 *lse,
-                                                    int64_t ignore, int64_t vocab, int64_t M, int scaled, LossRow *rows,
-                                                    int *src, int *pos, LossPlan *plan) {
+// Each block goes through all the targets, four a thread at a time, keeps the
+// `per` places that are its own, and copies their rows to 16-byte boundaries
+// (zeros where they fill up): one launch, where a plan by one block and a copy
+// after it took 10 us.  scaled (fp16): the power of two that brings the largest
+// |dloss| of a row that takes part to [2^14, 2^15), so that Z keeps the
+// probabilities down to 2^-38.
+struct LossRows {
+    const float *dloss;
+    const int64_t *target;
+    const float2 *lse;
+    int64_t ignore, vocab, M;
+    const unsigned short *h;
+    int64_t ldh, cols;
+    bool vec, scaled;
+    int per;
+    LossRow *rows;
+    int *src, *pos;
+    LossPlan *plan;
+    unsigned short *out;
+    int64_t ldo;
+};
+__global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
     after_previous();
     __shared__ float red[32];
-    __shared__ int sums[33];
+    __shared__ int sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     int shift = 0;
-    if (scaled) {
+    if (p.scaled) {
         float top = 0.0f;
-        for (int64_t m = threadIdx.x; m < M; m += 1024)
-            if (target[m] != ignore) top = fmaxf(top, fabsf(dloss[m]));
+        for (int64_t m = threadIdx.x; m < p.M; m += 1024)
+            if (p.target[m] != p.ignore) top = fmaxf(top, fabsf(p.dloss[m]));
         for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if (lane == 0) red[warp] = top;
         __syncthreads();
         for (int i = 0; i < 32; i++) top = fmaxf(top, red[i]);
         shift = top > 0.0f && top < INFINITY ? max(-100, min(120, 14 - ilogbf(top))) : 0;
     }
+    const int first = blockIdx.x * p.per, last = first + p.per;
     int base = 0;
-    for (int64_t m0 = 0; m0 < M; m0 += 4096) {
+    for (int64_t m0 = 0; m0 < p.M; m0 += 4096) {
         int64_t t[4];
         int mine = 0;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int64_t m = m0 + threadIdx.x * 4 + k;
-            t[k] = m < M ? target[m] : ignore;
-            mine += t[k] != ignore;
+            t[k] = m < p.M ? p.target[m] : p.ignore;
+            mine += t[k] != p.ignore;
         }
         int before = mine;
         for (int o = 1; o < 32; o <<= 1) {
@@ -309,45 +326,40 @@ __global__ void __launch_bounds__(1024) k_loss_plan(const float *dloss, const in
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int64_t m = m0 + threadIdx.x * 4 + k;
-            if (m >= M) break;
-            if (t[k] == ignore) {
-                pos[m] = -1;
-                continue;
+            if (m >= p.M) break;
+            const bool on = t[k] != p.ignore;
+            if (blockIdx.x == 0) p.pos[m] = on ? j : -1;
+            if (!on) continue;
+            if (j >= first && j < last) {
+                const bool in = t[k] >= 0 && t[k] < p.vocab;
+                const float2 l = p.lse[m];
+                LossRow r;
+                r.g = in ? p.dloss[m] : NAN;
+                if (shift) r.g = ldexpf(r.g, shift);
+                r.max = l.x;
+                r.add = log2f(fabsf(r.g)) - l.y * kLog2e;
+                r.target = in ? (int)t[k] : -1;
+                p.rows[j] = r;
+                p.src[j] = (int)m;
             }
-            const bool in = t[k] >= 0 && t[k] < vocab;
-            const float2 l = lse[m];
-            LossRow r;
-            r.g = in ? dloss[m] : NAN;
-            if (shift) r.g = ldexpf(r.g, shift);
-            r.max = l.x;
-            r.add = log2f(fabsf(r.g)) - l.y * kLog2e;
-            r.target = in ? (int)t[k] : -1;
-            rows[j] = r;
-            src[j] = (int)m;
-            pos[m] = j++;
+            j++;
         }
         __syncthreads();
     }
-    const int filled = max(256, (base + 255) / 256 * 256);
-    for (int j = base + threadIdx.x; j < filled; j += 1024) {
-        rows[j] = {0.0f, 0.0f, 0.0f, kNoTarget};
-        src[j] = -1;
+    const int filled = max(256, (base + 255) / 256 * 256), end = min(last, filled);
+    for (int j = max(first, base) + threadIdx.x; j < end; j += 1024) {
+        p.rows[j] = {0.0f, 0.0f, 0.0f, kNoTarget};
+        p.src[j] = -1;
     }
-    if (threadIdx.x == 0) *plan = {filled, base, shift};
-}
-
-// The rows that take part, on 16-byte boundaries; zeros where rows fill up.  A
-// warp a row.
-__global__ void __launch_bounds__(256) k_loss_gather(const unsigned short *h, int64_t ld, int64_t cols, bool vec,
-                                                     const int *src, const LossPlan *plan, unsigned short *out,
-                                                     int64_t ldo) {
-    after_previous();
-    const int64_t j = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (j >= plan->filled) return;
-    const int64_t m = src[j];
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.plan = {filled, base, shift};
+    __syncthreads();
+    for (int j = first + warp; j < end; j += 32) {  // a warp a row
+        const int64_t m = p.src[j];
 #pragma unroll 4
-    for (int64_t c = (threadIdx.x & 31) * 8; c < ldo; c += 256)
-        *reinterpret_cast<uint4 *>(out + j * ldo + c) = m < 0 ? make_uint4(0, 0, 0, 0) : load8(h + m * ld, c, cols, vec);
+        for (int64_t c = lane * 8; c < p.ldo; c += 256)
+            *reinterpret_cast<uint4 *>(p.out + j * p.ldo + c) =
+                m < 0 ? make_uint4(0, 0, 0, 0) : load8(p.h + m * p.ldh, c, p.cols, p.vec);
+    }
 }
 
 // 32 logits of a row, the first of them column `col` of the vocabulary, to Z,
