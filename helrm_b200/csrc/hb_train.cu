@@ -159,7 +159,10 @@ struct Matrix {
     const void *p = nullptr;
     int64_t rows = 0, cols = 0, ld = 0;
 };
-static int64_t pitch(int64_t cols) { return pad(cols, 8); }
+// Row pitch of the workspace's matrices: whole 128-byte lines, so that a tile's
+// rows touch no line twice (gated forward of 2048 x 1000 x 1536 with rows of
+// 2000 bytes 18.3 us, of 2048 bytes 15.0), for narrow rows whole 16 bytes.
+static int64_t pitch(int64_t cols) { return pad(cols, cols > 64 ? 64 : 8); }
 static bool fits_vectors(const void *p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 // Operands that the TMA unit can read: what lies on 16-byte boundaries as it
@@ -188,7 +191,7 @@ struct Operands {
             const Matrix &m = copies[i].from;
             p.from[i] = static_cast<const unsigned short *>(m.p);
             p.to[i] = copies[i].to;
-            p.ld[i] = m.ld, p.rows[i] = m.rows, p.cols[i] = m.cols;
+            p.ld[i] = m.ld, p.rows[i] = m.rows, p.cols[i] = m.cols, p.pitch[i] = pitch(m.cols);
             const int64_t n = m.rows * ((m.cols + 7) / 8);
             if (n > most) most = n;
         }

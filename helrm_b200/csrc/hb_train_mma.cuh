@@ -664,15 +664,15 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs p, T *out) {
 struct Repitch {
     const unsigned short *from[4];
     unsigned short *to[4];
-    int64_t ld[4], rows[4], cols[4];
+    int64_t ld[4], rows[4], cols[4], pitch[4];
 };
 __global__ void k_repitch(const __grid_constant__ Repitch p) {
     after_previous();
     const int k = blockIdx.y;
-    const int64_t per = (p.cols[k] + 7) / 8, n = p.rows[k] * per;
+    const int64_t per = (p.cols[k] + 7) / 8, n = p.rows[k] * per;  // what lies past a row's end is never read
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
         const int64_t r = i / per, c = i % per * 8;
-        reinterpret_cast<uint4 *>(p.to[k])[i] = load8(p.from[k] + r * p.ld[k], c, p.cols[k], false);
+        *reinterpret_cast<uint4 *>(p.to[k] + r * p.pitch[k] + c) = load8(p.from[k] + r * p.ld[k], c, p.cols[k], false);
     }
 }
 
