@@ -242,6 +242,7 @@ struct Product {
     const LossPlan *plan = nullptr;
     bool plan_k = false;
     EpiArgs e;
+    int tile_cols() const { return N <= 128 ? 128 : kCols; }
 };
 template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
 static void launch(const Product &d, cudaStream_t s) {
@@ -255,7 +256,9 @@ static void launch(const Product &d, cudaStream_t s) {
     p.M = d.M;
     p.N = d.N;
     p.tiles_m = (int)blocks(d.M, kRows);
-    p.tiles_n = (int)blocks(d.N, dual ? 128 : kCols);
+    p.cols = d.tile_cols();
+    static_assert(BMAJ == MN_MAJOR || (EPI != EPI_STORE && EPI != EPI_SUM), "a K-major B comes in 256-column tiles");
+    p.tiles_n = (int)blocks(d.N, dual ? 128 : EPI == EPI_STORE || EPI == EPI_SUM ? p.cols : kCols);
     p.outputs = d.outputs;
     p.splits = d.splits;
     p.kb = (int)blocks(d.K, kDepth);

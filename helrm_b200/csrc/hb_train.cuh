@@ -364,14 +364,15 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
 
 // 32 logits of a row, the first of them column `col` of the vocabulary, to Z,
 // packed in 16 words.  The target's exp(..) - 1 is formed without cancellation.
+// any: whether some row of the warp may have its target here.
 template <class T>
-__device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col,
+__device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col, bool any,
                                        const float2 *lse, const int *src, int64_t m, float grow) {
-    const int at = r.target >= col && r.target < col + 32 ? r.target - col : -1;
-    const bool any = __any_sync(0xffffffffu, at >= 0);
+    int at = -1;
     float hot = 0.0f;
     if (any) {
         asm volatile("");  // a branch: not 32 selections for every 32 logits
+        if (r.target >= col && r.target < col + 32) at = r.target - col;
         float x = v[0];
 #pragma unroll
         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;

@@ -324,6 +324,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                 next = fetch(first + t * 128);
                 if (!(ok = wait_all(sfull + 8 * set, (n >> 1) & 1))) break;
                 tc::fence_after();
+                const bool any = __any_sync(0xffffffffu, row.target >= col && row.target < col + 64);
                 unsigned char *z = zbuf + set * 2 * kPanel + (quarter & 1) * kPanel + r * 128;
 #pragma unroll 1
                 for (int c = 0; c < 2; c++) {
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
                     }
-                    loss_z<T>(v, w, row, col + c * 32, p.lse, p.src, m, 1.0f);
+                    loss_z<T>(v, w, row, col + c * 32, any, p.lse, p.src, m, 1.0f);
                     // the products that read this buffer two tiles ago
                     if (!c && !(ok = wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1))) break;
 #pragma unroll

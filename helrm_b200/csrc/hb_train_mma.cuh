@@ -51,6 +51,7 @@ struct ProductArgs {
     CUtensorMap a, a1, b, b1;
     int64_t M, N;
     int tiles_m, tiles_n;  // of one output
+    int cols;              // accumulator columns of a tile: 256, or 128 for a narrow output (EPI_STORE, EPI_SUM)
     int outputs;           // 2: a second product A1 B^T into o1
     int splits;            // the depth in this many parts, each with a partial sum of its own
     int kb, kb1;           // slices of (A, B), and after them of (A1, B1)
@@ -292,6 +293,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 
     // The launch has fewer than 2^31 items, so that all of this is 32-bit
     // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
+    // columns of a tile: half of its products would be with zeros at 128 or fewer
+    constexpr bool kNarrowTiles = EPI == EPI_STORE || EPI == EPI_SUM;
+    const int cols = kNarrowTiles ? p.cols : kCols;
     int tiles_m = p.tiles_m, kb = p.kb;
     int64_t M = p.M;
     if (p.plan) {
@@ -344,13 +348,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             for (unsigned i = first_item; ok && i < items; i += step) {
                 const Item t = item(i);
                 const int m = t.mt * kRows + 128 * (int)rank;
-                const int n = kDual ? t.nt * 128 : t.nt * kCols + 128 * (int)rank;
+                const int n = kDual ? t.nt * 128 : t.nt * cols + cols / 2 * (int)rank;
                 for (int k = t.k0; k < t.k1; k++) {
                     if (!mbar_wait(empty + 8 * s, ph ^ 1, s_abort, s_error, 1)) {
                         ok = false;
                         break;
                     }
-                    if (rank == 0) tc::mbar_arrive_tx(full + 8 * s, 4 * kOperand);
+                    if (rank == 0) tc::mbar_arrive_tx(full + 8 * s, 2 * kOperand + 256 * cols / 2);
                     const unsigned bar = ptx::of_first(full + 8 * s);
                     const bool second = k >= kb;
                     const int x = (second ? k - kb : k) * kDepth;
@@ -367,7 +371,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         ptx::tma_load(db, mb, x, n, bar);
                     } else {
                         ptx::tma_load(db, mb, n, x, bar);
-                        ptx::tma_load(db + kOperand / 2, mb, n + 64, x, bar);
+                        if (cols > 128) ptx::tma_load(db + kOperand / 2, mb, n + 64, x, bar);
                     }
                     loads++;
                     if (++s == kStages) s = 0, ph ^= 1;
@@ -387,7 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         if (rank == 0 && lane == 0) {
             // 32-bit sums of bf16 or fp16, 256 x 256 over the pair
             const unsigned idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) |
-                                   ((unsigned)AMAJ << 15) | ((unsigned)BMAJ << 16) | ((kCols >> 3) << 17) |
+                                   ((unsigned)AMAJ << 15) | ((unsigned)BMAJ << 16) | ((unsigned)(cols >> 3) << 17) |
                                    ((kRows >> 4) << 24);
             // 16 of k: 32 bytes along a row, or 16 rows of 128 bytes
             constexpr unsigned step_a = AMAJ == K_MAJOR ? 32 : 2048, step_b = BMAJ == K_MAJOR ? 32 : 2048;
@@ -497,16 +501,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     }
                 }
             } else if constexpr (EPI == EPI_STORE || EPI == EPI_SUM) {
-                const int64_t n0 = (int64_t)t.nt * kCols;
+                const int64_t n0 = (int64_t)t.nt * cols;
                 const float scale = EPI == EPI_STORE && e.plan ? ldexpf(1.0f, -e.plan->shift) : 1.0f;
                 const bool nothing = t.k0 == t.k1;  // a part of a depth that turned out short: no product ran
 #pragma unroll 1
-                for (int c = 0; c < 4; c++) {
-                    const int col = half * 128 + c * 32;
+                for (int c = 0; c < cols / 64; c++) {
+                    const int col = half * (cols / 2) + c * 32;
                     float v[32];
                     ptx::load32(acc + col, v);
                     ptx::wait32(v);
-                    if (c == 3) release();
+                    if (c == cols / 64 - 1) release();
                     if (n0 + col >= p.N) continue;
                     if (nothing) {
 #pragma unroll
@@ -526,7 +530,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             } else if constexpr (EPI == EPI_LSE) {
                 constexpr int kWide = kCols / 2;  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
-                const int64_t tg = target - n0;
+                // columns of the vocabulary here, and which of them is the row's target: looked at once a tile, since
+                // few tiles hold a target or the end
+                const int wide = (int)(p.N - n0 < kWide ? p.N - n0 : kWide);
+                const int tg = target >= n0 && target < n0 + wide ? (int)(target - n0) : -1;
+                const bool any = __any_sync(0xffffffffu, tg >= 0);
                 float top = -INFINITY, sum = 0.0f;
                 const float log2e = kLog2e * e.grow;
 #pragma unroll 1
@@ -535,20 +543,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::load32(acc + half * kWide + c * 32, v);
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
-                    const int left = (int)(p.N - n0 < kWide ? p.N - n0 : kWide) - c * 32;  // columns that exist
-                    if (left < 32) {
+                    if (wide < kWide) {
                         asm volatile("");  // a branch, not 32 selections in every tile
 #pragma unroll
                         for (int j = 0; j < 32; j++)
-                            if (j >= left) v[j] = -INFINITY;
+                            if (c * 32 + j >= wide) v[j] = -INFINITY;
                     }
-                    const int at = tg >= c * 32 && tg < c * 32 + 32 && tg < c * 32 + left ? (int)tg - c * 32 : -1;
-                    if (__any_sync(0xffffffffu, at >= 0)) {
+                    if (any) {
                         asm volatile("");
+                        const int at = tg - c * 32;
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        if (at >= 0) e.at[m] = x * e.grow;
+                        if (at >= 0 && at < 32) e.at[m] = x * e.grow;
                     }
                     float m0 = max3(top, v[0], v[1]), m1 = v[2];
 #pragma unroll
@@ -578,6 +585,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
+                const int col0 = (int)(e.col0 + n0);
+                const bool any = __any_sync(0xffffffffu, row.target >= col0 && row.target < col0 + kWide);
 #pragma unroll 1
                 for (int c = 0; c < kWide / 32; c++) {
                     float v[32];
@@ -586,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    loss_z<T>(v, w, row, (int)(e.col0 + n0) + c * 32, e.lse, e.src, m, e.grow);
+                    loss_z<T>(v, w, row, col0 + c * 32, any, e.lse, e.src, m, e.grow);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }
