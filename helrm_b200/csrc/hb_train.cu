@@ -276,11 +276,13 @@ static void launch(const Product &d, cudaStream_t s) {
 }
 
 // Parts of the depth for a product of few tiles: enough to give every SM pair
-// one, each at least 4 slices deep.
+// one, each at least 4 slices deep, and none below 16 slices, where joining
+// costs more than it saves (weight gradients of 512 x 512 x 512, 8 slices: 19.4
+// us in two parts, 16.3 in one; its dX, 16 slices: 18.0 in four, 18.5 in two).
 static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
     const int64_t tiles = (int64_t)blocks(M, kRows) * blocks(N, kCols) * outputs, slices = blocks(depth, kDepth);
     const int64_t n = 74 / tiles < slices / 4 ? 74 / tiles : slices / 4;
-    return n > 1 ? (int)n : 1;
+    return n > 1 && slices >= 16 ? (int)n : 1;
 }
 template <class T>
 static void join(const JoinArgs &j, void *out, cudaStream_t s) {
@@ -332,17 +334,33 @@ static void by_act(int act, F &&f) {
 }
 
 // Whether the loss's gradients come from the kernel that keeps Z in shared
-// memory, and its shape.
+// memory, and its shape.  It wins where every block has whole rounds of
+// vocabulary rows to itself and few tokens' dH to write out; the estimates (us)
+// are fitted to what both ways measured:
+//   tokens x inner x vocab    by pieces   Z in shared memory
+//   64 x 16 x 40000               38          22
+//   1024 x 16 x 19000             46          36
+//   1024 x 64 x 19000             46          57   (149 groups of rows for 148 blocks)
+//   8192 x 16 x 32001            352         208
+//   8192 x 64 x 19000            260         400
+//   8192 x 64 x 131072          1408         901
+//   32768 x 64 x 32001          1529        1640   (1.2 GB of partial sums)
 struct Narrow {
     bool on = false;
     int depth = 0, group = 0, grid = 0;
 };
 static Narrow narrow(int64_t tokens, int64_t inner, int64_t vocab) {
     Narrow n;
+    if (inner > kNarrow) return n;
     n.depth = (int)pad(inner, 16);
     n.group = 128 / n.depth;
-    n.grid = 148;
-    n.on = inner <= kNarrow && vocab >= 128 * 148 && tokens * n.depth <= (1 << 19);
+    const int64_t groups = blocks(vocab, 128);
+    n.grid = (int)(groups < 148 ? groups : 148);
+    const double t = (double)pad(tokens, 128), rows = 128.0 * (double)blocks(groups, 148) * 148;
+    const double sums = 4.0 * n.grid * t * n.depth;  // bytes of the blocks' dH
+    const double here = 12 + t * rows * (3.4e-7 + 8e-9 * n.depth) + 2 * sums / 5e6;
+    const double pieces = 20 + 1.35e-6 * t * (double)vocab;
+    n.on = here < pieces && sums <= 512e6;
     return n;
 }
 
@@ -357,10 +375,17 @@ static float logit_scale(int64_t inner) {
     return inner <= kNarrow ? 1.0f : (float)(1.0 + 1.52e-8 * (double)blocks(inner, 16));
 }
 
-// Columns of a vocabulary piece: Z of a piece takes at most 256 MiB.
+// Columns of a vocabulary piece: Z of a piece takes at most 512 MiB (256 MiB:
+// 907 us for 4096 x 128 x 131072 where 704 are reached with 1 GiB, 64 MiB:
+// 1140), in whole rounds of the SM pairs for dW where that many fit.
 static int64_t piece_columns(int64_t tokens, int64_t vocab) {
-    const int64_t most = ((int64_t)128 << 20) / (tokens > 0 ? tokens : 1);
-    const int64_t c = most < 2048 ? 2048 : most / 256 * 256;
+    const int64_t most = ((int64_t)256 << 20) / (tokens > 0 ? tokens : 1), round = 74 * kCols;
+    int64_t c = most / 256 * 256;
+    if (most >= round)
+        c = most / round * round;
+    else if (most >= round / 2)
+        c = round / 2;
+    if (c < 2048) c = 2048;
     return c < vocab ? c : vocab;
 }
 

@@ -364,9 +364,11 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
 
 // 32 logits of a row, the first of them column `col` of the vocabulary, to Z,
 // packed in 16 words.  The target's exp(..) - 1 is formed without cancellation.
-// any: whether some row of the warp may have its target here.
+// any: whether some row of the warp may have its target here; wide: how many of
+// the columns are in the vocabulary (past its end exp(0 - lse) may be infinite,
+// and zero times that is no zero in the products).
 template <class T>
-__device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col, bool any,
+__device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col, int wide, bool any,
                                        const float2 *lse, const int *src, int64_t m, float grow) {
     int at = -1;
     float hot = 0.0f;
@@ -390,6 +392,11 @@ __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const 
         asm volatile("");
 #pragma unroll
         for (int j = 0; j < 32; j++) v[j] = at == j ? hot : v[j];
+    }
+    if (wide < 32) {
+        asm volatile("");
+#pragma unroll
+        for (int j = 0; j < 32; j++) v[j] = j < wide ? v[j] : 0.0f;
     }
     const unsigned mask = r.target == kNoTarget ? 0u : 0xffffffffu, sign = r.g < 0.0f ? 0x80008000u : 0u;
 #pragma unroll

@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
                     }
-                    loss_z<T>(v, w, row, col + c * 32, any, p.lse, p.src, m, 1.0f);
+                    loss_z<T>(v, w, row, col + c * 32, (int)p.vocab - col - c * 32, any, p.lse, p.src, m, 1.0f);
                     // the products that read this buffer two tiles ago
                     if (!c && !(ok = wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1))) break;
 #pragma unroll

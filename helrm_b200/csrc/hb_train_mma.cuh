@@ -595,7 +595,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
                     if (n0 + c * 32 >= p.N) continue;
-                    loss_z<T>(v, w, row, col0 + c * 32, any, e.lse, e.src, m, e.grow);
+                    loss_z<T>(v, w, row, col0 + c * 32, 32, any, e.lse, e.src, m, e.grow);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, p.N, e.vec & 1, lane);
                 }
             }

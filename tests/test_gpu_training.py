@@ -430,6 +430,21 @@ def test_loss_target_out_of_range(tr):
     assert torch.isnan(dh).all(1).tolist() == [False, False, True, True, False, False]
 
 
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_loss_very_negative_logits(tr, dt):
+    """Every logit far below zero: what a tile computes past the vocabulary's end may overflow and has to stay out."""
+    dt = DTYPES[dt]
+    for v in (1, 5, 19001):
+        h = torch.full((3, 16), 4.0, device="cuda", dtype=dt)
+        w = torch.full((v, 16), -2.0, device="cuda", dtype=dt) + rand(v, 16, dtype=dt, std=0.01)
+        t = torch.tensor([0, v - 1, v // 2], device="cuda")
+        g = torch.ones(3, device="cuda")
+        loss, lse = tr.vocabulary_loss_forward(h, w, t)
+        within(loss, loss_values(h, w, t)[2], "loss")
+        for got, want, what in zip(tr.vocabulary_loss_backward(g, h, w, t, lse), loss_grads(g, h, w, t), ("dh", "dw")):
+            within(got, want, what)
+
+
 def test_loss_large_logits(tr):
     """Logits of thousands, and vocabulary rows at the type's lowest value."""
     h = torch.tensor([[100.0, 1.0], [-100.0, 1.0]], device="cuda", dtype=torch.bfloat16)
