@@ -20,7 +20,8 @@
  *     process, orion/backend/lattigo/scheme.go:32); all GPU work is
  *     enqueued on the library's own stream (the asynchronous batch
  *     transfers on two more, ordered with events) and synchronised only
- *     where a result crosses to the host.
+ *     where a result crosses to the host.  The training operators need no
+ *     scheme and run on the caller's stream, from any thread.
  * Levels follow Orion: a ciphertext at level l has l+1 residue limbs, a
  * fresh one sits at len(LogQ)-1 (orion/backend/python/parameters.py:258).
  * Rotation by k is a left shift, rot(ct,k)[i] = ct[i+k], shifts reduced to

@@ -697,3 +697,46 @@ def test_refusals_of_the_c_entries(tr):
         with pytest.raises(ValueError):
             _capi.check(-1)
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ long tensors
+def test_offsets_past_32_bits(tr):
+    """Results and inputs of more than 2^31 elements: their last rows are right."""
+    dt = torch.bfloat16
+    t, k, f = 140001, 16, 16384  # h: 2.3e9 elements
+    x, wg, wu = rand(t, k, dtype=dt), rand(f, k, dtype=dt, std=0.25, seed=1), rand(f, k, dtype=dt, std=0.25, seed=2)
+    h = tr.gated_forward(x, wg, wu)
+    assert h.numel() > 2 ** 31
+    rows = torch.tensor([0, 131071, 131072, 139999, 140000], device="cuda")
+    within(h[rows], gated(x[rows], wg, wu, "silu"), "h")
+    c = tr.pack_checkpoint(h)
+    back = tr.unpack_checkpoint(c)
+    assert torch.equal(back[rows], tr.unpack_checkpoint(tr.pack_checkpoint(h[rows])))
+    # dh as long: its gradients over the last rows alone
+    dx, _, _ = tr.gated_backward(h, x, wg, wu, needs=(True, False, False))
+    within(dx[rows], gated_grads(h[rows], x[rows], wg, wu, "silu")[0], "dx")
+    del h, c, back, dx
+    v, k, n = 1060000, 2048, 130  # w: 2.2e9 elements
+    w = torch.empty(v, k, dtype=dt, device="cuda")
+    for i in range(0, v, 106000):
+        w[i:i + 106000] = rand(106000, k, dtype=dt, std=k ** -0.5, seed=i)
+    assert w.numel() > 2 ** 31
+    x = rand(n, k, dtype=dt)
+    t = torch.full((n,), v - 1, device="cuda")
+    t[::2] = 0
+    loss, lse = tr.vocabulary_loss_forward(x, w, t)
+    ends = torch.stack([w[0], w[-1]])
+    at = (x.double() @ ends.double().T).gather(1, (t > 0).long()[:, None])[:, 0]
+    top = torch.full((n,), -math.inf, dtype=torch.float64, device="cuda")
+    for i in range(0, v, 106000):
+        top = torch.logaddexp(top, torch.logsumexp(x.double() @ w[i:i + 106000].double().T, 1))
+    assert ((loss.double() - (top - at)).abs() < 1e-4).all()
+    dh, dw = tr.vocabulary_loss_backward(torch.ones(n, device="cuda"), x, w, t, lse)
+    z = torch.exp(x.double() @ ends.double().T - top[:, None])
+    z[:, 0] -= (t == 0).double()
+    z[:, 1] -= (t > 0).double()
+    want = z.T @ x.double()
+    mag = z.abs().T @ x.double().abs()
+    # z to 2^-8 and 1e-4 of its exponential, 130 terms in 32 bits, the result to 2^-8
+    assert ((dw[[0, -1]].double() - want).abs() <= mag * (2.0 ** -8 + 1.5e-4) + 2.0 ** -8 * want.abs()).all()
+    assert torch.isfinite(dh).all()
