@@ -278,6 +278,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         *s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 0 && lane < 4) {
+        const CUtensorMap *map = lane == 0 ? &p.a : lane == 1 ? &p.b : lane == 2 ? &p.a1 : &p.b1;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+    }
     if (warp == 2) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(s_tmem)),
                      "r"(512)
@@ -291,9 +295,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     const unsigned tmem = *s_tmem;
     after_previous();
 
-    // The launch has fewer than 2^31 items, so that all of this is 32-bit
-    // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
-    // columns of a tile: half of its products would be with zeros at 128 or fewer
+    // half of a 256-column tile's products would be with zeros at 128 columns or fewer
     constexpr bool kNarrowTiles = EPI == EPI_STORE || EPI == EPI_SUM;
     const int cols = kNarrowTiles ? p.cols : kCols;
     int tiles_m = p.tiles_m, kb = p.kb;
@@ -305,6 +307,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         else
             tiles_m = n / kRows, M = n;
     }
+    // The launch has fewer than 2^31 items, so that all of this is 32-bit
+    // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
     const unsigned tiles = (unsigned)tiles_m * p.tiles_n;
     const unsigned items = tiles * p.splits * p.outputs;
     const int depth = kb + p.kb1;

@@ -489,6 +489,20 @@ def test_loss_pieces(tr):
     within(dw, V(wdw, mag * (2.0 ** -8 + 2.0 ** -17 + n * ACC)), "dw")
 
 
+def test_loss_forward_pieces(tr):
+    """So many rows over so large a vocabulary that the forward pass takes the rows in several pieces."""
+    n, k, v = 9000, 16, 2100003
+    h, w = rand(n, k, dtype=torch.bfloat16), rand(v, k, dtype=torch.bfloat16, std=0.25)
+    t = torch.randint(0, v, (n,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    loss, lse = tr.vocabulary_loss_forward(h, w, t)
+    rows = torch.tensor([0, 1, 4095, 4096, 4097, 8191, 8192, 8999], device="cuda")
+    _, wlse, wloss, _, _ = loss_values(h[rows], w, t[rows])
+    within(lse[rows].sum(1), wlse, "lse")
+    within(loss[rows], wloss, "loss")
+    one, _ = tr.vocabulary_loss_forward(h[:100], w, t[:100])
+    assert torch.equal(one, loss[:100])
+
+
 # ------------------------------------------------------------------ gradients against differences
 def test_gated_differences(tr):
     """h is quadratic in x for the identity gate, so the central difference
