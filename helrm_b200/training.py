@@ -102,8 +102,7 @@ def _entry(name: str):
     return fn
 
 
-def _stream(index: int) -> int:
-    return torch._C._cuda_getCurrentRawStream(index)
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # absent where torch has no CUDA
 
 
 class _Plan:
@@ -139,10 +138,9 @@ def _remember(key, plan):
     return plan
 
 
-def _run(name: str, like, needs, odd, *args):
+def _run(fn, like, needs, odd, *args):
     """One entry point that takes a workspace, on the current stream of
     like's device.  needs: the bytes it takes, by odd."""
-    fn = _entry(name)
     need = needs.get(odd)
     if need is None:
         n = ctypes.c_size_t(0)
@@ -183,10 +181,11 @@ def gated_forward(x, w_gate, w_up, activation: str = "silu"):
         if xm.data_ptr() == x.data_ptr() and wg is w_gate and wu is w_up:
             _remember(key, plan)
         x, w_gate, w_up = xm, wg, wu  # the copies, where the strides asked for some
-    h = plan.out.new()
+    o = plan.out
+    h = torch.empty_strided(o.shape, o.strides, dtype=o.dtype, device=o.device)
     px, pg, pu = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
     lx, lg, lu = plan.pitches
-    _run("helrm_GatedForward", x, plan.needs, (px & 15, pg & 15, pu & 15), *plan.head, px, lx, pg, lg, pu, lu,
+    _run(_entry("helrm_GatedForward"), x, plan.needs, (px & 15, pg & 15, pu & 15), *plan.head, px, lx, pg, lg, pu, lu,
          h.data_ptr())
     return h
 
@@ -238,7 +237,7 @@ def gated_backward(dh, x, w_gate, w_up, activation: str = "silu", needs=(True, T
         ld, lx, lg, lu = plan.pitches
         pd, pg, pu = dh.data_ptr(), w_gate.data_ptr(), w_up.data_ptr()
         px, pq, pe = (None, x.q.data_ptr(), x.e.data_ptr()) if kept else (x.data_ptr(), None, None)
-        _run("helrm_GatedBackward", dh, plan.needs, ((px or 0) & 15, pg & 15, pu & 15), *plan.head, pd, ld, px, lx, pq,
+        _run(_entry("helrm_GatedBackward"), dh, plan.needs, ((px or 0) & 15, pg & 15, pu & 15), *plan.head, pd, ld, px, lx, pq,
              pe, pg, lg, pu, lu, None if dx is None else dx.data_ptr(), None if dwg is None else dwg.data_ptr(),
              None if dwu is None else dwu.data_ptr())
     return dx, dwg, dwu
@@ -395,7 +394,7 @@ def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
     h, w, t, plan = _loss_call(h, w, targets)
     loss, lse = plan.out[0].new(), plan.out[1].new()
     ph, pw = h.data_ptr(), w.data_ptr()
-    _run("helrm_VocabularyLossForward", h, plan.needs, (ph & 15, pw & 15), *plan.head, ph, plan.pitches[0], pw,
+    _run(_entry("helrm_VocabularyLossForward"), h, plan.needs, (ph & 15, pw & 15), *plan.head, ph, plan.pitches[0], pw,
          plan.pitches[1], t.data_ptr(), int(ignore_index), loss.data_ptr(), lse.data_ptr())
     return loss, lse
 
@@ -410,7 +409,7 @@ def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100
     dw = out_w.new() if needs[1] else None
     if any(needs):
         ph, pw = h.data_ptr(), w.data_ptr()
-        _run("helrm_VocabularyLossBackward", h, plan.needs, (ph & 15, pw & 15, bool(needs[0]), bool(needs[1])),
+        _run(_entry("helrm_VocabularyLossBackward"), h, plan.needs, (ph & 15, pw & 15, bool(needs[0]), bool(needs[1])),
              *plan.head, g.data_ptr(), ph, plan.pitches[0], pw, plan.pitches[1], t.data_ptr(), l.data_ptr(),
              int(ignore_index), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr())
     return dh, dw
