@@ -1,4 +1,5 @@
 """A gated model trained in the clear and answered on ciphertexts."""
+import gc
 import math
 
 import numpy as np
@@ -6,9 +7,18 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_memory_back():
+    """The tests after these find torch's allocator as if these had not run."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
+
 
 def test_trained_model_runs_encrypted():
-    pytest.importorskip("torch")
     from helrm_b200 import pretrain
     r = pretrain.main(["--steps", "120", "--rows", "2048", "--vocab", "500", "--width", "48", "--queries", "3"])
     losses = r["losses"]

@@ -8,6 +8,7 @@ bfloat16, 2^-11 for half precision, whose subnormals add 2^-25), and a
 function adds its slope times the bound plus 2^-20 of its value for its own
 evaluation.  Every element has to lie within its own bound.
 """
+import gc
 import math
 
 import pytest
@@ -15,6 +16,15 @@ import pytest
 pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module", autouse=True)
+def give_memory_back():
+    """The tests after these find torch's allocator as if these had not run."""
+    yield
+    gc.collect()
+    torch.cuda.empty_cache()
+
 
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 ACC = 2.0 ** -23
