@@ -1,8 +1,10 @@
 // hb_train.cu -- the training operators' launches and their extern "C"
 // entry points (include/helrm_b200.h).
 #include <atomic>
+#include <cmath>
 #include <mutex>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "hb_error.hpp"
@@ -236,57 +238,115 @@ static CUtensorMap tensor_map(const Matrix &m, bool bf16, int major) {
     return map;
 }
 
-// One product launch.  a, b (and a1, b1 where used) lie K-major or MN-major:
-// a K-major operand has the product's depth in its columns, an MN-major one in
-// its rows.
+// One product.  a, b (and a1, b1 where used) lie K-major or MN-major: a K-major
+// operand has the product's depth in its columns, an MN-major one in its rows.
 struct Product {
     Matrix a, b, a1, b1;
     int64_t M = 0, N = 0, K = 0, K1 = 0;
-    int outputs = 1, splits = 1;
+    int amaj = K_MAJOR, outputs = 1, splits = 1;
     const LossPlan *plan = nullptr;
     bool plan_k = false;
     EpiArgs e;
-    int tile_cols() const { return N <= 128 ? 128 : kCols; }
+    void *out[2] = {};    // gradients: dense 16-bit rows; with none, acc is the result
+    float *acc = nullptr;  // of a split depth
+    int cols() const { return N <= 128 ? 128 : kCols; }
+    int64_t tiles() const { return (int64_t)blocks(M, kRows) * blocks(N, cols()) * outputs; }
+    int64_t slices() const { return (int64_t)blocks(K, kDepth) + blocks(K1, kDepth); }
+    int64_t sums() const { return splits > 1 ? (int64_t)outputs * splits * M * pad(N, 4) : 0; }
 };
-template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
-static void launch(const Product &d, cudaStream_t s) {
-    constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-    constexpr bool dual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
-    ProductArgs p;
-    p.a = tensor_map(d.a, bf16, AMAJ);
-    p.b = tensor_map(d.b, bf16, BMAJ);
-    p.a1 = d.a1.p ? tensor_map(d.a1, bf16, AMAJ) : p.a;
-    p.b1 = d.b1.p ? tensor_map(d.b1, bf16, BMAJ) : p.b;
-    p.M = d.M;
-    p.N = d.N;
-    p.tiles_m = (int)blocks(d.M, kRows);
-    p.cols = d.tile_cols();
-    static_assert(BMAJ == MN_MAJOR || (EPI != EPI_STORE && EPI != EPI_SUM), "a K-major B comes in 256-column tiles");
-    p.tiles_n = (int)blocks(d.N, dual ? 128 : EPI == EPI_STORE || EPI == EPI_SUM ? p.cols : kCols);
-    p.outputs = d.outputs;
-    p.splits = d.splits;
-    p.kb = (int)blocks(d.K, kDepth);
-    p.kb1 = (int)blocks(d.K1, kDepth);
-    p.plan = d.plan;
-    p.plan_k = d.plan_k;
-    p.e = d.e;
-    p.error = runtime().error;
-    auto kernel = k_mma_product<T, AMAJ, BMAJ, EPI, ACT>;
-    raise_shared_memory<k_mma_product<T, AMAJ, BMAJ, EPI, ACT>>(kProductSmem);
-    const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits * p.outputs, pairs = sm_count() / 2;
+static void fill(Job &j, const Product &d, bool bf16, int amaj, int bmaj, int cols_n) {
+    j.a = tensor_map(d.a, bf16, amaj);
+    j.b = tensor_map(d.b, bf16, bmaj);
+    j.a1 = d.a1.p ? tensor_map(d.a1, bf16, amaj) : j.a;
+    j.b1 = d.b1.p ? tensor_map(d.b1, bf16, bmaj) : j.b;
+    j.M = d.M;
+    j.N = d.N;
+    j.tiles_m = (int)blocks(d.M, kRows);
+    j.tiles_n = (int)blocks(d.N, cols_n);
+    j.cols = d.cols();
+    j.outputs = d.outputs;
+    j.splits = d.splits;
+    j.kb = (int)blocks(d.K, kDepth);
+    j.kb1 = (int)blocks(d.K1, kDepth);
+    j.amaj = amaj;
+    j.plan = d.plan;
+    j.plan_k = d.plan_k;
+    j.e = d.e;
+}
+static unsigned product_grid(int64_t items) {
     require(items < (int64_t)1 << 31, "more than 2^31 tiles in one product");
-    start("training product", kernel, dim3((unsigned)(2 * (items < pairs ? items : pairs))), product_threads(EPI),
-          kProductSmem, s, p);
+    const int64_t pairs = sm_count() / 2;
+    return (unsigned)(2 * (items < pairs ? items : pairs));
+}
+// The products with both operands K-major.
+template <class T, int EPI, int ACT>
+static void launch(const Product &d, cudaStream_t s) {
+    constexpr int cols_n = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? 128 : kCols;
+    ProductArgs<1> p;
+    fill(p.job[0], d, std::is_same<T, __nv_bfloat16>::value, K_MAJOR, K_MAJOR, cols_n);
+    p.error = runtime().error;
+    raise_shared_memory<k_mma_product<T, K_MAJOR, K_MAJOR, EPI, ACT, 1>>(kProductSmem);
+    start("training product", k_mma_product<T, K_MAJOR, K_MAJOR, EPI, ACT, 1>,
+          product_grid((int64_t)p.job[0].tiles_m * p.job[0].tiles_n), product_threads(EPI), kProductSmem, s, p);
 }
 
-// Parts of the depth for a product of few tiles: enough to give every SM pair
-// one, each at least 4 slices deep, and none below 16 slices, where joining
-// costs more than it saves (weight gradients of 512 x 512 x 512, 8 slices: 19.4
-// us in two parts, 16.3 in one; its dX, 16 slices: 18.0 in four, 18.5 in two).
-static int parts_for(int64_t M, int64_t N, int64_t depth, int outputs) {
-    const int64_t tiles = (int64_t)blocks(M, kRows) * blocks(N, kCols) * outputs, slices = blocks(depth, kDepth);
-    const int64_t n = 74 / tiles < slices / 4 ? 74 / tiles : slices / 4;
-    return n > 1 && slices >= 16 ? (int)n : 1;
+// Parts of the depth of each of a launch's products (two, or one): none whose
+// items are no longer than what every SM pair has to do on average, else as
+// many as bring them there, each at least 4 slices deep, and none below 16
+// slices, where joining costs more than it saves (weight gradients of 512 x 512
+// x 512, 8 slices: 19.4 us in two parts, 16.3 in one; its dX, 16 slices: 18.0
+// in four, 18.5 in two).
+static void split_depths(Product *d, int n) {
+    double work = 0;
+    for (int i = 0; i < n; i++) work += (double)d[i].tiles() * (double)d[i].slices();
+    for (int i = 0; i < n; i++) {
+        const int64_t slices = d[i].slices(), most = 74 / d[i].tiles() < slices / 4 ? 74 / d[i].tiles() : slices / 4;
+        int64_t parts = (int64_t)((double)slices * 74 / work + 0.3);
+        if (parts > most) parts = most;
+        d[i].splits = parts > 1 && slices >= 16 ? (int)parts : 1;
+    }
+}
+// Splits the two products' depths, for one launch of both or a launch each:
+// true for one.  Rounds are counted in slices, a tile's epilogue as two, a
+// launch of its own and a joining as eight each, and the kernel for two as 7 %
+// slower.  Measured, together and apart (us): gated gradients of 64 x 432 x 512
+// 18 and 24, 1024 x 1024 x 1024 28 and 41, 2047 x 1001 x 1500 58 and 61, 4096 x
+// 2048 x 2048 155 and 146; the loss's of 2048 x 256 x 20000 80 and 96, 777 x 432
+// x 32001 92 and 99, 4096 x 1024 x 32001 602 and 581.  Where what both read
+// outgrows L2 (the last), two orders of reading it at once lose what the rounds
+// gain.
+static bool together(Product *d) {
+    auto length = [](const Product &g) { return (double)(g.slices() / g.splits + 2); };
+    auto items = [](const Product &g) { return (double)(g.tiles() * g.splits); };
+    Product apart[2] = {d[0], d[1]};
+    double separate = 8;
+    for (Product &g : apart) {
+        split_depths(&g, 1);
+        separate += std::ceil(items(g) / 74) * length(g) + (g.splits > 1 ? 8 : 0);
+    }
+    split_depths(d, 2);
+    const int first = length(d[1]) > length(d[0]);
+    const Product &a = d[first], &b = d[1 - first];
+    const double full = std::floor(items(a) / 74), rest = items(a) - 74 * full, start = full * length(a);
+    double joint = d[0].splits > 1 || d[1].splits > 1 ? 8 : 0;
+    if (rest == 0) {
+        joint += start + std::ceil(items(b) / 74) * length(b);
+    } else {
+        const double beside = std::ceil(length(a) / length(b)) * (74 - rest);
+        if (items(b) <= beside) {
+            const double tail = std::ceil(items(b) / (74 - rest)) * length(b);
+            joint += start + (tail > length(a) ? tail : length(a));
+        } else {
+            joint += start + length(a) + std::ceil((items(b) - beside) / 74) * length(b);
+        }
+    }
+    // both read the same A (dG and dU, or Z)
+    double bytes = 2.0 * (double)d[0].M * (double)(d[0].K + d[0].K1);
+    for (int i = 0; i < 2; i++) bytes += 2.0 * (double)d[i].N * (double)(d[i].K + d[i].K1);
+    if (joint * 1.07 < separate && bytes <= 160e6) return true;
+    d[0].splits = apart[0].splits;
+    d[1].splits = apart[1].splits;
+    return false;
 }
 template <class T>
 static void join(const JoinArgs &j, void *out, cudaStream_t s) {
@@ -296,27 +356,50 @@ static void join(const JoinArgs &j, void *out, cudaStream_t s) {
     else
         start("join parts", k_join<T, false>, blocks(j.M * (j.ld / 4), 256), 256, 0, s, j, o);
 }
-// D = A B^T (+ A1 B1^T), or with outputs = 2 also A1 B^T, as dense 16-bit rows
-// at out[0], out[1]; the sums of a split depth are joined in acc.
-template <class T, int AMAJ, int BMAJ>
-static void product_out(Product d, void *const *out, float *acc, cudaStream_t s) {
-    if (d.splits == 1) {
-        d.e.o0 = out[0];
-        d.e.o1 = d.outputs > 1 ? out[1] : nullptr;
-        d.e.ldo = d.N;
-        d.e.vec = fits_vectors(out[0], d.N) && (d.outputs == 1 || fits_vectors(out[1], d.N));
-        launch<T, AMAJ, BMAJ, EPI_STORE, 0>(d, s);
-        return;
+// The gradients' products, B MN-major, two of them in one launch (4096 x 1024 x
+// 4096: dX of 64 tiles and the weights' of 128 leave 10 of the 74 SM pairs idle
+// in one round and 20 in the other on their own).  D = A B^T (+ A1 B1^T), or with
+// outputs = 2 also A1 B^T; the sums of a split depth are joined in acc.
+template <class T, int AMAJ, int JOBS>
+static void launch_gradients(Product *d, cudaStream_t s) {
+    ProductArgs<JOBS> p;
+    int64_t items = 0;
+    for (int i = 0; i < JOBS; i++) {
+        Product &g = d[i];
+        if (g.out[0] && g.splits == 1) {
+            g.e.o0 = g.out[0];
+            g.e.o1 = g.out[1];
+            g.e.ldo = g.N;
+            g.e.vec = fits_vectors(g.out[0], g.N) && (g.outputs == 1 || fits_vectors(g.out[1], g.N));
+        } else {
+            g.e.acc = g.acc;
+            g.e.ldo = pad(g.N, 4);
+        }
+        fill(p.job[i], g, std::is_same<T, __nv_bfloat16>::value, g.amaj, MN_MAJOR, g.cols());
+        items += g.tiles() * g.splits;
     }
-    d.e.acc = acc;
-    d.e.ldo = pad(d.N, 4);
-    launch<T, AMAJ, BMAJ, EPI_SUM, 0>(d, s);
-    for (int i = 0; i < d.outputs; i++)
-        join<T>({acc + (int64_t)i * d.splits * d.M * d.e.ldo, d.splits, d.M, d.M, d.N, d.e.ldo, d.e.plan, nullptr},
-                out[i], s);
+    p.error = runtime().error;
+    raise_shared_memory<k_mma_product<T, AMAJ, MN_MAJOR, EPI_OUT, 0, JOBS>>(kProductSmem);
+    start("training product", k_mma_product<T, AMAJ, MN_MAJOR, EPI_OUT, 0, JOBS>, product_grid(items),
+          product_threads(EPI_OUT), kProductSmem, s, p);
 }
-static int64_t sums(int64_t M, int64_t N, int splits, int outputs) {
-    return splits > 1 ? (int64_t)outputs * splits * M * pad(N, 4) : 0;
+template <class T>
+static void gradients(Product *d, int n, cudaStream_t s) {
+    if (n == 2) {
+        // the longer items first
+        if (d[1].slices() / d[1].splits > d[0].slices() / d[0].splits) std::swap(d[0], d[1]);
+        launch_gradients<T, K_MAJOR, 2>(d, s);
+    } else if (n == 1 && d[0].amaj == K_MAJOR) {
+        launch_gradients<T, K_MAJOR, 1>(d, s);
+    } else if (n == 1) {
+        launch_gradients<T, MN_MAJOR, 1>(d, s);
+    }
+    for (int i = 0; i < n; i++) {
+        const Product &g = d[i];
+        for (int k = 0; g.out[0] && g.splits > 1 && k < g.outputs; k++)
+            join<T>({g.acc + (int64_t)k * g.splits * g.M * g.e.ldo, g.splits, g.M, g.M, g.N, g.e.ldo, g.e.plan, nullptr},
+                    g.out[k], s);
+    }
 }
 
 template <class F>
@@ -424,7 +507,7 @@ HB_API int helrm_GatedForward(int device, int dtype, int act, int64_t tokens, in
         d.e.ldo = width;
         d.e.vec = fits_vectors(h, width);
         by_dtype(dtype, [&](auto t) {
-            by_act(act, [&](auto a) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_GATED, decltype(a)::value>(d, s); });
+            by_act(act, [&](auto a) { launch<decltype(t), EPI_GATED, decltype(a)::value>(d, s); });
         });
     });
 }
@@ -453,11 +536,25 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
         const Matrix mx = x ? in.fit({x, tokens, inner, ldx}) : Matrix{read, tokens, inner, pitch(inner)};
         const Matrix mg = in.fit({wg, width, inner, ldg}), mu = in.fit({wu, width, inner, ldu});
         const Matrix mdg{dg, tokens, width, ldd}, mdu{du, tokens, width, ldd};
-        const int both = dwg && dwu ? 2 : 1;
-        const int parts_x = dx ? parts_for(tokens, inner, 2 * width, 1) : 1;
-        const int parts_w = dwg || dwu ? parts_for(width, inner, tokens, both) : 1;
-        const int64_t sums_x = sums(tokens, inner, parts_x, 1), sums_w = sums(width, inner, parts_w, both);
-        float *acc = w.take<float>(sums_x > sums_w ? sums_x : sums_w);
+        // the depths are split as if all were wanted: an output has the same bits with or without the others
+        Product all[2], grads[2];
+        Product &gx = all[0], &gw = all[1];
+        gx.a = mdg, gx.b = mg, gx.a1 = mdu, gx.b1 = mu;
+        gx.M = tokens, gx.N = inner, gx.K = gx.K1 = width;
+        gx.out[0] = dx;
+        gw.a = dwg ? mdg : mdu, gw.a1 = mdu, gw.b = mx;
+        gw.amaj = MN_MAJOR;
+        gw.M = width, gw.N = inner, gw.K = tokens;
+        gw.outputs = 2;
+        gw.out[0] = dwg ? dwg : dwu, gw.out[1] = dwu;
+        const bool one = tokens && together(all);
+        gw.outputs = dwg && dwu ? 2 : 1;
+        int n = 0;
+        for (Product &g : all) {
+            if (!g.out[0]) continue;
+            g.acc = w.take<float>(g.sums());
+            grads[n++] = g;
+        }
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
@@ -479,22 +576,11 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
             d.e.dh = dh;
             d.e.lddh = lddh;
             d.e.vec = 1 | (fits_vectors(dh, lddh) ? 2 : 0);
-            by_act(act, [&](auto a) { launch<T, K_MAJOR, K_MAJOR, EPI_GATED_BWD, decltype(a)::value>(d, s); });
-            if (dx) {
-                Product g;
-                g.a = mdg, g.b = mg, g.a1 = mdu, g.b1 = mu;
-                g.M = tokens, g.N = inner, g.K = g.K1 = width;
-                g.splits = parts_x;
-                product_out<T, K_MAJOR, MN_MAJOR>(g, &dx, acc, s);
-            }
-            if (dwg || dwu) {
-                Product g;
-                g.a = dwg ? mdg : mdu, g.a1 = mdu, g.b = mx;
-                g.M = width, g.N = inner, g.K = tokens;
-                g.outputs = both;
-                g.splits = parts_w;
-                void *out[2] = {dwg ? dwg : dwu, dwu};
-                product_out<T, MN_MAJOR, MN_MAJOR>(g, out, acc, s);
+            by_act(act, [&](auto a) { launch<T, EPI_GATED_BWD, decltype(a)::value>(d, s); });
+            if (one) {
+                gradients<T>(grads, n, s);
+            } else {
+                for (int i = 0; i < n; i++) gradients<T>(grads + i, 1, s);
             }
         });
     });
@@ -570,7 +656,7 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
             d.e.at = at;
             d.e.target = targets + m0;
             d.e.grow = logit_scale(inner);
-            by_dtype(dtype, [&](auto t) { launch<decltype(t), K_MAJOR, K_MAJOR, EPI_LSE, 0>(d, s); });
+            by_dtype(dtype, [&](auto t) { launch<decltype(t), EPI_LSE, 0>(d, s); });
             const float *none = nullptr;
             const int64_t *no_targets = nullptr;
             if (joined)
@@ -649,10 +735,19 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         }
         const int64_t cols = piece_columns(cap, vocab), ldz = pitch(cols), lda = pad(inner, 4);
         uint16_t *z = w.take<uint16_t>(cap * ldz);
-        // dh is a 32-bit sum over the pieces, for each part of a piece's depth, of the rows that take part
-        const int parts_h = dh ? parts_for(cap, inner, cols, 1) : 1, parts_w = dw ? parts_for(cols, inner, cap, 1) : 1;
-        float *acc = w.take<float>(dh ? parts_h * cap * lda : 0);
-        float *acc_w = w.take<float>(sums(cols, inner, parts_w, 1));
+        // the products of the first, largest piece: dh is a 32-bit sum over the pieces, for each part of a piece's
+        // depth, of the rows that take part
+        Product all[2];
+        Product &gh = all[0], &gw = all[1];
+        gh.a = {z, cap, cols, ldz};
+        gh.M = cap, gh.N = inner, gh.K = cols;
+        gw.b = mh;
+        gw.amaj = MN_MAJOR;
+        gw.M = cols, gw.N = inner, gw.K = cap;
+        gw.plan_k = true;
+        const bool one = tokens && together(all);
+        float *acc = w.take<float>(dh ? gh.splits * cap * lda : 0);
+        float *acc_w = w.take<float>(dw ? gw.sums() : 0);
         if (sized(w, ws_bytes)) return;
         DeviceGuard dev(device);
         cudaStream_t s = (cudaStream_t)stream;
@@ -678,32 +773,36 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 d.e.lse = reinterpret_cast<const float2 *>(lse);
                 d.e.col0 = c0;
                 d.e.grow = logit_scale(inner);
-                launch<T, K_MAJOR, K_MAJOR, EPI_Z, 0>(d, s);
-                if (dw) {
-                    Product g;
-                    g.a = mz, g.b = mh;
-                    g.M = n, g.N = inner, g.K = cap;
-                    g.splits = parts_w;
-                    g.plan = plan;
-                    g.plan_k = true;
-                    g.e.plan = plan;
-                    void *out = static_cast<T *>(dw) + c0 * inner;
-                    product_out<T, MN_MAJOR, MN_MAJOR>(g, &out, acc_w, s);
-                }
+                launch<T, EPI_Z, 0>(d, s);
+                Product piece[2];
+                int np = 0;
                 if (dh) {
-                    Product g;
+                    Product &g = piece[np++] = gh;
                     g.a = mz, g.b = mc;
-                    g.M = cap, g.N = inner, g.K = n;
                     g.plan = plan;
+                    g.K = n;
                     // the last piece may be too short for every part: those keep their sums
-                    g.splits = parts_h < (int)blocks(n, kDepth) ? parts_h : (int)blocks(n, kDepth);
-                    g.e.acc = acc;
-                    g.e.ldo = lda;
+                    g.splits = gh.splits < (int)blocks(n, kDepth) ? gh.splits : (int)blocks(n, kDepth);
+                    g.acc = acc;
                     g.e.first = c0 == 0;
-                    launch<T, K_MAJOR, MN_MAJOR, EPI_SUM, 0>(g, s);
+                }
+                if (dw) {
+                    Product &g = piece[np++] = gw;
+                    g.a = mz;
+                    g.plan = plan;
+                    g.M = n;
+                    g.e.plan = plan;
+                    g.out[0] = static_cast<T *>(dw) + c0 * inner;
+                    g.acc = acc_w;
+                }
+                if (one) {
+                    gradients<T>(piece, np, s);
+                } else {
+                    // dW first: Z's last columns, just written, are its last rows
+                    for (int i = np - 1; i >= 0; i--) gradients<T>(piece + i, 1, s);
                 }
             }
-            if (dh) join<T>({acc, parts_h, cap, tokens, inner, lda, plan, pos}, dh, s);
+            if (dh) join<T>({acc, gh.splits, cap, tokens, inner, lda, plan, pos}, dh, s);
         });
     });
 }

@@ -149,14 +149,14 @@ __device__ __forceinline__ void act_df(float g, float &a, float &d) {
 }
 
 // ---------------------------------------------------------------- products
-enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_STORE, EPI_SUM, EPI_LSE, EPI_Z };
+enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_OUT, EPI_LSE, EPI_Z };
 struct EpiArgs {
     void *o0 = nullptr, *o1 = nullptr;  // 16-bit outputs
     int64_t ldo = 0;                    // their row pitch, or that of acc
     int vec = 0;                        // 1: outputs fit 16-byte stores, 2: dh fits 16-byte loads
     const void *dh = nullptr;
     int64_t lddh = 0;
-    float *acc = nullptr;               // EPI_SUM: 32-bit sums, [output][part][row][ldo]
+    float *acc = nullptr;               // EPI_OUT: 32-bit sums instead, [output][part][row][ldo]
     int first = 1;                      // 0: added to what acc holds
     float2 *part = nullptr;             // EPI_LSE: (max, sum) of each warp's columns, [part][row]
     float *at = nullptr;                // EPI_LSE: the target's logit

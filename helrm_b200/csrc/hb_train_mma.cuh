@@ -47,17 +47,26 @@ constexpr unsigned long long kWaitNs = 4000000000ull;
 
 enum { K_MAJOR = 0, MN_MAJOR = 1 };
 
-struct ProductArgs {
+// One product.  A launch of gradients (EPI_OUT) may hold two, which the clusters
+// share: those by the input and by the weights have nothing to do with each
+// other, and fill the SM pairs' rounds together.  A kernel of its own for that
+// (JOBS): what is fixed at compile time for one product costs a long one 7 %.
+struct Job {
     CUtensorMap a, a1, b, b1;
     int64_t M, N;
     int tiles_m, tiles_n;  // of one output
-    int cols;              // accumulator columns of a tile: 256, or 128 for a narrow output (EPI_STORE, EPI_SUM)
+    int cols;              // accumulator columns of a tile: 256, or 128 for a narrow output (EPI_OUT)
     int outputs;           // 2: a second product A1 B^T into o1
     int splits;            // the depth in this many parts, each with a partial sum of its own
     int kb, kb1;           // slices of (A, B), and after them of (A1, B1)
+    int amaj;              // two jobs: how A lies (B is MN-major)
     const LossPlan *plan;  // not NULL: the rows that take part, known on the device only, are
     int plan_k;            // 0: the rows of the tiles, 1: the depth
     EpiArgs e;
+};
+template <int JOBS>
+struct ProductArgs {
+    Job job[JOBS];
     int *error;            // host memory
 };
 
@@ -247,9 +256,9 @@ __device__ __forceinline__ void store_sums(unsigned char *st, const float (&v)[3
     __syncwarp();
 }
 
-template <class T, int AMAJ, int BMAJ, int EPI, int ACT>
+template <class T, int AMAJ, int BMAJ, int EPI, int ACT, int JOBS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI), 1)
-    k_mma_product(const __grid_constant__ ProductArgs p) {
+    k_mma_product(const __grid_constant__ ProductArgs<JOBS> p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
     constexpr int kWarps = epi_warps(EPI), kSets = kWarps / 8;
     extern __shared__ __align__(1024) unsigned char smem[];
@@ -279,7 +288,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 0 && lane < 4) {
-        const CUtensorMap *map = lane == 0 ? &p.a : lane == 1 ? &p.b : lane == 2 ? &p.a1 : &p.b1;
+        const Job &j = p.job[0];
+        const CUtensorMap *map = lane == 0 ? &j.a : lane == 1 ? &j.b : lane == 2 ? &j.a1 : &j.b1;
         asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     }
     if (warp == 2) {
@@ -295,49 +305,87 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     const unsigned tmem = *s_tmem;
     after_previous();
 
-    // half of a 256-column tile's products would be with zeros at 128 columns or fewer
-    constexpr bool kNarrowTiles = EPI == EPI_STORE || EPI == EPI_SUM;
-    const int cols = kNarrowTiles ? p.cols : kCols;
-    int tiles_m = p.tiles_m, kb = p.kb;
-    int64_t M = p.M;
-    if (p.plan) {
-        const int n = p.plan->filled;
-        if (p.plan_k)
-            kb = n / kDepth;
-        else
-            tiles_m = n / kRows, M = n;
-    }
-    // The launch has fewer than 2^31 items, so that all of this is 32-bit
-    // arithmetic: 64-bit divisions cost an epilogue warp more than 32 columns.
-    const unsigned tiles = (unsigned)tiles_m * p.tiles_n;
-    const unsigned items = tiles * p.splits * p.outputs;
-    const int depth = kb + p.kb1;
-    const unsigned first_item = blockIdx.x >> 1, step = gridDim.x >> 1;
+    constexpr bool kOut = EPI == EPI_OUT, kTwo = JOBS == 2;
+    // A job's shape, with the rows that take part.  The launch has fewer than
+    // 2^31 items, so that all of this is 32-bit arithmetic: 64-bit divisions
+    // cost an epilogue warp more than 32 columns.
+    struct Shape {
+        unsigned tiles_m, tiles, items;
+        int kb, depth;
+        int64_t M;
+    };
+    auto shape = [&](const Job &j) {
+        Shape h;
+        h.tiles_m = j.tiles_m, h.kb = j.kb, h.M = j.M;
+        if (j.plan) {
+            const int n = j.plan->filled;
+            if (j.plan_k)
+                h.kb = n / kDepth;
+            else
+                h.tiles_m = n / kRows, h.M = n;
+        }
+        h.tiles = h.tiles_m * j.tiles_n;
+        h.items = h.tiles * j.splits * j.outputs;
+        h.depth = h.kb + j.kb1;
+        return h;
+    };
+    const Shape s0 = shape(p.job[0]);
+    Shape s1 = {};
+    if (kTwo) s1 = shape(p.job[JOBS - 1]);
+    const unsigned cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+    constexpr unsigned kNoItem = 0xffffffffu;
+    // The k-th item of this cluster, the second job's numbered after the first's.
+    // The first job's items are the longer ones and go round first; clusters that
+    // its last round leaves out take the second job's until that round ends.
+    auto nth = [&](unsigned k) -> unsigned {
+        if (!kTwo) {
+            const unsigned i = cluster + k * clusters;
+            return i < s0.items ? i : kNoItem;
+        }
+        const unsigned rounds = s0.items / clusters, rest = s0.items - rounds * clusters;
+        const unsigned own = rounds + (cluster < rest);
+        if (k < own) return k * clusters + cluster;
+        k -= own;
+        unsigned ahead = 0, beside = 0;
+        if (rest) {
+            const unsigned c0 = s0.depth / p.job[0].splits + 2, c1 = s1.depth / p.job[JOBS - 1].splits + 2;
+            beside = (c0 + c1 - 1) / c1;
+            ahead = beside * (clusters - rest);
+        }
+        const unsigned i = rest && cluster >= rest && k < beside
+                               ? k * (clusters - rest) + cluster - rest
+                               : ahead + (k - (rest && cluster >= rest ? beside : 0)) * clusters + cluster;
+        return i < s1.items ? s0.items + i : kNoItem;
+    };
     struct Item {
-        int out, split, mt, nt, k0, k1;
+        int job, out, split, mt, nt, k0, k1;
     };
     // Tiles go down groups of 8 tile rows, column after column, so that the
     // clusters at work share a few panels of A and of B in L2.
     auto item = [&](unsigned i) {
         Item t;
+        t.job = kTwo && i >= s0.items;
+        if (t.job) i -= s0.items;
+        const Shape &h = kTwo && t.job ? s1 : s0;
+        const Job &j = p.job[kTwo ? t.job : 0];
         t.out = t.split = t.k0 = 0;
-        t.k1 = depth;
-        if (items > tiles) {
-            unsigned q = i / tiles;
-            i -= q * tiles;
-            t.out = q / p.splits;
-            t.split = q - t.out * p.splits;
-            t.k0 = (int)((int64_t)depth * t.split / p.splits);
-            t.k1 = (int)((int64_t)depth * (t.split + 1) / p.splits);
+        t.k1 = h.depth;
+        if (h.items > h.tiles) {
+            unsigned q = i / h.tiles;
+            i -= q * h.tiles;
+            t.out = q / j.splits;
+            t.split = q - t.out * j.splits;
+            t.k0 = (int)((int64_t)h.depth * t.split / j.splits);
+            t.k1 = (int)((int64_t)h.depth * (t.split + 1) / j.splits);
         }
-        const unsigned per = 8u * p.tiles_n, g = tiles_m > 8 ? i / per : 0;
-        const unsigned r = i - g * per, h = tiles_m - g * 8;
-        if (h >= 8) {
+        const unsigned per = 8u * j.tiles_n, g = h.tiles_m > 8 ? i / per : 0;
+        const unsigned r = i - g * per, rows = h.tiles_m - g * 8;
+        if (rows >= 8) {
             t.mt = g * 8 + (r & 7);
             t.nt = r >> 3;
         } else {
-            t.nt = r / h;
-            t.mt = g * 8 + (r - t.nt * h);
+            t.nt = r / rows;
+            t.mt = g * 8 + (r - t.nt * rows);
         }
         return t;
     };
@@ -349,8 +397,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             unsigned ph = 0;
             int64_t loads = 0;
             bool ok = true;
-            for (unsigned i = first_item; ok && i < items; i += step) {
+            for (unsigned q = 0, i; ok && (i = nth(q)) != kNoItem; q++) {
                 const Item t = item(i);
+                const Job &j = p.job[kTwo ? t.job : 0];
+                const int cols = kOut ? j.cols : kCols, kb = kTwo && t.job ? s1.kb : s0.kb;
+                const bool mn_a = kTwo ? j.amaj == MN_MAJOR : AMAJ == MN_MAJOR;
                 const int m = t.mt * kRows + 128 * (int)rank;
                 const int n = kDual ? t.nt * 128 : t.nt * cols + cols / 2 * (int)rank;
                 for (int k = t.k0; k < t.k1; k++) {
@@ -362,10 +413,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     const unsigned bar = ptx::of_first(full + 8 * s);
                     const bool second = k >= kb;
                     const int x = (second ? k - kb : k) * kDepth;
-                    const CUtensorMap *ma = second || t.out ? &p.a1 : &p.a;
-                    const CUtensorMap *mb = second || (kDual && rank) ? &p.b1 : &p.b;
+                    const CUtensorMap *ma = second || t.out ? &j.a1 : &j.a;
+                    const CUtensorMap *mb = second || (kDual && rank) ? &j.b1 : &j.b;
                     const unsigned da = sA + s * kOperand, db = sB + s * kOperand;
-                    if (AMAJ == K_MAJOR) {
+                    if (!mn_a) {
                         ptx::tma_load(da, ma, x, m, bar);
                     } else {
                         ptx::tma_load(da, ma, m, x, bar);
@@ -393,18 +444,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     } else if (warp == 1) {
         // ------------------------------------------------------------ MMA
         if (rank == 0 && lane == 0) {
-            // 32-bit sums of bf16 or fp16, 256 x 256 over the pair
-            const unsigned idesc = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) |
-                                   ((unsigned)AMAJ << 15) | ((unsigned)BMAJ << 16) | ((unsigned)(cols >> 3) << 17) |
-                                   ((kRows >> 4) << 24);
+            // 32-bit sums of bf16 or fp16, 256 rows over the pair
+            constexpr unsigned kType = (1u << 4) | (std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u) |
+                                       ((unsigned)BMAJ << 16) | ((kRows >> 4) << 24);
             // 16 of k: 32 bytes along a row, or 16 rows of 128 bytes
-            constexpr unsigned step_a = AMAJ == K_MAJOR ? 32 : 2048, step_b = BMAJ == K_MAJOR ? 32 : 2048;
+            constexpr unsigned step_b = BMAJ == K_MAJOR ? 32 : 2048;
             int s = 0;
             unsigned ph = 0;
             unsigned n = 0;
             bool ok = true;
-            for (unsigned i = first_item; ok && i < items; i += step, n++) {
+            for (unsigned i; ok && (i = nth(n)) != kNoItem; n++) {
                 const Item t = item(i);
+                const Job &job = p.job[kTwo ? t.job : 0];
+                const bool mn_a = kTwo ? job.amaj == MN_MAJOR : AMAJ == MN_MAJOR;
+                const unsigned idesc = kType | ((unsigned)mn_a << 15) | ((unsigned)((kOut ? job.cols : kCols) >> 3) << 17);
+                const unsigned step_a = mn_a ? 2048 : 32;
                 const int buf = (int)(n & 1);
                 if (!mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2)) break;
                 tc::fence_after();
@@ -436,27 +490,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         const int quad = warp & 3, half = (warp - 4) >> 2 & 1, set = kSets > 1 ? (warp - 4) >> 3 : 0;
         unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
-        const EpiArgs &e = p.e;
         unsigned cnt = set;
         // What the loss needs to know of this lane's row, fetched a tile ahead.
         int64_t next_target = -1;
         LossRow next_row = {0.0f, 0.0f, 0.0f, kNoTarget};
-        Item next = item(first_item + set * step);
+        unsigned following = nth(set);
+        Item next = {};
         auto fetch = [&] {
+            next = item(following);
+            if (EPI != EPI_LSE && EPI != EPI_Z) return;
+            const EpiArgs &e = p.job[0].e;
+            const int64_t M = s0.M;
             const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
             if (EPI == EPI_LSE) next_target = m < M ? e.target[m] : -1;
             if (EPI == EPI_Z && m < M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
-        if (first_item + set * step < items) fetch();
-        for (unsigned i = first_item + set * step; i < items; i += kSets * step, cnt += kSets) {
+        if (following != kNoItem) fetch();
+        while (following != kNoItem) {
             const Item t = next;
             const int64_t target = next_target;
             const LossRow row = next_row;
-            if (i + kSets * step < items) {
-                next = item(i + kSets * step);
-                fetch();
-            }
-            const int buf = (int)(cnt & 1);
+            const Job &job = p.job[kTwo ? t.job : 0];
+            const EpiArgs &e = job.e;
+            const int64_t M = kTwo && t.job ? s1.M : s0.M, N = job.N;
+            const int buf_use = (int)cnt;
+            cnt += kSets;
+            following = nth(cnt);
+            if (following != kNoItem) fetch();
+            const int buf = buf_use & 1;
             const int64_t m0 = (int64_t)t.mt * kRows + 128 * rank + 32 * quad, m = m0 + lane;
             const unsigned acc = tmem + ((unsigned)(32 * quad) << 16) + buf * kCols;
             auto release = [&] {
@@ -464,7 +525,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 __syncwarp();
                 if (lane == 0) ptx::arrive_cluster(bar_empty + 8 * buf);
             };
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((cnt >> 1) & 1), s_abort, s_error,
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((buf_use >> 1) & 1), s_abort, s_error,
                                                        4)))
                 break;
             tc::fence_after();
@@ -480,7 +541,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::load32(acc + col, g);
                     ptx::load32(acc + 128 + col, u);
                     if constexpr (EPI == EPI_GATED_BWD)
-                        load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, M, n0 + col, p.N, vdh, lane);
+                        load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, M, n0 + col, N, vdh, lane);
                     ptx::wait32(g);
                     ptx::wait32(u);
                     if (c == 1) release();
@@ -488,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
 #pragma unroll
                         for (int j = 0; j < 16; j++)
                             w[j] = pack2<T>(act_f<ACT>(g[2 * j]) * u[2 * j], act_f<ACT>(g[2 * j + 1]) * u[2 * j + 1]);
-                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, N, vec, lane);
                     } else {
                         unsigned wu[16];
 #pragma unroll
@@ -500,13 +561,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                             w[j] = pack2<T>(dh.x * u[2 * j] * d0, dh.y * u[2 * j + 1] * d1);
                             wu[j] = pack2<T>(dh.x * a0, dh.y * a1);
                         }
-                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, p.N, vec, lane);
-                        store_block<T>(st, wu, o1, e.ldo, m0, M, n0 + col, p.N, vec, lane);
+                        store_block<T>(st, w, o0, e.ldo, m0, M, n0 + col, N, vec, lane);
+                        store_block<T>(st, wu, o1, e.ldo, m0, M, n0 + col, N, vec, lane);
                     }
                 }
-            } else if constexpr (EPI == EPI_STORE || EPI == EPI_SUM) {
+            } else if constexpr (kOut) {
+                const int cols = job.cols;
+                const bool summed = e.acc != nullptr;
                 const int64_t n0 = (int64_t)t.nt * cols;
-                const float scale = EPI == EPI_STORE && e.plan ? ldexpf(1.0f, -e.plan->shift) : 1.0f;
+                const float scale = !summed && e.plan ? ldexpf(1.0f, -e.plan->shift) : 1.0f;
                 const bool nothing = t.k0 == t.k1;  // a part of a depth that turned out short: no product ran
 #pragma unroll 1
                 for (int c = 0; c < cols / 64; c++) {
@@ -515,19 +578,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::load32(acc + col, v);
                     ptx::wait32(v);
                     if (c == cols / 64 - 1) release();
-                    if (n0 + col >= p.N) continue;
+                    if (n0 + col >= N) continue;
                     if (nothing) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) v[j] = 0.0f;
                     }
-                    if constexpr (EPI == EPI_STORE) {
+                    if (!summed) {
                         unsigned w[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) w[j] = pack2<T>(v[2 * j] * scale, v[2 * j + 1] * scale);
-                        store_block<T>(st, w, static_cast<T *>(t.out ? e.o1 : e.o0), e.ldo, m0, M, n0 + col, p.N,
+                        store_block<T>(st, w, static_cast<T *>(t.out ? e.o1 : e.o0), e.ldo, m0, M, n0 + col, N,
                                        e.vec & 1, lane);
                     } else {
-                        float *o = e.acc + ((int64_t)t.out * p.splits + t.split) * p.M * e.ldo;
+                        float *o = e.acc + ((int64_t)t.out * job.splits + t.split) * job.M * e.ldo;
                         store_sums(st, v, o, e.ldo, m0, M, n0 + col, !e.first, lane);
                     }
                 }
@@ -536,7 +599,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 // columns of the vocabulary here, and which of them is the row's target: looked at once a tile, since
                 // few tiles hold a target or the end
-                const int wide = (int)(p.N - n0 < kWide ? p.N - n0 : kWide);
+                const int wide = (int)(N - n0 < kWide ? N - n0 : kWide);
                 const int tg = target >= n0 && target < n0 + wide ? (int)(target - n0) : -1;
                 const bool any = __any_sync(0xffffffffu, tg >= 0);
                 float top = -INFINITY, sum = 0.0f;
@@ -585,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + (s0 + s1);
                     top = mx;
                 }
-                if (m < M) e.part[((int64_t)t.nt * 2 + half) * p.M + m] = make_float2(top * e.grow, sum);
+                if (m < M) e.part[((int64_t)t.nt * 2 + half) * job.M + m] = make_float2(top * e.grow, sum);
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
@@ -598,9 +661,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     ptx::load32(acc + half * kWide + c * 32, v);
                     ptx::wait32(v);
                     if (c == kWide / 32 - 1) release();
-                    if (n0 + c * 32 >= p.N) continue;
+                    if (n0 + c * 32 >= N) continue;
                     loss_z<T>(v, w, row, col0 + c * 32, 32, any, e.lse, e.src, m, e.grow);
-                    store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, p.N, e.vec & 1, lane);
+                    store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, N, e.vec & 1, lane);
                 }
             }
         }
