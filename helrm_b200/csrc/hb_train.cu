@@ -682,7 +682,6 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
         const Matrix mw = in.fit({wt, vocab, inner, ldw});
-        const bool scaled = dtype == HELRM_FP16;
         const int64_t cap = pad(tokens, 256);  // the rows that take part, filled up
         uint16_t *hc = w.take<uint16_t>(cap * pitch(inner));
         const Matrix mh{hc, cap, inner, pitch(inner)};
@@ -692,7 +691,8 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         auto prepare = [&](cudaStream_t s) {
             in.copy(s);
             LossRows r = {dloss, targets, reinterpret_cast<const float2 *>(lse), ignore_index, vocab, tokens,
-                          static_cast<const unsigned short *>(h), ldh, inner, fits_vectors(h, ldh), scaled, 0, rows, src,
+                          static_cast<const unsigned short *>(h), ldh, inner, fits_vectors(h, ldh),
+                          dtype == HELRM_FP16 ? 32768.0f : 1.0f, 0, rows, src,
                           pos, plan, hc, pitch(inner)};
             // 32 rows a block, or at most 512 blocks
             r.per = (int)(cap > 32 * 512 ? pad(blocks(cap, 512), 32) : 32);

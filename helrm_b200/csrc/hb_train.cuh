@@ -166,7 +166,7 @@ struct EpiArgs {
     const struct LossRow *rows = nullptr;
     const int *src = nullptr;
     int64_t col0 = 0;                   // EPI_Z: first column of the piece in the vocabulary
-    const struct LossPlan *plan = nullptr;  // fp16: Z is scaled by 2^shift, undone when the products with it are stored
+    const struct LossPlan *plan = nullptr;  // Z's scale is undone when the products with it are stored
 };
 
 // 16-bit values col..col+7 of a row as four words; zeros past the end
@@ -255,14 +255,16 @@ constexpr int kNoTarget = -2147483647 - 1;
 struct LossPlan {
     int filled;  // rows, with those that fill up
     int count;   // rows that take part
-    int shift;   // fp16: Z is scaled by 2^shift
+    float unscale;  // what Z is to be multiplied by
 };
 // Each block goes through all the targets, four a thread at a time, keeps the
 // `per` places that are its own, and copies their rows to 16-byte boundaries
 // (zeros where they fill up): one launch, where a plan by one block and a copy
-// after it took 10 us.  scaled (fp16): the power of two that brings the largest
-// |dloss| of a row that takes part to [2^14, 2^15), so that Z keeps the
-// probabilities down to 2^-38.
+// after it took 10 us.
+// Z is scaled: the largest |dloss| of a row that takes part becomes 1, for fp16
+// 2^15, so that probabilities down to 2^-39 keep a place in that type's range.
+// A batch whose rows all weigh the same (a mean) then has its targets' entries
+// at a power of two, which 16 bits hold without an error.
 struct LossRows {
     const float *dloss;
     const int64_t *target;
@@ -270,7 +272,8 @@ struct LossRows {
     int64_t ignore, vocab, M;
     const unsigned short *h;
     int64_t ldh, cols;
-    bool vec, scaled;
+    bool vec;
+    float most;  // what the largest |dloss| becomes
     int per;
     LossRow *rows;
     int *src, *pos;
@@ -283,17 +286,16 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
     __shared__ float red[32];
     __shared__ int sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int shift = 0;
-    if (p.scaled) {
-        float top = 0.0f;
-        for (int64_t m = threadIdx.x; m < p.M; m += 1024)
-            if (p.target[m] != p.ignore) top = fmaxf(top, fabsf(p.dloss[m]));
-        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (lane == 0) red[warp] = top;
-        __syncthreads();
-        for (int i = 0; i < 32; i++) top = fmaxf(top, red[i]);
-        shift = top > 0.0f && top < INFINITY ? max(-100, min(120, 14 - ilogbf(top))) : 0;
-    }
+    float top = 0.0f;
+    for (int64_t m = threadIdx.x; m < p.M; m += 1024)
+        if (p.target[m] != p.ignore) top = fmaxf(top, fabsf(p.dloss[m]));
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (lane == 0) red[warp] = top;
+    __syncthreads();
+    for (int i = 0; i < 32; i++) top = fmaxf(top, red[i]);
+    if (!(top > 0.0f && top < INFINITY)) top = p.most;
+    top = fminf(fmaxf(top, 1e-30f), 1e30f);  // so that neither factor overflows
+    const float scale = p.most / top, unscale = top / p.most;
     const int first = blockIdx.x * p.per, last = first + p.per;
     int base = 0;
     for (int64_t m0 = 0; m0 < p.M; m0 += 4096) {
@@ -334,8 +336,7 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
                 const bool in = t[k] >= 0 && t[k] < p.vocab;
                 const float2 l = p.lse[m];
                 LossRow r;
-                r.g = in ? p.dloss[m] : NAN;
-                if (shift) r.g = ldexpf(r.g, shift);
+                r.g = in ? p.dloss[m] * scale : NAN;
                 r.max = l.x;
                 r.add = log2f(fabsf(r.g)) - l.y * kLog2e;
                 r.target = in ? (int)t[k] : -1;
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
         p.rows[j] = {0.0f, 0.0f, 0.0f, kNoTarget};
         p.src[j] = -1;
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.plan = {filled, base, shift};
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.plan = {filled, base, unscale};
     __syncthreads();
     for (int j = first + warp; j < end; j += 32) {  // a warp a row
         const int64_t m = p.src[j];

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
         auto wait_all = [&](unsigned a, unsigned parity) {
             return __all_sync(0xffffffffu, mbar_wait(a, parity, s_abort, s_error, 4));
         };
-        const float unscale = ldexpf(1.0f, -p.plan->shift);
+        const float unscale = p.plan->unscale;
         const bool vec = p.inner % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dw) & 15) == 0;
         auto fetch = [&](int64_t m) {  // the rows that fill up the last tile are there
             LossRow q;

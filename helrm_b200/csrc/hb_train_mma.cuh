@@ -569,7 +569,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int cols = job.cols;
                 const bool summed = e.acc != nullptr;
                 const int64_t n0 = (int64_t)t.nt * cols;
-                const float scale = !summed && e.plan ? ldexpf(1.0f, -e.plan->shift) : 1.0f;
+                const float scale = !summed && e.plan ? e.plan->unscale : 1.0f;
                 const bool nothing = t.k0 == t.k1;  // a part of a depth that turned out short: no product ran
 #pragma unroll 1
                 for (int c = 0; c < cols / 64; c++) {
@@ -688,7 +688,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     }
 }
 
-// out[m][n] = 16-bit (2^-shift * sum over the parts of acc[part][m][n]), four
+// out[m][n] = 16-bit (scale * sum over the parts of acc[part][m][n]), four
 // columns a lane; with pos the sums are those of row pos[m], or none (-1).
 // MANY: the 8 warps of a block take every 8th part each and are added up in
 // order (148 parts of 1024 x 16: 37 us with a thread going through all of them).
@@ -696,7 +696,7 @@ struct JoinArgs {
     const float *acc;
     int parts;
     int64_t rows, M, N, ld;  // rows of a part, rows and columns of the result, pitch of acc
-    const LossPlan *plan;    // not NULL: its shift
+    const LossPlan *plan;    // not NULL: its scale
     const int *pos;
 };
 template <class T, bool MANY>
@@ -723,7 +723,7 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs p, T *out) {
         for (int k = 1; k < 8; k++) add(red[k][lane]);
     }
     const int64_t n = c * 4;
-    const float scale = p.plan ? ldexpf(1.0f, -p.plan->shift) : 1.0f;
+    const float scale = p.plan ? p.plan->unscale : 1.0f;
     const float v[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
     T *o = out + m * p.N + n;
     if (p.N % 4 == 0 && n < p.N && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {
