@@ -225,16 +225,23 @@ __global__ void __launch_bounds__(1024) k_loss(const float2 *part, int64_t parts
     }
     red[warp][lane] = make_float2(top, s);
     __syncthreads();
-    if (warp || m >= M) return;
-    for (int i = 1; i < 32; i++) join(red[i][lane]);
+    // a warp a row from here
+    const float2 mine = red[lane][warp];
+    top = mine.x, s = mine.y;
+    for (int o = 16; o; o >>= 1) {
+        const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, top, o), __shfl_xor_sync(0xffffffffu, s, o));
+        join(other);
+    }
+    const int64_t row = (int64_t)blockIdx.x * 32 + warp;
+    if (lane || row >= M) return;
     if (!LAST) {
-        lse[blockIdx.y * M + m] = make_float2(top, s);
+        lse[blockIdx.y * M + row] = make_float2(top, s);
         return;
     }
     const float l = logf(s);
-    const int64_t t = target[m];
-    lse[m] = make_float2(top, l);
-    loss[m] = t == ignore ? 0.0f : t < 0 || t >= vocab ? NAN : top - at[m] + l;
+    const int64_t t = target[row];
+    lse[row] = make_float2(top, l);
+    loss[row] = t == ignore ? 0.0f : t < 0 || t >= vocab ? NAN : top - at[row] + l;
 }
 
 // What the gradients' epilogues need to know of a row, in one 16-byte load:
