@@ -464,7 +464,8 @@ static float logit_scale(int64_t inner) {
 
 // Columns of a vocabulary piece: Z of a piece takes at most 512 MiB (256 MiB:
 // 907 us for 4096 x 128 x 131072 where 704 are reached with 1 GiB, 64 MiB:
-// 1140), in whole rounds of the SM pairs for dW where that many fit.
+// 1140), in whole rounds of the SM pairs for dW where that many fit; 2048 at
+// least, which more than 131072 rows fill beyond that.
 static int64_t piece_columns(int64_t tokens, int64_t vocab) {
     const int64_t most = ((int64_t)256 << 20) / (tokens > 0 ? tokens : 1), round = 74 * kCols;
     int64_t c = most / 256 * 256;
