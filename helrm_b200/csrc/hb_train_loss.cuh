@@ -21,7 +21,9 @@
 // afterwards: no atomics, the same bits in every run.
 //
 // Bounds at 1024 tokens x 1000003 rows x 16: the exponentials, 16 a clock and
-// SM, 0.23 ms; operand bytes 64 MB.
+// SM, 0.23 ms; operand bytes 64 MB.  It takes 0.44 ms: about 2000 clocks a tile,
+// of which the exponentials are 1024 and the sixteen small products 1150, with
+// three hand-offs between them.
 #pragma once
 
 namespace hb {
