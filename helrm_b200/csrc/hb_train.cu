@@ -451,17 +451,6 @@ static Narrow narrow(int64_t tokens, int64_t inner, int64_t vocab) {
     return n;
 }
 
-// The tensor cores cut a sum's last bits off at every 16-deep step, towards
-// zero: a logit comes out short by 1.52e-8 of itself a step on average (a row's
-// largest logit by 0.48e-6, 0.97e-6, 1.99e-6, 3.87e-6 at 512, 1024, 2048, 4096
-// features, whatever its size, where rounding to nearest would leave 1e-7).
-// Multiplying by this takes the loss at 4096 features from 1.5e-6 off to the
-// noise of 32 bits; it costs nothing, being part of a multiplication that is
-// there.  It is 1 for narrow rows, whose gradients' kernel has no use for it.
-static float logit_scale(int64_t inner) {
-    return inner <= kNarrow ? 1.0f : (float)(1.0 + 1.52e-8 * (double)blocks(inner, 16));
-}
-
 // Columns of a vocabulary piece: Z of a piece takes at most 512 MiB (256 MiB:
 // 907 us for 4096 x 128 x 131072 where 704 are reached with 1 GiB, 64 MiB:
 // 1140), in whole rounds of the SM pairs for dW where that many fit; 2048 at
@@ -656,8 +645,12 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
             d.e.part = part;
             d.e.at = at;
             d.e.target = targets + m0;
-            d.e.grow = logit_scale(inner);
-            by_dtype(dtype, [&](auto t) { launch<decltype(t), EPI_LSE, 0>(d, s); });
+            by_dtype(dtype, [&](auto t) {
+                if (inner > kChunk * kDepth)
+                    launch<decltype(t), EPI_LSE_LONG, 0>(d, s);
+                else
+                    launch<decltype(t), EPI_LSE, 0>(d, s);
+            });
             const float *none = nullptr;
             const int64_t *no_targets = nullptr;
             if (joined)
@@ -773,8 +766,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 d.e.src = src;
                 d.e.lse = reinterpret_cast<const float2 *>(lse);
                 d.e.col0 = c0;
-                d.e.grow = logit_scale(inner);
-                launch<T, EPI_Z, 0>(d, s);
+                    launch<T, EPI_Z, 0>(d, s);
                 Product piece[2];
                 int np = 0;
                 if (dh) {

@@ -149,7 +149,7 @@ __device__ __forceinline__ void act_df(float g, float &a, float &d) {
 }
 
 // ---------------------------------------------------------------- products
-enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_OUT, EPI_LSE, EPI_Z };
+enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_OUT, EPI_LSE, EPI_LSE_LONG, EPI_Z };
 struct EpiArgs {
     void *o0 = nullptr, *o1 = nullptr;  // 16-bit outputs
     int64_t ldo = 0;                    // their row pitch, or that of acc
@@ -160,7 +160,6 @@ struct EpiArgs {
     int first = 1;                      // 0: added to what acc holds
     float2 *part = nullptr;             // EPI_LSE: (max, sum) of each warp's columns, [part][row]
     float *at = nullptr;                // EPI_LSE: the target's logit
-    float grow = 1.0f;                  // EPI_LSE, EPI_Z: what a logit is multiplied by (logit_scale)
     const int64_t *target = nullptr;
     const float2 *lse = nullptr;        // EPI_Z: the row's (maximum, log of the sum relative to it)
     const struct LossRow *rows = nullptr;
@@ -377,7 +376,7 @@ __global__ void __launch_bounds__(1024) k_loss_rows(LossRows p) {
 // and zero times that is no zero in the products).
 template <class T>
 __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const LossRow &r, int col, int wide, bool any,
-                                       const float2 *lse, const int *src, int64_t m, float grow) {
+                                       const float2 *lse, const int *src, int64_t m) {
     int at = -1;
     float hot = 0.0f;
     if (any) {
@@ -386,13 +385,12 @@ __device__ __forceinline__ void loss_z(float (&v)[32], unsigned (&w)[16], const 
         float x = v[0];
 #pragma unroll
         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-        if (at >= 0) hot = expm1f(fmaf(x, grow, -r.max) - lse[src[m]].y) * fabsf(r.g);
+        if (at >= 0) hot = expm1f((x - r.max) - lse[src[m]].y) * fabsf(r.g);
     }
-    const uint64_t grow2 = join2(grow, grow), max2 = join2(-r.max, -r.max), log2 = join2(kLog2e, kLog2e),
-                   more2 = join2(r.add, r.add);
+    const uint64_t max2 = join2(-r.max, -r.max), log2 = join2(kLog2e, kLog2e), more2 = join2(r.add, r.add);
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-        split2(fma2(fma2(join2(v[j], v[j + 1]), grow2, max2), log2, more2), v[j], v[j + 1]);
+        split2(fma2(add2(join2(v[j], v[j + 1]), max2), log2, more2), v[j], v[j + 1]);
         v[j] = ex2(v[j]);
         v[j + 1] = ex2(v[j + 1]);
     }

@@ -68,22 +68,6 @@ __device__ __forceinline__ void mma_own(unsigned d, uint64_t a, uint64_t b, unsi
 __device__ __forceinline__ void commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void load16(unsigned addr, float (&v)[16]) {
-    unsigned *r = reinterpret_cast<unsigned *>(v);
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(addr));
-}
-__device__ __forceinline__ void wait16(float (&v)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
-                   "+f"(v[15])
-                 :
-                 : "memory");
-}
 }  // namespace ptx
 
 template <class T>
@@ -339,7 +323,7 @@ __global__ void __launch_bounds__(kNarrowThreads, 1) k_loss_grads_narrow(const _
                         __syncwarp();
                         if (lane == 0) tc::mbar_arrive(sempty + 8 * set);
                     }
-                    loss_z<T>(v, w, row, col + c * 32, (int)p.vocab - col - c * 32, any, p.lse, p.src, m, 1.0f);
+                    loss_z<T>(v, w, row, col + c * 32, (int)p.vocab - col - c * 32, any, p.lse, p.src, m);
                     // the products that read this buffer two tiles ago
                     if (!c && !(ok = wait_all(zempty + 8 * set, ((n >> 1) & 1) ^ 1))) break;
 #pragma unroll

@@ -51,6 +51,18 @@ constexpr int kProductSmem = 2 * kStages * kOperand + kStageOut + 8 * kBarriers 
 // results); the others need the registers of 8.
 __host__ __device__ constexpr int epi_warps(int epi) { return epi == EPI_LSE || epi == EPI_Z ? 16 : 8; }
 __host__ __device__ constexpr int product_threads(int epi) { return 128 + 32 * epi_warps(epi); }
+// The tensor cores cut a running sum towards zero at every 16-deep step, by half
+// a unit in its last place on average: a row's largest logit came out 0.5e-6 of
+// itself short at 512 features and 3.9e-6 at 4096, always to the same side.  So
+// a loss over more than kChunk slices (512 features) accumulates that many at a
+// time and adds the parts, rounded to nearest, in its epilogue's registers
+// (EPI_LSE_LONG): what is lost stays at the first figure for any depth, the loss
+// within 1.6e-7 of itself (8192 x 4096 x 131072: 1.5e-6 in one sum).  An
+// accumulator goes back as soon as it is read, so the additions and the
+// exponentials run under the products to come; reading it takes tensor memory's
+// time.  4096 x 2048 x 37888: 460 us in one sum, 469 in parts of 1024 (loss
+// within 3.4e-7), 488 in parts of 512, 525 in parts of 256 (0.9e-7).
+constexpr int kChunk = 8;
 constexpr unsigned long long kWaitNs = 4000000000ull;
 
 enum { K_MAJOR = 0, MN_MAJOR = 1 };
@@ -173,6 +185,22 @@ __device__ __forceinline__ void wait32(float (&v)[32]) {
                  :
                  : "memory");
 }
+__device__ __forceinline__ void load16(unsigned addr, float (&v)[16]) {
+    unsigned *r = reinterpret_cast<unsigned *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr));
+}
+__device__ __forceinline__ void wait16(float (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                   "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]),
+                   "+f"(v[15])
+                 :
+                 : "memory");
+}
 }  // namespace ptx
 
 // A warp's 32 x 32 block of 16-bit values between registers (a row a lane) and
@@ -269,6 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     k_mma_product(const __grid_constant__ ProductArgs<JOBS> p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
     constexpr int kWarps = epi_warps(EPI), kSets = kWarps / 8;
+    constexpr bool kLong = EPI == EPI_LSE_LONG;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *stage = smem + 2 * kStages * kOperand;
     uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kStageOut);
@@ -459,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             constexpr unsigned step_b = BMAJ == K_MAJOR ? 32 : 2048;
             int s = 0;
             unsigned ph = 0;
-            unsigned n = 0;
+            unsigned n = 0, use = 0;  // items, and accumulators filled
             bool ok = true;
             for (unsigned i; ok && (i = nth(n)) != kNoItem; n++) {
                 const Item t = item(i);
@@ -467,24 +496,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const bool mn_a = kTwo ? job.amaj == MN_MAJOR : AMAJ == MN_MAJOR;
                 const unsigned idesc = kType | ((unsigned)mn_a << 15) | ((unsigned)((kOut ? job.cols : kCols) >> 3) << 17);
                 const unsigned step_a = mn_a ? 2048 : 32;
-                const int buf = (int)(n & 1);
-                if (!mbar_wait(tempty + 8 * buf, (unsigned)((n >> 1) & 1) ^ 1, s_abort, s_error, 2)) break;
-                tc::fence_after();
-                const unsigned d = tmem + buf * kCols;
-                for (int k = t.k0; k < t.k1; k++) {
-                    if (!mbar_wait(full + 8 * s, ph, s_abort, s_error, 2)) {
+                int k = t.k0;
+                do {  // an accumulator's share of the depth: all of it, but for kLong
+                    const int k0 = k, k1 = kLong && k + kChunk < t.k1 ? k + kChunk : t.k1;
+                    const int buf = (int)(use & 1);
+                    if (!mbar_wait(tempty + 8 * buf, (unsigned)((use >> 1) & 1) ^ 1, s_abort, s_error, 2)) {
                         ok = false;
                         break;
                     }
+                    use++;
                     tc::fence_after();
-                    const uint64_t da = ptx::descriptor(sA + s * kOperand), db = ptx::descriptor(sB + s * kOperand);
+                    const unsigned d = tmem + buf * kCols;
+                    for (; k < k1; k++) {
+                        if (!mbar_wait(full + 8 * s, ph, s_abort, s_error, 2)) {
+                            ok = false;
+                            break;
+                        }
+                        tc::fence_after();
+                        const uint64_t da = ptx::descriptor(sA + s * kOperand), db = ptx::descriptor(sB + s * kOperand);
 #pragma unroll
-                    for (int j = 0; j < kDepth / 16; j++)
-                        ptx::mma(d, da + ((j * step_a) >> 4), db + ((j * step_b) >> 4), idesc, k > t.k0 || j > 0);
-                    ptx::commit_both(empty + 8 * s);
-                    if (++s == kStages) s = 0, ph ^= 1;
-                }
-                if (ok) ptx::commit_both(tfull + 8 * buf);
+                        for (int j = 0; j < kDepth / 16; j++)
+                            ptx::mma(d, da + ((j * step_a) >> 4), db + ((j * step_b) >> 4), idesc, k > k0 || j > 0);
+                        ptx::commit_both(empty + 8 * s);
+                        if (++s == kStages) s = 0, ph ^= 1;
+                    }
+                    if (ok) ptx::commit_both(tfull + 8 * buf);
+                } while (kLong && ok && k < t.k1);
             }
             // after a failure too, no MMA is left in flight
             ptx::commit_own(drain);
@@ -498,7 +535,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         const int quad = warp & 3, half = (warp - 4) >> 2 & 1, set = kSets > 1 ? (warp - 4) >> 3 : 0;
         unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
-        unsigned cnt = set;
+        unsigned cnt = set, use = 0;  // items; with kLong, accumulators read
         // What the loss needs to know of this lane's row, fetched a tile ahead.
         int64_t next_target = -1;
         LossRow next_row = {0.0f, 0.0f, 0.0f, kNoTarget};
@@ -506,11 +543,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         Item next = {};
         auto fetch = [&] {
             next = item(following);
-            if (EPI != EPI_LSE && EPI != EPI_Z) return;
+            if (EPI != EPI_LSE && !kLong && EPI != EPI_Z) return;
             const EpiArgs &e = p.job[0].e;
             const int64_t M = s0.M;
             const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
-            if (EPI == EPI_LSE) next_target = m < M ? e.target[m] : -1;
+            if (EPI == EPI_LSE || kLong) next_target = m < M ? e.target[m] : -1;
             if (EPI == EPI_Z && m < M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
         if (following != kNoItem) fetch();
@@ -528,15 +565,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             const int buf = buf_use & 1;
             const int64_t m0 = (int64_t)t.mt * kRows + 128 * rank + 32 * quad, m = m0 + lane;
             const unsigned acc = tmem + ((unsigned)(32 * quad) << 16) + buf * kCols;
-            auto release = [&] {
+            auto release = [&](int buf) {
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::arrive_cluster(bar_empty + 8 * buf);
             };
-            if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((buf_use >> 1) & 1), s_abort, s_error,
+            if constexpr (!kLong) {
+                if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((buf_use >> 1) & 1), s_abort, s_error,
                                                        4)))
-                break;
-            tc::fence_after();
+                    break;
+                tc::fence_after();
+            }
             if constexpr (kDual) {
                 const int64_t n0 = (int64_t)t.nt * 128;
                 T *o0 = static_cast<T *>(e.o0), *o1 = static_cast<T *>(e.o1);
@@ -552,7 +591,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         load_block<T>(st, w, static_cast<const T *>(e.dh), e.lddh, m0, M, n0 + col, N, vdh, lane);
                     ptx::wait32(g);
                     ptx::wait32(u);
-                    if (c == 1) release();
+                    if (c == 1) release(buf);
                     if constexpr (EPI == EPI_GATED) {
 #pragma unroll
                         for (int j = 0; j < 16; j++)
@@ -585,7 +624,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     float v[32];
                     ptx::load32(acc + col, v);
                     ptx::wait32(v);
-                    if (c == cols / 64 - 1) release();
+                    if (c == cols / 64 - 1) release(buf);
                     if (n0 + col >= N) continue;
                     if (nothing) {
 #pragma unroll
@@ -602,7 +641,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         store_sums(st, v, o, e.ldo, m0, M, n0 + col, !e.first, lane);
                     }
                 }
-            } else if constexpr (EPI == EPI_LSE) {
+            } else if constexpr (EPI == EPI_LSE || kLong) {
                 constexpr int kWide = kCols / 2;  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 // columns of the vocabulary here, and which of them is the row's target: looked at once a tile, since
@@ -611,13 +650,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int tg = target >= n0 && target < n0 + wide ? (int)(target - n0) : -1;
                 const bool any = __any_sync(0xffffffffu, tg >= 0);
                 float top = -INFINITY, sum = 0.0f;
-                const float log2e = kLog2e * e.grow;
-#pragma unroll 1
-                for (int c = 0; c < kWide / 32; c++) {
-                    float v[32];
-                    ptx::load32(acc + half * kWide + c * 32, v);
-                    ptx::wait32(v);
-                    if (c == kWide / 32 - 1) release();
+                auto take = [&](float (&v)[32], int c) {
                     if (wide < kWide) {
                         asm volatile("");  // a branch, not 32 selections in every tile
 #pragma unroll
@@ -630,7 +663,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         float x = v[0];
 #pragma unroll
                         for (int j = 1; j < 32; j++) x = at == j ? v[j] : x;
-                        if (at >= 0 && at < 32) e.at[m] = x * e.grow;
+                        if (at >= 0 && at < 32) e.at[m] = x;
                     }
                     float m0 = max3(top, v[0], v[1]), m1 = v[2];
 #pragma unroll
@@ -641,7 +674,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     const float mx = max3(m0, m1, v[31]);
                     // a row of minus infinities so far: relative to 0, nothing to add
                     const float ref = mx == -INFINITY ? 0.0f : mx;
-                    const uint64_t ref2 = join2(-ref, -ref), log2 = join2(log2e, log2e);
+                    const uint64_t ref2 = join2(-ref, -ref), log2 = join2(kLog2e, kLog2e);
                     uint64_t sum0 = 0, sum1 = 0;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
@@ -653,10 +686,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     }
                     float s0, s1;
                     split2(add2(sum0, sum1), s0, s1);
-                    sum = (top == mx ? sum : sum * ex2((top - ref) * log2e)) + (s0 + s1);
+                    sum = (top == mx ? sum : sum * ex2((top - ref) * kLog2e)) + (s0 + s1);
                     top = mx;
+                };
+                if constexpr (kLong) {
+                    float v[kWide / 32][32];
+                    bool ok = true;
+                    for (int k = t.k0; k < t.k1; k += kChunk, use++) {
+                        const unsigned b = use & 1, from = tmem + ((unsigned)(32 * quad) << 16) + b * kCols + half * kWide;
+                        if (!(ok = __all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (use >> 1) & 1, s_abort, s_error, 4))))
+                            break;
+                        tc::fence_after();
+                        if (k == t.k0) {
+#pragma unroll
+                            for (int c = 0; c < kWide / 32; c++) {
+                                ptx::load32(from + c * 32, v[c]);
+                                ptx::wait32(v[c]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < kWide / 16; c++) {
+                                float x[16];
+                                ptx::load16(from + c * 16, x);
+                                ptx::wait16(x);
+#pragma unroll
+                                for (int j = 0; j < 16; j++) v[c / 2][c % 2 * 16 + j] += x[j];
+                            }
+                        }
+                        release(b);
+                    }
+                    if (!ok) break;
+#pragma unroll
+                    for (int c = 0; c < kWide / 32; c++) take(v[c], c);
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < kWide / 32; c++) {
+                        float v[32];
+                        ptx::load32(acc + half * kWide + c * 32, v);
+                        ptx::wait32(v);
+                        if (c == kWide / 32 - 1) release(buf);
+                        take(v, c);
+                    }
                 }
-                if (m < M) e.part[((int64_t)t.nt * 2 + half) * job.M + m] = make_float2(top * e.grow, sum);
+                if (m < M) e.part[((int64_t)t.nt * 2 + half) * job.M + m] = make_float2(top, sum);
             } else if constexpr (EPI == EPI_Z) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
@@ -668,9 +740,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     unsigned w[16];
                     ptx::load32(acc + half * kWide + c * 32, v);
                     ptx::wait32(v);
-                    if (c == kWide / 32 - 1) release();
+                    if (c == kWide / 32 - 1) release(buf);
                     if (n0 + c * 32 >= N) continue;
-                    loss_z<T>(v, w, row, col0 + c * 32, 32, any, e.lse, e.src, m, e.grow);
+                    loss_z<T>(v, w, row, col0 + c * 32, 32, any, e.lse, e.src, m);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, N, e.vec & 1, lane);
                 }
             }
