@@ -397,7 +397,7 @@ static void gradients(Product *d, int n, cudaStream_t s) {
     for (int i = 0; i < n; i++) {
         const Product &g = d[i];
         for (int k = 0; g.out[0] && g.splits > 1 && k < g.outputs; k++)
-            join<T>({g.acc + (int64_t)k * g.splits * g.M * g.e.ldo, g.splits, g.M, g.M, g.N, g.e.ldo, g.e.plan, nullptr},
+            join<T>({g.acc + (int64_t)k * g.splits * g.M * g.e.ldo, g.splits, g.M, g.M, g.N, g.e.ldo, g.e.unscale, nullptr},
                     g.out[k], s);
     }
 }
@@ -539,6 +539,10 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
         gw.out[0] = dwg ? dwg : dwu, gw.out[1] = dwu;
         const bool one = tokens && together(all);
         gw.outputs = dwg && dwu ? 2 : 1;
+        const bool scaled = dtype == HELRM_FP16;
+        float4 *range = scaled ? w.take<float4>(kRangeBlocks) : nullptr;
+        float *unscale = scaled ? w.take<float>(1) : nullptr;
+        gx.e.unscale = gw.e.unscale = unscale;
         int n = 0;
         for (Product &g : all) {
             if (!g.out[0]) continue;
@@ -566,6 +570,25 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
             d.e.dh = dh;
             d.e.lddh = lddh;
             d.e.vec = 1 | (fits_vectors(dh, lddh) ? 2 : 0);
+            if (scaled) {
+                GatedRange r = {};
+                int64_t tasks = 0;
+                const Matrix of[4] = {{dh, tokens, width, lddh}, mx, mg, mu};
+                for (int k = 0; k < 4; k++) {
+                    const Matrix &m = of[k];
+                    r.p[k] = static_cast<const unsigned short *>(m.p);
+                    r.ld[k] = m.ld, r.rows[k] = m.rows, r.cols[k] = m.cols;
+                    r.segments[k] = blocks(m.cols, kRangeSegment);
+                    tasks += m.cols <= 256 ? blocks(m.rows, 8) : m.rows * r.segments[k];
+                    r.end[k] = tasks;
+                }
+                r.vec = fits_vectors(dh, lddh);
+                r.part = range;
+                d.e.ranges = blocks(tasks, kRangeWarps) < kRangeBlocks ? (int)blocks(tasks, kRangeWarps) : kRangeBlocks;
+                d.e.range = range;
+                d.e.made = unscale;
+                start("gradients' range", k_gated_range, d.e.ranges, kRangeThreads, 0, s, r);
+            }
             by_act(act, [&](auto a) { launch<T, EPI_GATED_BWD, decltype(a)::value>(d, s); });
             if (one) {
                 gradients<T>(grads, n, s);
@@ -723,7 +746,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 a.error = runtime().error;
                 raise_shared_memory<k_loss_grads_narrow<T>>(kNarrowSmem);
                 start("loss gradients", k_loss_grads_narrow<T>, nr.grid, kNarrowThreads, kNarrowSmem, s, a);
-                if (dh) join<T>({part, nr.grid, cap, tokens, inner, nr.depth, plan, pos}, dh, s);
+                if (dh) join<T>({part, nr.grid, cap, tokens, inner, nr.depth, &plan->unscale, pos}, dh, s);
             });
             return;
         }
@@ -784,7 +807,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                     g.a = mz;
                     g.plan = plan;
                     g.M = n;
-                    g.e.plan = plan;
+                    g.e.unscale = &plan->unscale;
                     g.out[0] = static_cast<T *>(dw) + c0 * inner;
                     g.acc = acc_w;
                 }
@@ -795,7 +818,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                     for (int i = np - 1; i >= 0; i--) gradients<T>(piece + i, 1, s);
                 }
             }
-            if (dh) join<T>({acc, gh.splits, cap, tokens, inner, lda, plan, pos}, dh, s);
+            if (dh) join<T>({acc, gh.splits, cap, tokens, inner, lda, &plan->unscale, pos}, dh, s);
         });
     });
 }

@@ -165,7 +165,10 @@ struct EpiArgs {
     const struct LossRow *rows = nullptr;
     const int *src = nullptr;
     int64_t col0 = 0;                   // EPI_Z: first column of the piece in the vocabulary
-    const struct LossPlan *plan = nullptr;  // Z's scale is undone when the products with it are stored
+    const float *unscale = nullptr;     // EPI_OUT: the operands' scale is undone when a product with them is stored
+    const float4 *range = nullptr;      // EPI_GATED_BWD in fp16: what k_gated_range found, a block each,
+    int ranges = 0;
+    float *made = nullptr;              // and where the scale's inverse goes
 };
 
 // 16-bit values col..col+7 of a row as four words; zeros past the end
@@ -186,6 +189,142 @@ __device__ __forceinline__ void store8(unsigned short *row, int64_t col, int64_t
 #pragma unroll
     for (int k = 0; k < 8; k++)
         if (col + k < cols) row[col + k] = (unsigned short)(p[k >> 1] >> (16 * (k & 1)));
+}
+
+// ---------------------------------------------------------------- fp16's range
+// dG = dH U act'(G) and dU = dH act(G) enter products whose results fp16 may hold
+// where it does not hold them (dH 6e4, U 4, weights of 1e-2), or holds few of
+// their bits (dH 1e-5, act(G) 1e-2).  So they are scaled by a power of two that
+// brings a bound of both to at least 2^14, below 2^15:
+//   max |dH| max_i |x_i| max(1.13 max_j |wu_j|, max_j |wg_j|)
+// with the norms of rows (Cauchy and Schwarz; |act'| <= 1.13, |act(g)| <= |g|).
+// Values down to 2^-28 of the bound keep all their bits.  dH and rows that are not
+// finite have no say.  bf16 has a float's range and no scale.  It reads what the
+// next kernel will read (58 MB of 4096 x 1024 x 4096 in 17 us of the call's 190,
+// 1.5 MB of 64 x 432 x 512 in 2.5 of 24; with 148 blocks 18 and 2.5).
+// Long rows go in segments; a squared norm is at most their number times the
+// largest segment's.  A warp takes a segment, or eight rows of at most 256
+// columns, with its loads in flight together.
+constexpr int kRangeBlocks = 2 * 148, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32, kRangeSegment = 8192;
+struct GatedRange {
+    const unsigned short *p[4];  // dH, x, wg, wu; rows on 16-byte boundaries but for dH's (vec)
+    int64_t ld[4], rows[4], cols[4], segments[4];
+    int64_t end[4];              // tasks of a matrix and those before it
+    bool vec;
+    float4 *part;                // a block's max |dH| and largest squared norms
+};
+__device__ __forceinline__ void range_of(unsigned two, bool norm, float &s) {
+    const float2 f = unpack2<__half>(two);
+    const float a = fabsf(f.x), b = fabsf(f.y);
+    s = norm ? fmaf(f.x, f.x, fmaf(f.y, f.y, s)) : fmaxf(s, fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f));
+}
+__device__ __forceinline__ void range_of(uint4 v, bool norm, float &s) {
+    range_of(v.x, norm, s);
+    range_of(v.y, norm, s);
+    range_of(v.z, norm, s);
+    range_of(v.w, norm, s);
+}
+__global__ void __launch_bounds__(kRangeThreads) k_gated_range(const __grid_constant__ GatedRange p) {
+    after_previous();
+    __shared__ float red[kRangeWarps][4];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t i = blockIdx.x * kRangeWarps + warp; i < p.end[3]; i += gridDim.x * kRangeWarps) {
+        const int k = i < p.end[0] ? 0 : i < p.end[1] ? 1 : i < p.end[2] ? 2 : 3;
+        const int64_t rows = p.rows[k], cols = p.cols[k], ld = p.ld[k], t = k ? i - p.end[k - 1] : i;
+        const bool norm = k > 0;
+        float most = 0.0f;
+        auto keep = [&](float s) {
+            for (int o = 16; norm && o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (s < INFINITY) most = fmaxf(most, s);
+        };
+        if (norm || p.vec) {
+            const uint4 none = make_uint4(0, 0, 0, 0);
+            if (cols <= 256) {
+                const unsigned short *in = p.p[k] + t * 8 * ld;
+                const int whole = (int)cols / 8, c = whole * 8 + lane;
+                uint4 v[8];
+                unsigned short last[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const bool on = t * 8 + j < rows;
+                    v[j] = on && lane < whole ? *reinterpret_cast<const uint4 *>(in + j * ld + lane * 8) : none;
+                    last[j] = on && c < cols ? in[j * ld + c] : (unsigned short)0;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    float s = 0.0f;
+                    range_of(v[j], norm, s);
+                    range_of(last[j], norm, s);
+                    keep(s);
+                }
+            } else {
+                const int64_t r = t / p.segments[k], c0 = (t - r * p.segments[k]) * kRangeSegment;
+                const unsigned short *in = p.p[k] + r * ld + c0;
+                const int n = (int)(cols - c0 < kRangeSegment ? cols - c0 : kRangeSegment), whole = n / 8 * 8;
+                const unsigned short last = whole + lane < n ? in[whole + lane] : (unsigned short)0;
+                float s = 0.0f;
+                for (int c = lane * 8; c < whole; c += 8 * 256) {
+                    uint4 v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        v[j] = c + j * 256 < whole ? *reinterpret_cast<const uint4 *>(in + c + j * 256) : none;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) range_of(v[j], norm, s);
+                }
+                range_of(last, norm, s);
+                keep(s);
+            }
+        } else {  // dH's rows on any boundary
+            const bool narrow = cols <= 256;
+            const int64_t r0 = narrow ? t * 8 : t / p.segments[0], c0 = narrow ? 0 : (t - r0 * p.segments[0]) * kRangeSegment;
+            const int64_t r1 = narrow ? (r0 + 8 < rows ? r0 + 8 : rows) : r0 + 1;
+            const int n = (int)(cols - c0 < kRangeSegment ? cols - c0 : kRangeSegment);
+            for (int64_t r = r0; r < r1; r++) {
+                const unsigned short *in = p.p[0] + r * ld + c0;
+                for (int c = lane; c < n; c += 256) {
+                    unsigned short v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = c + j * 32 < n ? in[c + j * 32] : (unsigned short)0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) range_of(v[j], false, most);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j == k) top[j] = fmaxf(top[j], most);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        for (int o = 16; o; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+        if (lane == 0) red[warp][k] = top[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < 4) {
+        float t = 0.0f;
+        for (int i = 0; i < kRangeWarps; i++) t = fmaxf(t, red[i][threadIdx.x]);
+        if (threadIdx.x > 0) t *= (float)p.segments[threadIdx.x];
+        reinterpret_cast<float *>(p.part + blockIdx.x)[threadIdx.x] = t;
+    }
+}
+// The scale from what n blocks found, in every lane of a warp.
+__device__ __forceinline__ float gated_scale(const float4 *part, int n) {
+    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < (kRangeBlocks + 31) / 32; k++) {  // all loads at once
+        const int i = 32 * k + (threadIdx.x & 31);
+        const float4 v = i < n ? part[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        t = make_float4(fmaxf(t.x, v.x), fmaxf(t.y, v.y), fmaxf(t.z, v.z), fmaxf(t.w, v.w));
+    }
+    for (int o = 16; o; o >>= 1) {
+        t.x = fmaxf(t.x, __shfl_xor_sync(0xffffffffu, t.x, o));
+        t.y = fmaxf(t.y, __shfl_xor_sync(0xffffffffu, t.y, o));
+        t.z = fmaxf(t.z, __shfl_xor_sync(0xffffffffu, t.z, o));
+        t.w = fmaxf(t.w, __shfl_xor_sync(0xffffffffu, t.w, o));
+    }
+    const float bound = t.x * sqrtf(t.y) * fmaxf(1.13f * sqrtf(t.w), sqrtf(t.z));  // 2^-75 to 2^80, or 0
+    return bound > 0.0f ? __uint_as_float((unsigned)(127 + 14 + 127 - (int)(__float_as_uint(bound) >> 23)) << 23) : 1.0f;
 }
 
 // ---------------------------------------------------------------- the loss

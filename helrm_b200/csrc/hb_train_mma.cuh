@@ -297,7 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     k_mma_product(const __grid_constant__ ProductArgs<JOBS> p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
     constexpr int kWarps = epi_warps(EPI), kSets = kWarps / 8;
-    constexpr bool kLong = EPI == EPI_LSE_LONG;
+    constexpr bool kLong = EPI == EPI_LSE_LONG, kScaled = EPI == EPI_GATED_BWD && std::is_same<T, __half>::value;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *stage = smem + 2 * kStages * kOperand;
     uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kStageOut);
@@ -536,6 +536,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         unsigned char *st = stage + (warp - 4) * (kStageOut / kWarps);
         const unsigned bar_empty = ptx::of_first(tempty);
         unsigned cnt = set, use = 0;  // items; with kLong, accumulators read
+        float scale = 1.0f;
+        if constexpr (kScaled) {
+            const EpiArgs &e = p.job[0].e;
+            scale = gated_scale(e.range, e.ranges);
+            if (blockIdx.x == 0 && threadIdx.x == 128) *e.made = 1.0f / scale;
+        }
         // What the loss needs to know of this lane's row, fetched a tile ahead.
         int64_t next_target = -1;
         LossRow next_row = {0.0f, 0.0f, 0.0f, kNoTarget};
@@ -601,7 +607,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         unsigned wu[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            const float2 dh = unpack2<T>(w[j]);
+                            float2 dh = unpack2<T>(w[j]);
+                            if constexpr (kScaled) dh.x *= scale, dh.y *= scale;
                             float a0, d0, a1, d1;
                             act_df<ACT>(g[2 * j], a0, d0);
                             act_df<ACT>(g[2 * j + 1], a1, d1);
@@ -616,7 +623,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 const int cols = job.cols;
                 const bool summed = e.acc != nullptr;
                 const int64_t n0 = (int64_t)t.nt * cols;
-                const float scale = !summed && e.plan ? e.plan->unscale : 1.0f;
+                const float scale = !summed && e.unscale ? *e.unscale : 1.0f;
                 const bool nothing = t.k0 == t.k1;  // a part of a depth that turned out short: no product ran
 #pragma unroll 1
                 for (int c = 0; c < cols / 64; c++) {
@@ -776,7 +783,7 @@ struct JoinArgs {
     const float *acc;
     int parts;
     int64_t rows, M, N, ld;  // rows of a part, rows and columns of the result, pitch of acc
-    const LossPlan *plan;    // not NULL: its scale
+    const float *unscale;    // not NULL: the scale
     const int *pos;
 };
 template <class T, bool MANY>
@@ -803,7 +810,7 @@ __global__ void __launch_bounds__(256) k_join(JoinArgs p, T *out) {
         for (int k = 1; k < 8; k++) add(red[k][lane]);
     }
     const int64_t n = c * 4;
-    const float scale = p.plan ? p.plan->unscale : 1.0f;
+    const float scale = p.unscale ? *p.unscale : 1.0f;
     const float v[4] = {s.x * scale, s.y * scale, s.z * scale, s.w * scale};
     T *o = out + m * p.N + n;
     if (p.N % 4 == 0 && n < p.N && (reinterpret_cast<uintptr_t>(out) & 7) == 0) {

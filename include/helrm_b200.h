@@ -361,8 +361,10 @@ int helrm_GatedForward(int device, int dtype, int act, int64_t tokens, int64_t i
                        size_t *ws_bytes, void *stream);
 /* The gradients dx [tokens][inner], dwg and dwu [width][inner] of a loss
  * whose gradient by h is dh [tokens][width].  The projections are formed
- * again from x, or, with x NULL, from its 8-bit checkpoint (q, e).  An output
- * that is NULL is not computed. */
+ * again from x, or, with x NULL, from its 8-bit checkpoint (q, e).  The
+ * gradients by the projections are rounded to the 16-bit type once, as operands
+ * of the products with x and the weights; in fp16 relative to a power of two
+ * that keeps them in range.  An output that is NULL is not computed. */
 int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, int64_t inner, int64_t width, const void *dh,
                         int64_t lddh, const void *x, int64_t ldx, const int8_t *q, const uint8_t *e, const void *wg,
                         int64_t ldg, const void *wu, int64_t ldu, void *dx, void *dwg, void *dwu, void *ws,
