@@ -516,7 +516,7 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
                     "neither x nor an aligned checkpoint is given");
         check_matrix(wg, ldg, inner, width);
         check_matrix(wu, ldu, inner, width);
-        require(dx || dwg || dwu, "no output is asked for");
+        require(tokens == 0 || dx || dwg || dwu, "no output is asked for");  // an empty dx has no address
         require(act >= 0 && act <= HELRM_ACT_GELU, "unknown activation");
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
@@ -695,7 +695,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         check_matrix(wt, ldw, inner, vocab);
         require(tokens == 0 || (targets && dloss && lse), "dloss, targets or lse is NULL");
         require(((uintptr_t)lse & 7) == 0, "lse is not 8-byte aligned");
-        require(dh || dw, "no output is asked for");
+        require(tokens == 0 || dh || dw, "no output is asked for");
         Workspace w{static_cast<char *>(ws)};
         Operands in(w);
         const Matrix mw = in.fit({wt, vocab, inner, ldw});

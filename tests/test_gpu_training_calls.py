@@ -1,0 +1,34 @@
+"""The training operators' calls at their edges, on a B200."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_training import DTYPES, block, give_memory_back  # noqa: E402,F401
+
+
+@pytest.fixture(scope="module")
+def tr():
+    from helrm_b200 import training
+    return training
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_an_empty_batch_of_a_frozen_block(tr, dt):
+    """No tokens, and the input's gradient alone is wanted: it is empty."""
+    dt = DTYPES[dt]
+    _, wg, wu, _ = block((1, 40, 24), dt)
+    x, dh = torch.empty(0, 40, device="cuda", dtype=dt), torch.empty(0, 24, device="cuda", dtype=dt)
+    for kept in (x, tr.pack_checkpoint(x)):
+        dx, dwg, dwu = tr.gated_backward(dh, kept, wg, wu, needs=(True, False, False))
+        assert dx.shape == (0, 40) and dwg is None and dwu is None
+    t = torch.empty(0, device="cuda", dtype=torch.int64)
+    loss, lse = tr.vocabulary_loss_forward(x, wg, t)
+    for w in (wg, torch.empty(30000, 40, device="cuda", dtype=dt), torch.empty(300, 100, device="cuda", dtype=dt)):
+        h = torch.empty(0, w.shape[1], device="cuda", dtype=dt)
+        dh, dw = tr.vocabulary_loss_backward(loss, h, w, t, lse, needs=(True, False))
+        assert dh.shape == h.shape and dw is None
+    x.requires_grad_()
+    tr.gated_feed_forward(x, wg, wu).sum().backward()
+    assert x.grad.shape == (0, 40)
