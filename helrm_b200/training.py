@@ -85,7 +85,7 @@ def _same(first, **others):
 
 
 def _activation(name: str) -> int:
-    if name not in ACTIVATIONS:
+    if not isinstance(name, str) or name not in ACTIVATIONS:
         raise ValueError(f"activation {name!r} is none of {sorted(ACTIVATIONS)}")
     return ACTIVATIONS[name]
 
@@ -132,10 +132,11 @@ class _Out:
 
 
 def _remember(key, plan):
+    if key is None:  # of something that cannot be a key, a shape in a list
+        return
     if len(_plans) > 4096:
         _plans.clear()
     _plans[key] = plan
-    return plan
 
 
 def _run(fn, like, needs, odd, *args):
@@ -272,8 +273,8 @@ def gated_feed_forward(x, w_gate, w_up, activation: str = "silu", checkpoint: bo
 
 # ------------------------------------------------------------------ 8-bit checkpoints
 def _check_checkpoint(c):
-    q, e = c.q, c.e
-    if not isinstance(q, torch.Tensor) or not isinstance(e, torch.Tensor) or len(c.shape) < 1:
+    if (not isinstance(c.q, torch.Tensor) or not isinstance(c.e, torch.Tensor) or not isinstance(c.dtype, torch.dtype)
+            or not isinstance(c.shape, (tuple, list)) or not c.shape or not all(isinstance(n, int) for n in c.shape)):
         raise ValueError("not a checkpoint that pack_checkpoint returned")
     rows = 1
     for n in c.shape[:-1]:
@@ -328,8 +329,8 @@ def unpack_checkpoint(c: Checkpoint):
     except (AttributeError, TypeError):
         key = plan = None
     if plan is None:
-        plan = _Plan((q.device.index, _DTYPES.get(dtype), _check_checkpoint(c), shape[-1]), None,
-                     _Out(shape, dtype, q.device))
+        rows = _check_checkpoint(c)
+        plan = _Plan((q.device.index, _DTYPES[dtype], rows, shape[-1]), None, _Out(shape, dtype, q.device))
         _remember(key, plan)
     x = plan.out.new()
     rc = _entry("helrm_UnpackCheckpoint")(*plan.head, q.data_ptr(), e.data_ptr(), x.data_ptr(),

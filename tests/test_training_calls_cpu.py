@@ -30,3 +30,27 @@ def test_an_empty_gradient_needs_no_address(lib):
     assert gated(3, None, None) == -1 and gated(3, p, None) == 0
     for vocab in (300, 40000):
         assert loss(0, vocab, None, None) == 0 and loss(3, vocab, None, None) == -1
+
+
+def test_what_is_no_checkpoint_is_refused():
+    """ValueError, whichever part is not what pack_checkpoint returns."""
+    from helrm_b200 import training as tr
+    q, e = torch.zeros(4, 32, dtype=torch.int8), torch.zeros(4, 1, dtype=torch.uint8)
+    good = dict(q=q, e=e, shape=(4, 8), dtype=torch.bfloat16)
+    for part in (dict(q=None), dict(q=[1, 2]), dict(q=q.numpy()), dict(e=None), dict(e=3), dict(shape=None), dict(shape=8),
+                 dict(shape=()), dict(shape=("a", 8)), dict(shape=[4, 8]), dict(dtype=None), dict(dtype=[]),
+                 dict(dtype="bf16"), dict(dtype=torch.float32)):
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                tr.unpack_checkpoint(tr.Checkpoint(**{**good, **part}))
+    assert None not in tr._plans
+
+
+def test_an_activation_that_is_no_name_is_refused():
+    from helrm_b200 import training as tr
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    for bad in ([], {}, None, 2, "tanh"):
+        with pytest.raises(ValueError):
+            tr.gated_forward(x, x, x, bad)
+        with pytest.raises(ValueError):
+            tr.gated_backward(x, x, x, x, bad)
