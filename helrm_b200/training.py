@@ -266,8 +266,12 @@ class _GatedFeedForward(torch.autograd.Function):
 
 def gated_feed_forward(x, w_gate, w_up, activation: str = "silu", checkpoint: bool = False):
     """act(x w_gate^T) * (x w_up^T), differentiable.  The backward pass needs
-    x alone; with checkpoint it keeps x in 8 bits (half the memory) and its
-    gradients are those at the values the 8 bits stand for."""
+    x alone; with checkpoint it keeps x in 8 bits (33 bytes for 32 features of a
+    row, or a part of 32: half the memory of long rows, more than all of it for
+    16 features or fewer) and its gradients are those at the values the 8 bits
+    stand for.  Where no gradient is recorded nothing is kept."""
+    if checkpoint:
+        checkpoint = torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, w_gate, w_up))
     return _GatedFeedForward.apply(x, w_gate, w_up, activation, checkpoint)
 
 

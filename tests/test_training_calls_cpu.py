@@ -54,3 +54,25 @@ def test_an_activation_that_is_no_name_is_refused():
             tr.gated_forward(x, x, x, bad)
         with pytest.raises(ValueError):
             tr.gated_backward(x, x, x, x, bad)
+
+
+def test_nothing_is_kept_where_no_gradient_is_recorded(monkeypatch):
+    """Stand-ins for the passes, since they take no tensors of the CPU."""
+    from helrm_b200 import training as tr
+    packed = []
+
+    def pack(x):
+        packed.append(x.shape)
+        return tr.Checkpoint(x.clone(), x.clone(), tuple(x.shape), x.dtype)
+    monkeypatch.setattr(tr, "pack_checkpoint", pack)
+    monkeypatch.setattr(tr, "gated_forward", lambda x, wg, wu, act: (x @ wg.T) * (x @ wu.T))
+    x, w = torch.ones(4, 8), torch.ones(6, 8)
+    assert not tr.gated_feed_forward(x, w, w, checkpoint=True).requires_grad and not packed
+    for leaf in range(3):
+        args = [t.clone().requires_grad_(i == leaf) for i, t in enumerate((x, w, w))]
+        with torch.no_grad():
+            assert not tr.gated_feed_forward(*args, checkpoint=True).requires_grad and not packed
+        with torch.inference_mode():
+            assert not tr.gated_feed_forward(*args, checkpoint=True).requires_grad and not packed
+        assert tr.gated_feed_forward(*args, checkpoint=True).requires_grad and len(packed) == 1
+        packed.clear()
