@@ -22,6 +22,7 @@ bits.  Failures raise like the backend's: ``ValueError`` for arguments,
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import NamedTuple
 
 import torch
@@ -355,6 +356,16 @@ def _targets(targets, lead, dev):
     return targets.to(torch.int64).contiguous()
 
 
+def _ignored(index) -> int:
+    try:
+        index = operator.index(index)
+    except TypeError:
+        raise ValueError(f"ignore_index {index!r} is no whole number") from None
+    if not -2 ** 63 <= index < 2 ** 63:
+        raise ValueError(f"ignore_index {index} does not fit 64 bits")
+    return index
+
+
 def _floats(t, name: str, like: _Out):
     if (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != like.device
             or t.shape != like.shape):
@@ -396,17 +407,19 @@ def vocabulary_loss_forward(h, w, targets, ignore_index: int = -100):
     the largest logit and the log of the sum relative to it.  h [..., inner],
     w [vocab, inner], targets [...].  Rows whose target is ignore_index have
     loss 0, other targets outside the vocabulary NaN."""
+    ignore_index = _ignored(ignore_index)
     h, w, t, plan = _loss_call(h, w, targets)
     loss, lse = plan.out[0].new(), plan.out[1].new()
     ph, pw = h.data_ptr(), w.data_ptr()
     _run(_entry("helrm_VocabularyLossForward"), h, plan.needs, (ph & 15, pw & 15), *plan.head, ph, plan.pitches[0], pw,
-         plan.pitches[1], t.data_ptr(), int(ignore_index), loss.data_ptr(), lse.data_ptr())
+         plan.pitches[1], t.data_ptr(), ignore_index, loss.data_ptr(), lse.data_ptr())
     return loss, lse
 
 
 def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100, needs=(True, True)):
     """(dh, dw) from dloss [...] (float32) and vocabulary_loss_forward's lse.
     needs: which of the two are wanted (None in their place)."""
+    ignore_index = _ignored(ignore_index)
     h, w, t, plan = _loss_call(h, w, targets)
     out_loss, out_lse, out_h, out_w = plan.out
     g, l = _floats(dloss, "dloss", out_loss), _floats(lse, "lse", out_lse)
@@ -416,7 +429,7 @@ def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100
         ph, pw = h.data_ptr(), w.data_ptr()
         _run(_entry("helrm_VocabularyLossBackward"), h, plan.needs, (ph & 15, pw & 15, bool(needs[0]), bool(needs[1])),
              *plan.head, g.data_ptr(), ph, plan.pitches[0], pw, plan.pitches[1], t.data_ptr(), l.data_ptr(),
-             int(ignore_index), None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr())
+             ignore_index, None if dh is None else dh.data_ptr(), None if dw is None else dw.data_ptr())
     return dh, dw
 
 
@@ -442,6 +455,7 @@ def vocabulary_cross_entropy(h, w, targets, ignore_index: int = -100, reduction:
     are not ignored, "sum", or "none"."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction {reduction!r} is none of 'mean', 'sum', 'none'")
+    ignore_index = _ignored(ignore_index)
     loss = _VocabularyLoss.apply(h, w, targets, ignore_index)
     if reduction == "none":
         return loss

@@ -76,3 +76,14 @@ def test_nothing_is_kept_where_no_gradient_is_recorded(monkeypatch):
             assert not tr.gated_feed_forward(*args, checkpoint=True).requires_grad and not packed
         assert tr.gated_feed_forward(*args, checkpoint=True).requires_grad and len(packed) == 1
         packed.clear()
+
+
+def test_an_ignore_index_that_is_no_whole_number_is_refused():
+    """A half would leave rows out of the loss and not out of its mean."""
+    from helrm_b200 import training as tr
+    x, t = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.int64)
+    for bad in (-100.5, 7.0, None, "7", 2 ** 63, -2 ** 63 - 1):
+        for call in (lambda: tr.vocabulary_loss_forward(x, x, t, bad), lambda: tr.vocabulary_cross_entropy(x, x, t, bad),
+                     lambda: tr.vocabulary_loss_backward(x, x, x, t, x, bad)):
+            with pytest.raises(ValueError, match="ignore_index"):
+                call()
