@@ -1918,14 +1918,24 @@ public:
 
 static std::unique_ptr<Context> g_ctx;
 
-// The last failure's message: a plain buffer, since a training call on
-// another thread may fail while the caller reads it.
-static char g_err[1024];
-void set_last_error(const char *msg) {
-    static std::mutex mu;
-    std::lock_guard<std::mutex> lk(mu);
-    std::strncpy(g_err, msg, sizeof(g_err) - 1);
+// The last failure's message, for each thread while its last call is the one that
+// failed (training calls fail on any thread), and for a thread without one the
+// process's: a caller whose next call runs on another thread, as a goroutine's
+// may, still finds it.
+static thread_local bool t_failed = false;
+static thread_local std::string t_err;
+static std::mutex g_err_mu;
+static std::string g_err;
+void set_last_error(const char *msg) noexcept {
+    try {
+        t_err = msg;
+        t_failed = true;
+        std::lock_guard<std::mutex> lk(g_err_mu);
+        g_err = t_err;
+    } catch (...) {  // no memory for a message
+    }
 }
+void call_succeeded() noexcept { t_failed = false; }
 
 static Context &C() {
     if (!g_ctx) HB_THROW(HB_ESTATE, "B200 backend not initialised. Call NewScheme first.");
@@ -1939,7 +1949,16 @@ using namespace hb;
 #define OUT(p) \
     if (!(p)) HB_THROW(HB_EINVAL, "null output pointer")
 
-HB_API const char *helrm_LastError(void) { return g_err; }
+HB_API const char *helrm_LastError(void) {
+    try {
+        if (!t_failed) {
+            std::lock_guard<std::mutex> lk(g_err_mu);
+            t_err = g_err;
+        }
+    } catch (...) {
+    }
+    return t_err.c_str();
+}
 
 HB_API int helrm_NewScheme(int logn, const int *logq, int nlogq, const int *logp, int nlogp, int logscale,
                            int hamming_weight, int dnum, uint64_t seed, int device) {

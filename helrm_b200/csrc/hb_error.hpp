@@ -25,13 +25,15 @@ inline void cuda_check(cudaError_t e, const char *what) {
     }
 }
 
-// Keeps the message that helrm_LastError() returns (one per process).
-void set_last_error(const char *msg);
+// Keeps the message that helrm_LastError() returns on this thread.
+void set_last_error(const char *msg) noexcept;
+void call_succeeded() noexcept;
 
 template <class F>
 int guard(F &&f) {
     try {
         f();
+        call_succeeded();
         return HB_OK;
     } catch (const HbError &e) {
         set_last_error(e.what());

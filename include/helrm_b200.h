@@ -45,7 +45,8 @@ extern "C" {
 #define HB_ENOMEM -5    /* device allocation failed (MemoryError) */
 #define HB_ENOTSUP -6   /* not implemented (NotImplementedError) */
 
-/* Message of the most recent failure ("" if none). */
+/* Message of the most recent failure ("" if none): the calling thread's, if
+ * its last call failed, else the process's.  Valid until the thread's next call. */
 const char *helrm_LastError(void);
 
 /* ---- lifecycle ---------------------------------------------------------- */

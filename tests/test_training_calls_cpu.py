@@ -87,3 +87,40 @@ def test_an_ignore_index_that_is_no_whole_number_is_refused():
                      lambda: tr.vocabulary_loss_backward(x, x, x, t, x, bad)):
             with pytest.raises(ValueError, match="ignore_index"):
                 call()
+
+
+def test_each_thread_reads_its_own_failure(lib):
+    """Two threads fail in turn, each then reads; a third one that has not failed finds the process's last."""
+    import threading
+    n = ctypes.c_size_t(0)
+
+    def fail(**kw):
+        a = dict(dtype=1, inner=40, ldx=40)
+        a.update(kw)
+        assert lib.helrm_GatedForward(0, a["dtype"], 2, 3, a["inner"], 24, 4096, a["ldx"], 4096, 40, 4096, 40, 4096, None,
+                                      ctypes.byref(n), None) == -1
+
+    turn = threading.Barrier(2)
+    got = {}
+
+    def run(name, first, **kw):
+        if not first:
+            turn.wait()
+        fail(**kw)
+        if first:
+            turn.wait()
+        turn.wait()  # both have failed
+        got[name] = lib.helrm_LastError()
+    threads = [threading.Thread(target=run, args=("dtype", True), kwargs=dict(dtype=7)),
+               threading.Thread(target=run, args=("pitch", False), kwargs=dict(ldx=3))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert b"dtype" in got["dtype"] and b"pitch" in got["pitch"]
+    other = threading.Thread(target=lambda: got.update(other=lib.helrm_LastError()))
+    other.start()
+    other.join()
+    assert b"pitch" in got["other"]
+    fail(inner=0)
+    assert b"sizes" in lib.helrm_LastError()
