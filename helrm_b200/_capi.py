@@ -137,6 +137,8 @@ SIGNATURES = {
                                    + [P(c_size), c_void],
     "helrm_VocabularyLossBackward": [c_int] * 2 + [c_i64] * 3 + [c_void] + [c_void, c_i64] * 2 + [c_void] * 2
                                     + [c_i64] + [c_void] * 3 + [P(c_size), c_void],
+    "helrm_TrainingSynchronize": [c_int, c_void],
+    "helrm_TrainingPostFailure": [c_int] * 2,
     "helrm_Synchronize": [],
     "helrm_TimerStart": [],
     "helrm_TimerStop": [P(c_double)],

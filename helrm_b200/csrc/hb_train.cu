@@ -2,6 +2,7 @@
 // entry points (include/helrm_b200.h).
 #include <atomic>
 #include <cmath>
+#include <cstring>
 #include <mutex>
 #include <type_traits>
 #include <utility>
@@ -99,10 +100,10 @@ static void check_matrix(const void *p, int64_t ld, int64_t cols, int64_t rows) 
     require(ld >= cols, "a row pitch is below the number of columns");
 }
 
-// ---- the process's state: a word of host memory that a kernel whose wait
-// ran out writes, and the driver's tensor-map encoder
+// ---- the process's state: for each device a word of host memory that a kernel
+// whose wait ran out writes, and the driver's tensor-map encoder
 struct Runtime {
-    int *error = nullptr;
+    int *errors = nullptr;
     decltype(&cuTensorMapEncodeTiled) encode = nullptr;
     std::atomic<int> sms[64] = {};
 };
@@ -119,9 +120,9 @@ static Runtime &runtime() {
             void *fn = nullptr;
             cudaDriverEntryPointQueryResult found;
             cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
-            if (e == cudaSuccess && !r.error) {
-                e = cudaHostAlloc(reinterpret_cast<void **>(&r.error), sizeof(int), cudaHostAllocPortable);
-                if (e == cudaSuccess) *r.error = 0;
+            if (e == cudaSuccess && !r.errors) {
+                e = cudaHostAlloc(reinterpret_cast<void **>(&r.errors), 64 * sizeof(int), cudaHostAllocPortable);
+                if (e == cudaSuccess) std::memset(r.errors, 0, 64 * sizeof(int));
             }
             cudaThreadExchangeStreamCaptureMode(&mode);
             cuda_check(e, "training set-up");
@@ -130,13 +131,27 @@ static Runtime &runtime() {
             ready = true;
         }
     }
-    if (const int code = *static_cast<volatile int *>(r.error)) {
-        *static_cast<volatile int *>(r.error) = 0;
-        HB_THROW(HB_ECUDA, "an earlier training call gave up waiting in its kernel (code " + std::to_string(code) +
-                               "): its results are not valid");
-    }
     return r;
 }
+// The current device's word.
+static int *error_word() {
+    int dev = 0;
+    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    return runtime().errors + (dev & 63);
+}
+// Reports a kernel of the current device that gave up waiting, once.
+static void report_earlier() {
+    int *word = error_word();
+    if (!*static_cast<volatile int *>(word)) return;
+    if (const int code = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL))
+        HB_THROW(HB_ECUDA, "an earlier training call gave up waiting in its kernel (code " + std::to_string(code) +
+                               "): its results are not valid");
+}
+// A call's device, and what its kernels before this call left.
+struct CallDevice {
+    DeviceGuard dev;
+    explicit CallDevice(int device) : dev(device) { report_earlier(); }
+};
 static int sm_count() {
     int dev = 0;
     cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
@@ -284,7 +299,7 @@ static void launch(const Product &d, cudaStream_t s) {
     constexpr int cols_n = EPI == EPI_GATED || EPI == EPI_GATED_BWD ? 128 : kCols;
     ProductArgs<1> p;
     fill(p.job[0], d, std::is_same<T, __nv_bfloat16>::value, K_MAJOR, K_MAJOR, cols_n);
-    p.error = runtime().error;
+    p.error = error_word();
     raise_shared_memory<k_mma_product<T, K_MAJOR, K_MAJOR, EPI, ACT, 1>>(kProductSmem);
     start("training product", k_mma_product<T, K_MAJOR, K_MAJOR, EPI, ACT, 1>,
           product_grid((int64_t)p.job[0].tiles_m * p.job[0].tiles_n), product_threads(EPI), kProductSmem, s, p);
@@ -378,7 +393,7 @@ static void launch_gradients(Product *d, cudaStream_t s) {
         fill(p.job[i], g, std::is_same<T, __nv_bfloat16>::value, g.amaj, MN_MAJOR, g.cols());
         items += g.tiles() * g.splits;
     }
-    p.error = runtime().error;
+    p.error = error_word();
     raise_shared_memory<k_mma_product<T, AMAJ, MN_MAJOR, EPI_OUT, 0, JOBS>>(kProductSmem);
     start("training product", k_mma_product<T, AMAJ, MN_MAJOR, EPI_OUT, 0, JOBS>, product_grid(items),
           product_threads(EPI_OUT), kProductSmem, s, p);
@@ -489,7 +504,7 @@ HB_API int helrm_GatedForward(int device, int dtype, int act, int64_t tokens, in
         d.b = in.fit({wg, width, inner, ldg});
         d.b1 = in.fit({wu, width, inner, ldu});
         if (sized(w, ws_bytes) || tokens == 0) return;
-        DeviceGuard dev(device);
+        CallDevice dev(device);
         cudaStream_t s = (cudaStream_t)stream;
         in.copy(s);
         d.M = tokens, d.N = width, d.K = inner;
@@ -550,7 +565,7 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
             grads[n++] = g;
         }
         if (sized(w, ws_bytes)) return;
-        DeviceGuard dev(device);
+        CallDevice dev(device);
         cudaStream_t s = (cudaStream_t)stream;
         if (tokens == 0) {
             for (void *p : {dwg, dwu})
@@ -607,8 +622,7 @@ HB_API int helrm_PackCheckpoint(int device, int dtype, int64_t tokens, int64_t i
         check_matrix(x, ldx, inner, tokens);
         if (tokens == 0) return;
         require(q && ex && ((uintptr_t)q & 15) == 0, "q or e is NULL, or q is not 16-byte aligned");
-        DeviceGuard dev(device);
-        runtime();
+        CallDevice dev(device);
         dim3 grid;
         const CkptPlan p = ckpt_plan(tokens, inner, fits_vectors(x, tokens > 1 ? ldx : pitch(inner)), grid);
         by_dtype(dtype, [&](auto t) {
@@ -626,8 +640,7 @@ HB_API int helrm_UnpackCheckpoint(int device, int dtype, int64_t tokens, int64_t
         require(inner <= 1 << 26, "rows of a checkpoint have at most 2^26 features");
         if (tokens == 0) return;
         require(q && ex && x && ((uintptr_t)q & 15) == 0, "q, e or x is NULL, or q is not 16-byte aligned");
-        DeviceGuard dev(device);
-        runtime();
+        CallDevice dev(device);
         by_dtype(dtype, [&](auto t) {
             typedef decltype(t) T;
             read_checkpoint<T>(q, ex, tokens, inner, static_cast<T *>(x), inner, (cudaStream_t)stream);
@@ -656,7 +669,7 @@ HB_API int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, in
         float2 *part = w.take<float2>(parts * piece), *few = w.take<float2>(joined * piece);
         float *at = w.take<float>(piece);
         if (sized(w, ws_bytes) || tokens == 0) return;
-        DeviceGuard dev(device);
+        CallDevice dev(device);
         cudaStream_t s = (cudaStream_t)stream;
         in.copy(s);
         for (int64_t m0 = 0; m0 < tokens; m0 += piece) {
@@ -722,7 +735,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             float *acc = w.take<float>(groups > 1 ? vocab * nr.depth : 0);
             void *dws = dw ? dw : w.take<uint16_t>(vocab * inner);
             if (sized(w, ws_bytes)) return;
-            DeviceGuard dev(device);
+            CallDevice dev(device);
             cudaStream_t s = (cudaStream_t)stream;
             if (tokens == 0) {
                 if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
@@ -743,7 +756,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 a.dw = dws;
                 a.acc_w = acc;
                 a.part_h = part;
-                a.error = runtime().error;
+                a.error = error_word();
                 raise_shared_memory<k_loss_grads_narrow<T>>(kNarrowSmem);
                 start("loss gradients", k_loss_grads_narrow<T>, nr.grid, kNarrowThreads, kNarrowSmem, s, a);
                 if (dh) join<T>({part, nr.grid, cap, tokens, inner, nr.depth, &plan->unscale, pos}, dh, s);
@@ -766,7 +779,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
         float *acc = w.take<float>(dh ? gh.splits * cap * lda : 0);
         float *acc_w = w.take<float>(dw ? gw.sums() : 0);
         if (sized(w, ws_bytes)) return;
-        DeviceGuard dev(device);
+        CallDevice dev(device);
         cudaStream_t s = (cudaStream_t)stream;
         if (tokens == 0) {
             if (dw) cuda_check(cudaMemsetAsync(dw, 0, (size_t)vocab * inner * 2, s), "zero gradient");
@@ -820,5 +833,20 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
             }
             if (dh) join<T>({acc, gh.splits, cap, tokens, inner, lda, &plan->unscale, pos}, dh, s);
         });
+    });
+}
+
+HB_API int helrm_TrainingSynchronize(int device, void *stream) {
+    return guard([&] {
+        DeviceGuard dev(device);
+        cuda_check(cudaStreamSynchronize((cudaStream_t)stream), "training call");
+        report_earlier();
+    });
+}
+HB_API int helrm_TrainingPostFailure(int device, int code) {
+    return guard([&] {
+        require(code > 0, "a kernel's code is above 0");
+        DeviceGuard dev(device);
+        __atomic_store_n(error_word(), code, __ATOMIC_RELEASE);
     });
 }

@@ -15,8 +15,8 @@ Each is differentiable; the ``*_forward`` / ``*_backward`` functions under
 them are the single passes.  Tensors are 16-bit floats (``torch.float16`` or
 ``torch.bfloat16``, one type per call) of one CUDA device, any leading
 dimensions; work goes to the device's current torch stream, workspaces come
-from torch's allocator, and nothing synchronises.  Losses and sums are in 32
-bits.  Failures raise like the backend's: ``ValueError`` for arguments,
+from torch's allocator, and nothing but :func:`synchronize` waits.  Losses and
+sums are in 32 bits.  Failures raise like the backend's: ``ValueError`` for arguments,
 ``RuntimeError`` for CUDA.
 """
 from __future__ import annotations
@@ -155,6 +155,16 @@ def _run(fn, like, needs, odd, *args):
         rc = fn(*args, 256, _NOTHING, _stream(args[0]))
     if rc:
         _capi.check(rc)
+
+
+def synchronize(device=None):
+    """Waits for the current stream of the device (the current one).  Raises
+    RuntimeError if a kernel of a call since the last report gave up waiting (a
+    hardware failure), as the next call on that device would; a program's last
+    call has no next one."""
+    with torch.cuda.device(device):
+        index = torch.cuda.current_device()
+    _capi.check(_entry("helrm_TrainingSynchronize")(index, _stream(index)))
 
 
 # ------------------------------------------------------------------ the gated block

@@ -346,8 +346,9 @@ int helrm_Synchronize(void);
  *     otherwise ws points to *ws_bytes of it, 256-byte aligned.  It holds
  *     nothing between calls; calls whose GPU work overlaps need one each;
  *   - tokens may be 0 (weight gradients are then zero), other sizes are >= 1;
- *     a call whose kernel gave up waiting (a hardware failure) makes the next
- *     training call on any stream return HB_ECUDA. */
+ *     a kernel that gave up waiting (a hardware failure; its results are not
+ *     valid) makes the next training call on its device return HB_ECUDA, once,
+ *     or helrm_TrainingSynchronize where no other call follows. */
 #define HELRM_FP16 0
 #define HELRM_BF16 1
 #define HELRM_ACT_IDENTITY 0
@@ -400,6 +401,12 @@ int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, int64_t 
                                  const float *dloss, const void *h, int64_t ldh, const void *w, int64_t ldw,
                                  const int64_t *targets, const float *lse, int64_t ignore_index, void *dh, void *dw,
                                  void *ws, size_t *ws_bytes, void *stream);
+
+/* Waits for the stream; HB_ECUDA if a kernel of a training call gave up
+ * waiting on this device since the last report. */
+int helrm_TrainingSynchronize(int device, void *stream);
+/* For tests of that report: leaves what such a kernel would (code > 0). */
+int helrm_TrainingPostFailure(int device, int code);
 
 /* ---- measurement (no reference counterpart; the reference times with
  * torch.cuda.synchronize + wall clock, examples/criteo/bench_sweep.py:192-222) -- */

@@ -32,3 +32,40 @@ def test_an_empty_batch_of_a_frozen_block(tr, dt):
     x.requires_grad_()
     tr.gated_feed_forward(x, wg, wu).sum().backward()
     assert x.grad.shape == (0, 40)
+
+
+def post(code):
+    from helrm_b200 import _capi
+    return _capi.load().helrm_TrainingPostFailure(0, code)
+
+
+def test_a_kernel_that_gave_up_is_reported_once(tr):
+    """By the next call or, after the last one, by synchronize.  The host leaves the word that the kernel would."""
+    x, wg, wu, dh = block((10, 40, 24), torch.bfloat16)
+    t = torch.zeros(10, dtype=torch.int64, device="cuda")
+    tr.synchronize()
+    loss, lse = tr.vocabulary_loss_forward(x, wg, t)
+    c = tr.pack_checkpoint(x)
+    for call in (lambda: tr.gated_forward(x, wg, wu), lambda: tr.gated_backward(dh, x, wg, wu),
+                 lambda: tr.pack_checkpoint(x), lambda: tr.unpack_checkpoint(c),
+                 lambda: tr.vocabulary_loss_forward(x, wg, t), lambda: tr.vocabulary_loss_backward(loss, x, wg, t, lse),
+                 tr.synchronize, lambda: tr.synchronize(0), lambda: tr.synchronize("cuda:0")):
+        assert post(4) == 0
+        with pytest.raises(RuntimeError, match="gave up waiting .*code 4"):
+            call()
+        call()
+        tr.synchronize()
+    assert post(0) == -1 and post(-1) == -1
+    tr.synchronize()
+
+
+def test_synchronize_waits_for_its_stream(tr):
+    x, wg, wu, _ = block((4096, 1024, 2048), torch.bfloat16)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(50):
+            tr.gated_forward(x, wg, wu)
+        done = s.record_event()
+        tr.synchronize()
+        assert done.query()

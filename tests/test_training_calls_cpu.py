@@ -124,3 +124,10 @@ def test_each_thread_reads_its_own_failure(lib):
     assert b"pitch" in got["other"]
     fail(inner=0)
     assert b"sizes" in lib.helrm_LastError()
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="what a host without a GPU answers")
+def test_no_device_is_an_error_code(lib):
+    assert lib.helrm_TrainingSynchronize(0, None) < 0 and lib.helrm_LastError()
+    assert lib.helrm_TrainingPostFailure(0, 4) < 0
+    assert lib.helrm_TrainingPostFailure(0, 0) == -1
