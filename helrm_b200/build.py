@@ -17,7 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhelrm_b200.so")
 SOURCES = ["hb_kernels.cu", "hb_context.cu", "hb_host.cpp", "hb_train.cu"]
 HEADERS = ["hb_arith.cuh", "hb_kernels.cuh", "hb_bsgs.cuh", "hb_bsgs_tc.cuh", "hb_host.hpp", "hb_error.hpp",
-           "hb_ptx.cuh", "hb_train.cuh", "hb_train_mma.cuh", "hb_train_loss.cuh"]
+           "hb_ptx.cuh", "hb_schedule.hpp", "hb_train.cuh", "hb_train_mma.cuh", "hb_train_loss.cuh"]
 
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -34,6 +34,7 @@
 #include <cuda.h>
 
 #include "hb_ptx.cuh"
+#include "hb_schedule.hpp"
 
 namespace hb {
 namespace train {
@@ -343,9 +344,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     after_previous();
 
     constexpr bool kOut = EPI == EPI_OUT, kTwo = JOBS == 2;
-    // A job's shape, with the rows that take part.  The launch has fewer than
-    // 2^31 items, so that all of this is 32-bit arithmetic: 64-bit divisions
-    // cost an epilogue warp more than 32 columns.
+    // A job's shape, with the rows that take part.
     struct Shape {
         unsigned tiles_m, tiles, items;
         int kb, depth;
@@ -370,35 +369,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     Shape s1 = {};
     if (kTwo) s1 = shape(p.job[JOBS - 1]);
     const unsigned cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
-    constexpr unsigned kNoItem = 0xffffffffu;
-    // The k-th item of this cluster, the second job's numbered after the first's.
-    // The first job's items are the longer ones and go round first; clusters that
-    // its last round leaves out take the second job's until that round ends.
     auto nth = [&](unsigned k) -> unsigned {
-        if (!kTwo) {
-            const unsigned i = cluster + k * clusters;
-            return i < s0.items ? i : kNoItem;
-        }
-        const unsigned rounds = s0.items / clusters, rest = s0.items - rounds * clusters;
-        const unsigned own = rounds + (cluster < rest);
-        if (k < own) return k * clusters + cluster;
-        k -= own;
-        unsigned ahead = 0, beside = 0;
-        if (rest) {
-            const unsigned c0 = s0.depth / p.job[0].splits + 2, c1 = s1.depth / p.job[JOBS - 1].splits + 2;
-            beside = (c0 + c1 - 1) / c1;
-            ahead = beside * (clusters - rest);
-        }
-        const unsigned i = rest && cluster >= rest && k < beside
-                               ? k * (clusters - rest) + cluster - rest
-                               : ahead + (k - (rest && cluster >= rest ? beside : 0)) * clusters + cluster;
-        return i < s1.items ? s0.items + i : kNoItem;
+        if (!kTwo) return nth_of_one(k, cluster, clusters, s0.items);
+        return nth_of_two(k, cluster, clusters, s0.items, s0.depth / p.job[0].splits + 2, s1.items,
+                          s1.depth / p.job[JOBS - 1].splits + 2);
     };
     struct Item {
         int job, out, split, mt, nt, k0, k1;
     };
-    // Tiles go down groups of 8 tile rows, column after column, so that the
-    // clusters at work share a few panels of A and of B in L2.
     auto item = [&](unsigned i) {
         Item t;
         t.job = kTwo && i >= s0.items;
@@ -412,18 +390,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
             i -= q * h.tiles;
             t.out = q / j.splits;
             t.split = q - t.out * j.splits;
-            t.k0 = (int)((int64_t)h.depth * t.split / j.splits);
-            t.k1 = (int)((int64_t)h.depth * (t.split + 1) / j.splits);
+            part_of(h.depth, t.split, j.splits, t.k0, t.k1);
         }
-        const unsigned per = 8u * j.tiles_n, g = h.tiles_m > 8 ? i / per : 0;
-        const unsigned r = i - g * per, rows = h.tiles_m - g * 8;
-        if (rows >= 8) {
-            t.mt = g * 8 + (r & 7);
-            t.nt = r >> 3;
-        } else {
-            t.nt = r / rows;
-            t.mt = g * 8 + (r - t.nt * rows);
-        }
+        tile_at(i, h.tiles_m, j.tiles_n, t.mt, t.nt);
         return t;
     };
 
