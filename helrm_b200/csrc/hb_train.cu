@@ -133,13 +133,9 @@ static Runtime &runtime() {
     }
     return r;
 }
-// The current device's word.
-static int *error_word() {
-    int dev = 0;
-    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-    return runtime().errors + (dev & 63);
-}
-// Reports a kernel of the current device that gave up waiting, once.
+static thread_local int t_device = 0;  // of the call that this thread is in
+static int *error_word() { return runtime().errors + (t_device & 63); }
+// Reports a kernel of the call's device that gave up waiting, once.
 static void report_earlier() {
     int *word = error_word();
     if (!*static_cast<volatile int *>(word)) return;
@@ -147,18 +143,19 @@ static void report_earlier() {
         HB_THROW(HB_ECUDA, "an earlier training call gave up waiting in its kernel (code " + std::to_string(code) +
                                "): its results are not valid");
 }
-// A call's device, and what its kernels before this call left.
+// Makes a call's device current, and reports what its kernels before this call left.
 struct CallDevice {
     DeviceGuard dev;
-    explicit CallDevice(int device) : dev(device) { report_earlier(); }
+    explicit CallDevice(int device, bool report = true) : dev(device) {
+        t_device = device;
+        if (report) report_earlier();
+    }
 };
 static int sm_count() {
-    int dev = 0;
-    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
-    std::atomic<int> &known = runtime().sms[dev & 63];
+    std::atomic<int> &known = runtime().sms[t_device & 63];
     int n = known;
     if (!n) {
-        cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev), "SM count");
+        cuda_check(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, t_device), "SM count");
         known = n;
     }
     return n;
@@ -168,8 +165,7 @@ static int sm_count() {
 template <auto KERNEL>
 static void raise_shared_memory(int bytes) {
     static std::atomic<uint64_t> set{0};
-    int dev = 0;
-    cuda_check(cudaGetDevice(&dev), "cudaGetDevice");
+    const int dev = t_device;
     if (set >> (dev & 63) & 1) return;
     cuda_check(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), "shared memory");
     set |= (uint64_t)1 << (dev & 63);
@@ -838,7 +834,7 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
 
 HB_API int helrm_TrainingSynchronize(int device, void *stream) {
     return guard([&] {
-        DeviceGuard dev(device);
+        CallDevice dev(device, false);
         cuda_check(cudaStreamSynchronize((cudaStream_t)stream), "training call");
         report_earlier();
     });
@@ -846,7 +842,7 @@ HB_API int helrm_TrainingSynchronize(int device, void *stream) {
 HB_API int helrm_TrainingPostFailure(int device, int code) {
     return guard([&] {
         require(code > 0, "a kernel's code is above 0");
-        DeviceGuard dev(device);
+        CallDevice dev(device, false);
         __atomic_store_n(error_word(), code, __ATOMIC_RELEASE);
     });
 }
