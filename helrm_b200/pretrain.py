@@ -1,15 +1,16 @@
 """Train a small gated model in the clear, then evaluate it on ciphertexts.
 
-    python -m helrm_b200.pretrain [--steps 200] [--rows 4096] [--width 64] [--vocab 1000]
+    python -m helrm_b200.pretrain [--steps 200] [--rows 4096] [--width 64] [--vocab 1000] [--checkpoint]
 
 The model predicts one categorical field from the 13 dense features: a gated
 feed-forward block with the identity activation, then a row of weights for
 every category, trained with the softmax cross entropy over the vocabulary
-(:mod:`helrm_b200.training`; the block keeps its input in 8 bits for the
-backward pass).  What was trained needs nothing a ciphertext cannot do: two
-linear transforms, one ciphertext product and a third transform, three
-levels.  The trained weights go to the backend's linear layers and a few
-queries are answered encrypted and compared with the clear model's logits.
+(:mod:`helrm_b200.training`; with --checkpoint the block keeps its input in 8
+bits for the backward pass, which pays for more features than these).  What
+was trained needs nothing a ciphertext cannot do: two linear transforms, one
+ciphertext product and a third transform, three levels.  The trained weights
+go to the backend's linear layers and a few queries are answered encrypted and
+compared with the clear model's logits.
 
 Data are synthetic: log1p(lognormal) features, categories drawn from a
 random model of the same form.
@@ -40,7 +41,8 @@ def make_data(rows: int, vocab: int, seed: int):
     return x, (logits + gumbel).argmax(1)
 
 
-def train(steps: int = 200, rows: int = 4096, width: int = 64, vocab: int = 1000, seed: int = 0, report=None):
+def train(steps: int = 200, rows: int = 4096, width: int = 64, vocab: int = 1000, seed: int = 0, report=None,
+          checkpoint: bool = False):
     """The trained weights (w_gate, w_up [width, 13], w_out [vocab, width],
     bfloat16) and the loss of every step."""
     import torch
@@ -57,7 +59,7 @@ def train(steps: int = 200, rows: int = 4096, width: int = 64, vocab: int = 1000
     losses = []
     for i in range(steps):
         w_gate, w_up, w_out = (p.to(torch.bfloat16) for p in master)  # gradients come back to the 32-bit weights
-        h = training.gated_feed_forward(x, w_gate, w_up, "identity", checkpoint=True)
+        h = training.gated_feed_forward(x, w_gate, w_up, "identity", checkpoint=checkpoint)
         loss = training.vocabulary_cross_entropy(h, w_out, y)
         opt.zero_grad(set_to_none=True)
         loss.backward()
@@ -121,6 +123,9 @@ def main(argv=None) -> dict:
     ap.add_argument("--width", type=int, default=64)
     ap.add_argument("--vocab", type=int, default=1000)
     ap.add_argument("--queries", type=int, default=4)
+    ap.add_argument("--checkpoint", action="store_true",
+                    help="keep the block's input in 8 bits for the backward pass (a row of 13 features takes 33 bytes "
+                         "then instead of 26; of 17 or more, less)")
     a = ap.parse_args(argv)
     slots = 1 << (CKKS.logn - 1)
     if not 1 <= a.vocab <= slots or not 1 <= a.width <= slots:
@@ -131,7 +136,7 @@ def main(argv=None) -> dict:
 
     from . import training
 
-    weights, losses = train(a.steps, a.rows, a.width, a.vocab, report=print)
+    weights, losses = train(a.steps, a.rows, a.width, a.vocab, report=print, checkpoint=a.checkpoint)
     x = torch.tensor(make_data(a.queries, a.vocab, seed=99)[0], device="cuda").to(torch.bfloat16)
     h = training.gated_forward(x, weights["w_gate"], weights["w_up"], "identity")
     clear = (h.double() @ weights["w_out"].double().T).cpu().numpy()
