@@ -20,16 +20,19 @@
 // out among the warps of a quadrant.
 //
 // What bounds it: long products the tensor pipe at the clock the power cap
-// leaves (gated forward of 8192 x 4096 x 4096 in 342 us, 1.61 PFLOP/s, the pipe
-// active 95 % of the time; its dX 350 us, its weights' gradients 366), short
-// ones, at full clock, the 64 bytes a clock and SM that a tile wants from L2 (dG
-// and dU of 4096 x 1024 x 4096 in 63 us, 8.6 TB/s), and products of a few
-// features their epilogue (the loss's exponentials: 72 % of the special-function
-// pipe at 16 features).
+// leaves (gated forward of 8192 x 4096 x 4096 in 341 us, 1.61 PFLOP/s at 1.54
+// GHz, the pipe active 90 % of the time; its dX 348 us, its weights' gradients
+// 365).  Short ones what does not follow the depth: dG and dU of 4096 x K x 4096
+// take 107, 169 and 294 thousand clocks at K = 1024, 2048 and 4096 with GELU, 91,
+// 154 and 279 with the identity, so 62 for each 1024 of depth (558 a slice, of
+// which the tensor pipe needs 512) and beside that 44 or 29, some 6 or 4 thousand
+// a tile and SM pair with launch and tail, that no products hide.  Products of a
+// few features their epilogue (the loss's exponentials: 72 % of the
+// special-function pipe at 16 features).
 //
 // Every wait is bounded: when one runs out, the block stops taking work,
 // waits for what it has in flight, frees its tensor memory and leaves a word
-// in host memory that the next training call reports.
+// in host memory that the next training call on the device reports.
 #pragma once
 #include <cuda.h>
 

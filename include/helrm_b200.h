@@ -395,8 +395,9 @@ int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, int64_t i
                                 float *loss, float *lse, void *ws, size_t *ws_bytes, void *stream);
 /* dh [tokens][inner] and dw [vocab][inner] from dloss [tokens] and the
  * forward call's lse.  The vocabulary is taken in pieces, whose logits are
- * formed again; ignored rows take no part, rows with a target out of range
- * give NaN.  An output that is NULL is not computed. */
+ * formed again; the gradient by them is rounded to the 16-bit type once, as an
+ * operand of the products with w and h, relative to the largest |dloss|;
+ * ignored rows take no part, rows with a target out of range give NaN.  An output that is NULL is not computed. */
 int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, int64_t inner, int64_t vocab,
                                  const float *dloss, const void *h, int64_t ldh, const void *w, int64_t ldw,
                                  const int64_t *targets, const float *lse, int64_t ignore_index, void *dh, void *dw,

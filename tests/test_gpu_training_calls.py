@@ -69,3 +69,24 @@ def test_synchronize_waits_for_its_stream(tr):
         done = s.record_event()
         tr.synchronize()
         assert done.query()
+
+
+def test_transforms_without_a_rule_are_refused(tr):
+    """Forward-mode derivatives and vmap have no rule here: they raise, and nothing comes back without its tangent."""
+    x, wg, wu, _ = block((10, 40, 24), torch.bfloat16)
+    w = torch.zeros(30, 24, dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(10, dtype=torch.int64, device="cuda")
+    h = tr.gated_forward(x, wg, wu)
+    for f, a in ((lambda v: tr.gated_feed_forward(v, wg, wu), x), (lambda v: tr.gated_feed_forward(v, wg, wu, checkpoint=True), x),
+                 (lambda v: tr.vocabulary_cross_entropy(v, w, t), h)):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            torch.func.jvp(f, (a,), (torch.ones_like(a),))
+    for f, a in ((lambda v: tr.gated_feed_forward(v, wg, wu), x), (lambda v: tr.vocabulary_cross_entropy(v, w, t[:1]), h)):
+        with pytest.raises((RuntimeError, NotImplementedError, ValueError)):
+            torch.func.vmap(f)(a[:, None])
+    # once differentiable: a second derivative raises
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(tr.gated_feed_forward(leaf, wg, wu).float().sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), leaf)
+    torch.cuda.synchronize()
