@@ -798,6 +798,9 @@ HB_API int helrm_VocabularyLossBackward(int device, int dtype, int64_t tokens, i
                 d.e.src = src;
                 d.e.lse = reinterpret_cast<const float2 *>(lse);
                 d.e.col0 = c0;
+                    if (inner > kChunk * kDepth)
+                    launch<T, EPI_Z_LONG, 0>(d, s);
+                else
                     launch<T, EPI_Z, 0>(d, s);
                 Product piece[2];
                 int np = 0;

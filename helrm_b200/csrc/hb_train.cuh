@@ -149,7 +149,7 @@ __device__ __forceinline__ void act_df(float g, float &a, float &d) {
 }
 
 // ---------------------------------------------------------------- products
-enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_OUT, EPI_LSE, EPI_LSE_LONG, EPI_Z };
+enum Epi { EPI_GATED, EPI_GATED_BWD, EPI_OUT, EPI_LSE, EPI_LSE_LONG, EPI_Z, EPI_Z_LONG };
 struct EpiArgs {
     void *o0 = nullptr, *o1 = nullptr;  // 16-bit outputs
     int64_t ldo = 0;                    // their row pitch, or that of acc

@@ -56,17 +56,17 @@ constexpr int kProductSmem = 2 * kStages * kOperand + kStageOut + 8 * kBarriers 
 __host__ __device__ constexpr int epi_warps(int epi) { return epi == EPI_LSE || epi == EPI_Z ? 16 : 8; }
 __host__ __device__ constexpr int product_threads(int epi) { return 128 + 32 * epi_warps(epi); }
 // The tensor cores cut a running sum towards zero at every 16-deep step, by half
-// a unit in its last place on average: a row's largest logit came out 0.5e-6 of
-// itself short at 512 features and 3.9e-6 at 4096, always to the same side.  So
-// a loss over more than kChunk slices (512 features) accumulates that many at a
-// time and adds the parts, rounded to nearest, in its epilogue's registers
-// (EPI_LSE_LONG): what is lost stays at the first figure for any depth, the loss
-// within 1.6e-7 of itself (8192 x 4096 x 131072: 1.5e-6 in one sum).  An
-// accumulator goes back as soon as it is read, so the additions and the
-// exponentials run under the products to come; reading it takes tensor memory's
-// time.  4096 x 2048 x 37888: 460 us in one sum, 469 in parts of 1024 (loss
-// within 3.4e-7), 488 in parts of 512, 525 in parts of 256 (0.9e-7).
-constexpr int kChunk = 8;
+// a unit in its last place on average: a row's largest logit comes out 0.5e-6 of
+// itself short at 512 features, 1.0e-6 at 1024 and would 3.9e-6 at 4096, always
+// to the same side.  So a loss over more than kChunk slices (1024 features)
+// accumulates that many at a time and adds the parts, rounded to nearest, in its
+// epilogue's registers (EPI_LSE_LONG, and EPI_Z_LONG, whose logits have to be the
+// forward pass's): what is lost stays at the second figure for any depth, the
+// loss within 3.5e-7 of itself (8192 x 4096 x 131072: 1.5e-6 in one sum).
+// Reading an accumulator holds the tensor pipe up by some 500 clocks: forward of
+// 4096 x 4096 x 18944 579,000 clocks in one sum, 653,000 in parts of 512 features
+// (loss within 1.6e-7), half of that difference in parts of 1024.
+constexpr int kChunk = 16;
 constexpr unsigned long long kWaitNs = 4000000000ull;
 
 enum { K_MAJOR = 0, MN_MAJOR = 1 };
@@ -301,7 +301,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
     k_mma_product(const __grid_constant__ ProductArgs<JOBS> p) {
     constexpr bool kDual = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
     constexpr int kWarps = epi_warps(EPI), kSets = kWarps / 8;
-    constexpr bool kLong = EPI == EPI_LSE_LONG, kScaled = EPI == EPI_GATED_BWD && std::is_same<T, __half>::value;
+    constexpr bool kLse = EPI == EPI_LSE || EPI == EPI_LSE_LONG, kZ = EPI == EPI_Z || EPI == EPI_Z_LONG;
+    constexpr bool kLong = EPI == EPI_LSE_LONG || EPI == EPI_Z_LONG, kScaled = EPI == EPI_GATED_BWD && std::is_same<T, __half>::value;
     extern __shared__ __align__(1024) unsigned char smem[];
     unsigned char *stage = smem + 2 * kStages * kOperand;
     uint64_t *bars = reinterpret_cast<uint64_t *>(stage + kStageOut);
@@ -521,12 +522,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
         Item next = {};
         auto fetch = [&] {
             next = item(following);
-            if (EPI != EPI_LSE && !kLong && EPI != EPI_Z) return;
+            if (!kLse && !kZ) return;
             const EpiArgs &e = p.job[0].e;
             const int64_t M = s0.M;
             const int64_t m = (int64_t)next.mt * kRows + 128 * rank + 32 * quad + lane;
-            if (EPI == EPI_LSE || kLong) next_target = m < M ? e.target[m] : -1;
-            if (EPI == EPI_Z && m < M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
+            if (kLse) next_target = m < M ? e.target[m] : -1;
+            if (kZ && m < M) *reinterpret_cast<float4 *>(&next_row) = reinterpret_cast<const float4 *>(e.rows)[m];
         };
         if (following != kNoItem) fetch();
         while (following != kNoItem) {
@@ -547,6 +548,32 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                 tc::fence_before();
                 __syncwarp();
                 if (lane == 0) ptx::arrive_cluster(bar_empty + 8 * buf);
+            };
+            // kLong: this warp's 128 columns summed over the parts of the depth
+            auto logits = [&](float (&v)[4][32], const Item &t) {
+                for (int k = t.k0; k < t.k1; k += kChunk, use++) {
+                    const unsigned b = use & 1, from = tmem + ((unsigned)(32 * quad) << 16) + b * kCols + half * 128;
+                    if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (use >> 1) & 1, s_abort, s_error, 4))) return false;
+                    tc::fence_after();
+                    if (k == t.k0) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            ptx::load32(from + c * 32, v[c]);
+                            ptx::wait32(v[c]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 8; c++) {
+                            float x[16];
+                            ptx::load16(from + c * 16, x);
+                            ptx::wait16(x);
+#pragma unroll
+                            for (int j = 0; j < 16; j++) v[c / 2][c % 2 * 16 + j] += x[j];
+                        }
+                    }
+                    release(b);
+                }
+                return true;
             };
             if constexpr (!kLong) {
                 if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * buf, (unsigned)((buf_use >> 1) & 1), s_abort, s_error,
@@ -620,7 +647,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                         store_sums(st, v, o, e.ldo, m0, M, n0 + col, !e.first, lane);
                     }
                 }
-            } else if constexpr (EPI == EPI_LSE || kLong) {
+            } else if constexpr (kLse) {
                 constexpr int kWide = kCols / 2;  // columns a warp
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 // columns of the vocabulary here, and which of them is the row's target: looked at once a tile, since
@@ -669,32 +696,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     top = mx;
                 };
                 if constexpr (kLong) {
-                    float v[kWide / 32][32];
-                    bool ok = true;
-                    for (int k = t.k0; k < t.k1; k += kChunk, use++) {
-                        const unsigned b = use & 1, from = tmem + ((unsigned)(32 * quad) << 16) + b * kCols + half * kWide;
-                        if (!(ok = __all_sync(0xffffffffu, mbar_wait(tfull + 8 * b, (use >> 1) & 1, s_abort, s_error, 4))))
-                            break;
-                        tc::fence_after();
-                        if (k == t.k0) {
-#pragma unroll
-                            for (int c = 0; c < kWide / 32; c++) {
-                                ptx::load32(from + c * 32, v[c]);
-                                ptx::wait32(v[c]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int c = 0; c < kWide / 16; c++) {
-                                float x[16];
-                                ptx::load16(from + c * 16, x);
-                                ptx::wait16(x);
-#pragma unroll
-                                for (int j = 0; j < 16; j++) v[c / 2][c % 2 * 16 + j] += x[j];
-                            }
-                        }
-                        release(b);
-                    }
-                    if (!ok) break;
+                    float v[4][32];
+                    if (!logits(v, t)) break;
 #pragma unroll
                     for (int c = 0; c < kWide / 32; c++) take(v[c], c);
                 } else {
@@ -708,21 +711,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(product_threads(EPI)
                     }
                 }
                 if (m < M) e.part[((int64_t)t.nt * 2 + half) * job.M + m] = make_float2(top, sum);
-            } else if constexpr (EPI == EPI_Z) {
+            } else if constexpr (kZ) {
                 constexpr int kWide = kCols / 2;
                 const int64_t n0 = (int64_t)t.nt * kCols + half * kWide;
                 const int col0 = (int)(e.col0 + n0);
                 const bool any = __any_sync(0xffffffffu, row.target >= col0 && row.target < col0 + kWide);
-#pragma unroll 1
-                for (int c = 0; c < kWide / 32; c++) {
-                    float v[32];
+                auto put = [&](float (&v)[32], int c) {
+                    if (n0 + c * 32 >= N) return;
                     unsigned w[16];
-                    ptx::load32(acc + half * kWide + c * 32, v);
-                    ptx::wait32(v);
-                    if (c == kWide / 32 - 1) release(buf);
-                    if (n0 + c * 32 >= N) continue;
                     loss_z<T>(v, w, row, col0 + c * 32, 32, any, e.lse, e.src, m);
                     store_block<T>(st, w, static_cast<T *>(e.o0), e.ldo, m0, M, n0 + c * 32, N, e.vec & 1, lane);
+                };
+                if constexpr (kLong) {
+                    float v[4][32];
+                    if (!logits(v, t)) break;
+#pragma unroll
+                    for (int c = 0; c < kWide / 32; c++) put(v[c], c);
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < kWide / 32; c++) {
+                        float v[32];
+                        ptx::load32(acc + half * kWide + c * 32, v);
+                        ptx::wait32(v);
+                        if (c == kWide / 32 - 1) release(buf);
+                        put(v, c);
+                    }
                 }
             }
         }

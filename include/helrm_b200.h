@@ -388,7 +388,7 @@ int helrm_UnpackCheckpoint(int device, int dtype, int64_t tokens, int64_t inner,
  * equal to ignore_index has loss 0; any other one outside [0, vocab) has
  * loss NaN.  lse [tokens][2] holds lse_i as a sum: the row's largest logit and
  * the log of the sum of exponentials relative to it.  Logits are 32-bit sums
- * over at most 512 features, each step of 16 cut towards zero, and those sums
+ * over at most 1024 features, each step of 16 cut towards zero, and those sums
  * added with rounding. */
 int helrm_VocabularyLossForward(int device, int dtype, int64_t tokens, int64_t inner, int64_t vocab, const void *h,
                                 int64_t ldh, const void *w, int64_t ldw, const int64_t *targets, int64_t ignore_index,
