@@ -200,12 +200,13 @@ __device__ __forceinline__ void store8(unsigned short *row, int64_t col, int64_t
 // with the norms of rows (Cauchy and Schwarz; |act'| <= 1.13, |act(g)| <= |g|).
 // Values down to 2^-28 of the bound keep all their bits.  dH and rows that are not
 // finite have no say.  bf16 has a float's range and no scale.  It reads what the
-// next kernel will read (58 MB of 4096 x 1024 x 4096 in 17 us of the call's 190,
-// 1.5 MB of 64 x 432 x 512 in 2.5 of 24; with 148 blocks 18 and 2.5).
-// Long rows go in segments; a squared norm is at most their number times the
-// largest segment's.  A warp takes a segment, or eight rows of at most 256
+// next kernel will read: 64 x 432 x 512 22.6 us without this kernel and 25.1 with
+// it, 2047 x 1001 x 1500 58.6 and 64.9, 4096 x 1024 x 4096 (58 MB, in 16 us) 176
+// and 191.
+// Long rows go in segments (dH's of one batch of loads); a squared norm is at most
+// their number times the largest segment's.  A warp takes a segment, or eight rows of at most 256
 // columns, with its loads in flight together.
-constexpr int kRangeBlocks = 2 * 148, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32, kRangeSegment = 8192;
+constexpr int kRangeBlocks = 2 * 148, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32, kRangeSegment = 8192, kRangeBatch = 2048;
 struct GatedRange {
     const unsigned short *p[4];  // dH, x, wg, wu; rows on 16-byte boundaries but for dH's (vec)
     int64_t ld[4], rows[4], cols[4], segments[4];
@@ -259,12 +260,13 @@ __global__ void __launch_bounds__(kRangeThreads) k_gated_range(const __grid_cons
                     keep(s);
                 }
             } else {
-                const int64_t r = t / p.segments[k], c0 = (t - r * p.segments[k]) * kRangeSegment;
+                const unsigned segments = (unsigned)p.segments[k], size = norm ? kRangeSegment : kRangeBatch;
+                const int64_t r = segments == 1 ? t : rows == 1 ? 0 : t / segments, c0 = (t - r * segments) * size;
                 const unsigned short *in = p.p[k] + r * ld + c0;
-                const int n = (int)(cols - c0 < kRangeSegment ? cols - c0 : kRangeSegment), whole = n / 8 * 8;
+                const int n = (int)(cols - c0 < size ? cols - c0 : size), whole = n / 8 * 8;
                 const unsigned short last = whole + lane < n ? in[whole + lane] : (unsigned short)0;
                 float s = 0.0f;
-                for (int c = lane * 8; c < whole; c += 8 * 256) {
+                for (int c = lane * 8; c < whole; c += kRangeBatch) {
                     uint4 v[8];
 #pragma unroll
                     for (int j = 0; j < 8; j++)
@@ -277,9 +279,9 @@ __global__ void __launch_bounds__(kRangeThreads) k_gated_range(const __grid_cons
             }
         } else {  // dH's rows on any boundary
             const bool narrow = cols <= 256;
-            const int64_t r0 = narrow ? t * 8 : t / p.segments[0], c0 = narrow ? 0 : (t - r0 * p.segments[0]) * kRangeSegment;
+            const int64_t r0 = narrow ? t * 8 : t / p.segments[0], c0 = narrow ? 0 : (t - r0 * p.segments[0]) * kRangeBatch;
             const int64_t r1 = narrow ? (r0 + 8 < rows ? r0 + 8 : rows) : r0 + 1;
-            const int n = (int)(cols - c0 < kRangeSegment ? cols - c0 : kRangeSegment);
+            const int n = (int)(cols - c0 < kRangeBatch ? cols - c0 : kRangeBatch);
             for (int64_t r = r0; r < r1; r++) {
                 const unsigned short *in = p.p[0] + r * ld + c0;
                 for (int c = lane; c < n; c += 256) {
