@@ -582,23 +582,13 @@ HB_API int helrm_GatedBackward(int device, int dtype, int act, int64_t tokens, i
             d.e.lddh = lddh;
             d.e.vec = 1 | (fits_vectors(dh, lddh) ? 2 : 0);
             if (scaled) {
-                GatedRange r = {};
-                int64_t tasks = 0;
-                Matrix mdh{dh, tokens, width, lddh};
-                // a maximum needs no rows: one long row on 16-byte boundaries, where the pitch leaves nothing out
-                if (lddh == width || tokens == 1) mdh = {dh, 1, tokens * width, pitch(tokens * width)};
-                const Matrix of[4] = {mdh, mx, mg, mu};
-                for (int k = 0; k < 4; k++) {
-                    const Matrix &m = of[k];
-                    r.p[k] = static_cast<const unsigned short *>(m.p);
-                    r.ld[k] = m.ld, r.rows[k] = m.rows, r.cols[k] = m.cols;
-                    r.segments[k] = blocks(m.cols, k ? kRangeSegment : kRangeBatch);
-                    tasks += m.cols <= 256 ? blocks(m.rows, 8) : m.rows * r.segments[k];
-                    r.end[k] = tasks;
-                }
-                r.vec = fits_vectors(dh, mdh.ld);
-                r.part = range;
-                d.e.ranges = blocks(tasks, kRangeWarps) < kRangeBlocks ? (int)blocks(tasks, kRangeWarps) : kRangeBlocks;
+                GatedRange r = {static_cast<const unsigned short *>(dh),
+                                static_cast<const unsigned short *>(mx.p),
+                                {static_cast<const unsigned short *>(mu.p), static_cast<const unsigned short *>(mg.p)},
+                                lddh, mx.ld, {mu.ld, mg.ld}, tokens, width, inner,
+                                fits_vectors(dh, tokens > 1 ? lddh : pitch(width)), range};
+                const int64_t rows = tokens + 2 * width;
+                d.e.ranges = blocks(rows, kRangeWarps) < kRangeBlocks ? (int)blocks(rows, kRangeWarps) : kRangeBlocks;
                 d.e.range = range;
                 d.e.made = unscale;
                 start("gradients' range", k_gated_range, d.e.ranges, kRangeThreads, 0, s, r);

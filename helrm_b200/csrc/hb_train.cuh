@@ -196,136 +196,121 @@ __device__ __forceinline__ void store8(unsigned short *row, int64_t col, int64_t
 // where it does not hold them (dH 6e4, U 4, weights of 1e-2), or holds few of
 // their bits (dH 1e-5, act(G) 1e-2).  So they are scaled by a power of two that
 // brings a bound of both to at least 2^14, below 2^15:
-//   max |dH| max_i |x_i| max(1.13 max_j |wu_j|, max_j |wg_j|)
+//   max_i (max |dH_i| |x_i|) max(1.13 max_j |wu_j|, max_j |wg_j|)
 // with the norms of rows (Cauchy and Schwarz; |act'| <= 1.13, |act(g)| <= |g|).
-// Values down to 2^-28 of the bound keep all their bits.  dH and rows that are not
-// finite have no say.  bf16 has a float's range and no scale.  It reads what the
-// next kernel will read: 64 x 432 x 512 22.6 us without this kernel and 25.1 with
-// it, 2047 x 1001 x 1500 58.6 and 64.9, 4096 x 1024 x 4096 (58 MB, in 16 us) 176
-// and 191.
-// Long rows go in segments (dH's of one batch of loads); a squared norm is at most
-// their number times the largest segment's.  A warp takes a segment, or eight rows of at most 256
-// columns, with its loads in flight together.
-constexpr int kRangeBlocks = 2 * 148, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32, kRangeSegment = 8192, kRangeBatch = 2048;
+// Values down to 2^-28 of the bound keep all their bits.  What is not finite, a
+// value of dH or a row, has no say.  bf16 has a float's range and no scale.
+// The kernel reads what the next one will read: 64 x 432 x 512 21.5 us without it
+// and 23.6 with it, 2047 x 1001 x 1500 58.6 and 65.6, 4096 x 1024 x 4096 (58 MB,
+// in 15 us) 172 and 187.
+constexpr int kRangeBlocks = 2 * 148, kRangeThreads = 512, kRangeWarps = kRangeThreads / 32;
+constexpr int kRangeBatch = 2048;  // columns of a warp's eight 16-byte loads a lane
 struct GatedRange {
-    const unsigned short *p[4];  // dH, x, wg, wu; rows on 16-byte boundaries but for dH's (vec)
-    int64_t ld[4], rows[4], cols[4], segments[4];
-    int64_t end[4];              // tasks of a matrix and those before it
+    const unsigned short *dh, *x, *w[2];  // wu, wg; rows on 16-byte boundaries, but for dh's (vec)
+    int64_t lddh, ldx, ldw[2], tokens, width, inner;
     bool vec;
-    float4 *part;                // a block's max |dH| and largest squared norms
+    float4 *part;  // a block's: (max |dH_i| |x_i|)^2, then |wu_j|^2 and |wg_j|^2
 };
-__device__ __forceinline__ void range_of(unsigned two, bool norm, float &s) {
-    const float2 f = unpack2<__half>(two);
-    const float a = fabsf(f.x), b = fabsf(f.y);
-    s = norm ? fmaf(f.x, f.x, fmaf(f.y, f.y, s)) : fmaxf(s, fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f));
+// A lane's share of a row's sum of squares (NORM) or of its largest finite
+// magnitude, over every step-th batch from the first on.
+template <bool NORM>
+__device__ __forceinline__ float range_of(const unsigned short *row, int64_t n, bool vec, int first, int step) {
+    const int lane = threadIdx.x & 31;
+    float s = 0.0f;
+    auto take = [&](unsigned two) {
+        const float2 f = unpack2<__half>(two);
+        const float a = fabsf(f.x), b = fabsf(f.y);
+        s = NORM ? fmaf(f.x, f.x, fmaf(f.y, f.y, s)) : fmaxf(s, fmaxf(a < INFINITY ? a : 0.0f, b < INFINITY ? b : 0.0f));
+    };
+    for (int64_t b = (int64_t)first * kRangeBatch; b < n; b += (int64_t)step * kRangeBatch) {
+        const unsigned short *in = row + b;
+        const int m = (int)(n - b < kRangeBatch ? n - b : kRangeBatch);
+        if (NORM || vec) {
+            const int whole = m / 8 * 8;
+            uint4 v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int c = lane * 8 + j * 256;
+                v[j] = c < whole ? *reinterpret_cast<const uint4 *>(in + c) : make_uint4(0, 0, 0, 0);
+            }
+            const unsigned short last = whole + lane < m ? in[whole + lane] : (unsigned short)0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) take(v[j].x), take(v[j].y), take(v[j].z), take(v[j].w);
+            take(last);
+        } else {
+            for (int c0 = lane; c0 < m; c0 += 256) {
+                unsigned short v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = c0 + j * 32 < m ? in[c0 + j * 32] : (unsigned short)0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) take(v[j]);
+            }
+        }
+    }
+    return s;
 }
-__device__ __forceinline__ void range_of(uint4 v, bool norm, float &s) {
-    range_of(v.x, norm, s);
-    range_of(v.y, norm, s);
-    range_of(v.z, norm, s);
-    range_of(v.w, norm, s);
+__device__ __forceinline__ float warp_sum(float s) {
+    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    return s;
+}
+__device__ __forceinline__ float warp_max(float s) {
+    for (int o = 16; o; o >>= 1) s = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, o));
+    return s;
 }
 __global__ void __launch_bounds__(kRangeThreads) k_gated_range(const __grid_constant__ GatedRange p) {
     after_previous();
-    __shared__ float red[kRangeWarps][4];
+    __shared__ float red[kRangeWarps][3];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float top[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t i = blockIdx.x * kRangeWarps + warp; i < p.end[3]; i += gridDim.x * kRangeWarps) {
-        const int k = i < p.end[0] ? 0 : i < p.end[1] ? 1 : i < p.end[2] ? 2 : 3;
-        const int64_t rows = p.rows[k], cols = p.cols[k], ld = p.ld[k], t = k ? i - p.end[k - 1] : i;
-        const bool norm = k > 0;
-        float most = 0.0f;
-        auto keep = [&](float s) {
-            for (int o = 16; norm && o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (s < INFINITY) most = fmaxf(most, s);
-        };
-        if (norm || p.vec) {
-            const uint4 none = make_uint4(0, 0, 0, 0);
-            if (cols <= 256) {
-                const unsigned short *in = p.p[k] + t * 8 * ld;
-                const int whole = (int)cols / 8, c = whole * 8 + lane;
-                uint4 v[8];
-                unsigned short last[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const bool on = t * 8 + j < rows;
-                    v[j] = on && lane < whole ? *reinterpret_cast<const uint4 *>(in + j * ld + lane * 8) : none;
-                    last[j] = on && c < cols ? in[j * ld + c] : (unsigned short)0;
-                }
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    float s = 0.0f;
-                    range_of(v[j], norm, s);
-                    range_of(last[j], norm, s);
-                    keep(s);
-                }
-            } else {
-                const unsigned segments = (unsigned)p.segments[k], size = norm ? kRangeSegment : kRangeBatch;
-                const int64_t r = segments == 1 ? t : rows == 1 ? 0 : t / segments, c0 = (t - r * segments) * size;
-                const unsigned short *in = p.p[k] + r * ld + c0;
-                const int n = (int)(cols - c0 < size ? cols - c0 : size), whole = n / 8 * 8;
-                const unsigned short last = whole + lane < n ? in[whole + lane] : (unsigned short)0;
-                float s = 0.0f;
-                for (int c = lane * 8; c < whole; c += kRangeBatch) {
-                    uint4 v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        v[j] = c + j * 256 < whole ? *reinterpret_cast<const uint4 *>(in + c + j * 256) : none;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) range_of(v[j], norm, s);
-                }
-                range_of(last, norm, s);
-                keep(s);
-            }
-        } else {  // dH's rows on any boundary
-            const bool narrow = cols <= 256;
-            const int64_t r0 = narrow ? t * 8 : t / p.segments[0], c0 = narrow ? 0 : (t - r0 * p.segments[0]) * kRangeBatch;
-            const int64_t r1 = narrow ? (r0 + 8 < rows ? r0 + 8 : rows) : r0 + 1;
-            const int n = (int)(cols - c0 < kRangeBatch ? cols - c0 : kRangeBatch);
-            for (int64_t r = r0; r < r1; r++) {
-                const unsigned short *in = p.p[0] + r * ld + c0;
-                for (int c = lane; c < n; c += 256) {
-                    unsigned short v[8];
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = c + j * 32 < n ? in[c + j * 32] : (unsigned short)0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) range_of(v[j], false, most);
-                }
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j == k) top[j] = fmaxf(top[j], most);
+    const int64_t warps = (int64_t)gridDim.x * kRangeWarps, mine = (int64_t)blockIdx.x * kRangeWarps + warp;
+    float top[3] = {0.0f, 0.0f, 0.0f};
+    const bool apart = p.width + p.inner > 8 * kRangeBatch;  // long rows: a token a block
+    for (int64_t r = blockIdx.x; apart && r < p.tokens; r += gridDim.x) {
+        const float d = warp_max(range_of<false>(p.dh + r * p.lddh, p.width, p.vec, warp, kRangeWarps));
+        const float n = warp_sum(range_of<true>(p.x + r * p.ldx, p.inner, true, warp, kRangeWarps));
+        if (lane == 0) red[warp][0] = d, red[warp][1] = n;
+        __syncthreads();
+        const float most = warp_max(lane < kRangeWarps ? red[lane][0] : 0.0f);
+        const float norm = warp_sum(lane < kRangeWarps ? red[lane][1] : 0.0f);
+        __syncthreads();
+        if (norm < INFINITY) top[0] = fmaxf(top[0], most * most * norm);
     }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        for (int o = 16; o; o >>= 1) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
-        if (lane == 0) red[warp][k] = top[k];
+    // a warp a token or a row of weights
+    const int64_t tokens = apart ? 0 : p.tokens;
+    for (int64_t i = mine; i < tokens + 2 * p.width; i += warps) {
+        if (i < tokens) {
+            const float d = range_of<false>(p.dh + i * p.lddh, p.width, p.vec, 0, 1);
+            const float n = range_of<true>(p.x + i * p.ldx, p.inner, true, 0, 1);
+            const float most = warp_max(d), norm = warp_sum(n);
+            if (norm < INFINITY) top[0] = fmaxf(top[0], most * most * norm);
+        } else {
+            const int64_t j = i - tokens;
+            const bool second = j >= p.width;
+            const float norm = warp_sum(
+                range_of<true>(second ? p.w[1] + (j - p.width) * p.ldw[1] : p.w[0] + j * p.ldw[0], p.inner, true, 0, 1));
+            if (norm < INFINITY) (second ? top[2] : top[1]) = fmaxf(second ? top[2] : top[1], norm);
+        }
     }
     __syncthreads();
-    if (threadIdx.x < 4) {
+    if (lane == 0)
+        for (int k = 0; k < 3; k++) red[warp][k] = top[k];  // the same in every lane
+    __syncthreads();
+    if (threadIdx.x < 3) {
         float t = 0.0f;
         for (int i = 0; i < kRangeWarps; i++) t = fmaxf(t, red[i][threadIdx.x]);
-        if (threadIdx.x > 0) t *= (float)p.segments[threadIdx.x];
         reinterpret_cast<float *>(p.part + blockIdx.x)[threadIdx.x] = t;
     }
 }
 // The scale from what n blocks found, in every lane of a warp.
 __device__ __forceinline__ float gated_scale(const float4 *part, int n) {
-    float4 t = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float d = 0.0f, u = 0.0f, g = 0.0f;
 #pragma unroll
     for (int k = 0; k < (kRangeBlocks + 31) / 32; k++) {  // all loads at once
         const int i = 32 * k + (threadIdx.x & 31);
         const float4 v = i < n ? part[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        t = make_float4(fmaxf(t.x, v.x), fmaxf(t.y, v.y), fmaxf(t.z, v.z), fmaxf(t.w, v.w));
+        d = fmaxf(d, v.x), u = fmaxf(u, v.y), g = fmaxf(g, v.z);
     }
-    for (int o = 16; o; o >>= 1) {
-        t.x = fmaxf(t.x, __shfl_xor_sync(0xffffffffu, t.x, o));
-        t.y = fmaxf(t.y, __shfl_xor_sync(0xffffffffu, t.y, o));
-        t.z = fmaxf(t.z, __shfl_xor_sync(0xffffffffu, t.z, o));
-        t.w = fmaxf(t.w, __shfl_xor_sync(0xffffffffu, t.w, o));
-    }
-    const float bound = t.x * sqrtf(t.y) * fmaxf(1.13f * sqrtf(t.w), sqrtf(t.z));  // 2^-75 to 2^80, or 0
+    // 2^-75 to 2^80, or 0
+    const float bound = sqrtf(warp_max(d)) * fmaxf(1.13f * sqrtf(warp_max(u)), sqrtf(warp_max(g)));
     return bound > 0.0f ? __uint_as_float((unsigned)(127 + 14 + 127 - (int)(__float_as_uint(bound) >> 23)) << 23) : 1.0f;
 }
 

@@ -2,7 +2,7 @@
 is outside that type's range and the gradients themselves are inside it.
 
 dG and dU are rounded to 16 bits once, relative to a power of two that brings
-a bound of both, B = max|dH| max(1.13 max|x_i| max|wu_j|, max|x_i| max|wg_j|)
+a bound of both, B = max_i(max|dH_i| |x_i|) max(1.13 max|wu_j|, max|wg_j|)
 (norms of rows), to at least 2^14: a subnormal step of half precision, 2^-24,
 is then at most 2^-38 of B, and rounding to it half of that.
 """
@@ -30,8 +30,8 @@ def grads(dh, x, wg, wu, name):
     dt = dh.dtype
     b = 0.0
     if dt == torch.float16:
-        rows = [t.double().norm(dim=1).max() for t in (x, wg, wu)]
-        b = float(dh.double().abs().max() * rows[0] * torch.maximum(1.13 * rows[2], rows[1]))
+        tokens = (dh.double().abs().max(1).values * x.double().norm(dim=1)).max()
+        b = float(tokens * torch.maximum(1.13 * wu.double().norm(dim=1).max(), wg.double().norm(dim=1).max()))
 
     def once(a):
         return V(a.v, a.e + unit(dt) * a.m + 2.0 ** -39 * 1.01 * b)
@@ -121,3 +121,16 @@ def test_long_rows(tr, shape):
     dt = torch.float16
     check(tr, normal(t, f, std=1000, dtype=dt, seed=1), normal(t, k, std=0.05, dtype=dt, seed=2),
           normal(f, k, std=0.01, dtype=dt, seed=3), normal(f, k, std=1.0, dtype=dt, seed=4), "silu")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+def test_outliers(tr, dt):
+    """Tokens of large dH and tokens of long x, not the same ones: neither takes the others' bits."""
+    dt = DTYPES[dt]
+    t, k, f = 300, 512, 136
+    dh, x = normal(t, f, std=1e-2, dtype=dt, seed=1), normal(t, k, std=0.5, dtype=dt, seed=2)
+    wg, wu = normal(f, k, std=0.02, dtype=dt, seed=3), normal(f, k, std=0.02, dtype=dt, seed=4)
+    dh[::50] = normal(6, f, std=2000, dtype=dt, seed=5)
+    x[7::50, 3] = 2000.0
+    for name in ("identity", "silu"):
+        check(tr, dh, x, wg, wu, name)
