@@ -438,6 +438,8 @@ def vocabulary_loss_backward(dloss, h, w, targets, lse, ignore_index: int = -100
     h, w, t, plan = _loss_call(h, w, targets)
     out_loss, out_lse, out_h, out_w = plan.out
     g, l = _floats(dloss, "dloss", out_loss), _floats(lse, "lse", out_lse)
+    if l.data_ptr() & 7:  # read in pairs
+        l = l.clone()
     dh = out_h.new() if needs[0] else None
     dw = out_w.new() if needs[1] else None
     if any(needs):

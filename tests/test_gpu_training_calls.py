@@ -90,3 +90,19 @@ def test_transforms_without_a_rule_are_refused(tr):
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.float().sum(), leaf)
     torch.cuda.synchronize()
+
+
+def test_statistics_on_any_boundary(tr):
+    """lse and dloss as views that start at an odd element give the same gradients."""
+    h = torch.randn(33, 40, device="cuda", generator=torch.Generator(device="cuda").manual_seed(0)).to(torch.bfloat16)
+    w, t = h.repeat(3, 1), torch.arange(33, device="cuda")
+    loss, lse = tr.vocabulary_loss_forward(h, w, t)
+    want = tr.vocabulary_loss_backward(loss, h, w, t, lse)
+
+    def odd(v):
+        buf = torch.empty(v.numel() + 1, device="cuda")
+        buf[1:] = v.reshape(-1)
+        return buf[1:].view(v.shape)
+    for _ in range(2):
+        got = tr.vocabulary_loss_backward(odd(loss), h, w, t, odd(lse))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
